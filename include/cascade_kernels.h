@@ -287,6 +287,101 @@ int ck_add_rms_norm_stats(const void *x1, const void *x2, const void *gamma, con
                           int dtype, int64_t mode, double eps, void *stream);
 
 /* ============================================================================
+ * Latent attention: K and V of all heads come from one cached row of 576 numbers a
+ * token, 512 of a normed latent c and 64 rotated key dims r. No counterpart in the
+ * reference (its attention ops take K and V per head). dtype is CK_DTYPE_BF16 or
+ * CK_DTYPE_F16, the type of every 16-bit operand of the call; sums, softmax
+ * statistics and norms are fp32. Pages hold 128 tokens: a pool is
+ * [num_blocks, 128, 576] contiguous, token j of request b is row j % 128 of page
+ * block_table[b * bt_cols + j / 128]; a page id outside the pool reads as zero rows.
+ * kv lengths are clamped to [0, bt_cols * 128]. Rows of a page past a length may hold
+ * anything. bt_cols * 128 is at most 2^30 and num_blocks at most 2^31.
+ * ========================================================================== */
+
+/* ----------------------------------------------------------------------------
+ * Writes tokens into the pages: per token t with slot s = slots[t],
+ *   cache[s, 0:512]   = c * rsqrt(mean(c^2) + eps) * gamma     c = kv[t, 0:512]
+ *   cache[s, 512:576] = the 32 pairs (a, b) of kv[t, 512:576] as
+ *                       (a cos - b sin, a sin + b cos); interleaved != 0: pairs
+ *                       (2i, 2i + 1), else (i, i + 32); results keep their places
+ *   kv         [tokens, 576], row stride kv_stride elements (>= 576, a multiple of 8)
+ *   gamma      [512]
+ *   cos_sin    fp32 [max_pos, 64]: 32 cosines, then 32 sines, row positions[t]
+ *   positions, slots  int64 [tokens] on the device; a slot is page * 128 + row. A
+ *              token whose slot is outside [0, num_blocks * 128) or whose position is
+ *              outside [0, max_pos) is not written (-1 pads a batch). Slots that are
+ *              written must be distinct: of two tokens with the same slot either may
+ *              leave each 16-byte piece.
+ * One rounding per value. Other rows of the cache are not touched. eps > 0, finite.
+ * -------------------------------------------------------------------------- */
+int ck_latent_cache_write(const void *kv, int64_t kv_stride, const void *gamma, const float *cos_sin,
+                          int64_t max_pos, const int64_t *positions, const int64_t *slots, void *cache,
+                          int64_t num_blocks, int64_t tokens, int dtype, float eps, int interleaved, void *stream);
+
+/* ----------------------------------------------------------------------------
+ * Absorbed attention over the pages, q_len tokens per request (any number >= 1):
+ * token i, head h of request b, x_j its cache rows:
+ *   s_j = scale * q . x_j,  j < kv_seqlens[b] - q_len + 1 + i  (causal among the
+ *   request's q_len newest tokens, which are in the cache already)
+ *   out = sum_j softmax(s)_j * x_j[0:512],  lse = log sum_j exp(s_j)
+ * A token that sees nothing gets out = 0, lse = -inf.
+ *   q        [batch * q_len, num_heads, 576]: the query's key part multiplied into the
+ *            latent space (512), then its rotated part (64)
+ *   kv_seqlens int64 [batch] on the device, the new tokens included
+ *   out      [batch * q_len, num_heads, 512], dtype
+ *   lse      fp32 [batch * q_len * num_heads]
+ *   workspace  of ck_latent_decode_plan's bytes for kv_cap = bt_cols * 128, 16-byte aligned
+ * P is rounded to dtype before the second product, its sum is not. scale finite, > 0.
+ * -------------------------------------------------------------------------- */
+int ck_latent_decode_plan(int64_t batch, int64_t q_len, int64_t num_heads, int64_t kv_cap,
+                          int64_t *workspace_bytes);
+
+int ck_latent_decode(const void *q, const void *cache, const int32_t *block_table, int64_t bt_cols,
+                     const int64_t *kv_seqlens, int64_t batch, int64_t q_len, int64_t num_heads, int64_t num_blocks,
+                     int64_t block_size, int dtype, float scale, void *out, float *lse, void *workspace,
+                     int64_t workspace_bytes, void *stream);
+
+/* ----------------------------------------------------------------------------
+ * The same for batch single-token queries that share a prefix: each attends to the
+ * prefix (one request: block table [1, prefix_bt_cols], length int64 [1] on the device)
+ * and then to its own suffix. The prefix is read once per 64 (sequence, head) rows; the
+ * parts are folded in fp32. Either may be empty (both: out = 0, lse = -inf); the two
+ * pools may be one. Arguments otherwise as above.
+ * -------------------------------------------------------------------------- */
+int ck_latent_cascade_decode_plan(int64_t batch, int64_t num_heads, int64_t prefix_cap, int64_t suffix_cap,
+                                  int64_t *workspace_bytes);
+
+int ck_latent_cascade_decode(const void *q, const void *prefix_cache, const int32_t *prefix_block_table,
+                             int64_t prefix_bt_cols, const int64_t *prefix_kv_seqlen, int64_t prefix_num_blocks,
+                             const void *suffix_cache, const int32_t *suffix_block_table, int64_t suffix_bt_cols,
+                             const int64_t *suffix_kv_seqlens, int64_t suffix_num_blocks, int64_t batch,
+                             int64_t num_heads, int64_t block_size, int dtype, float scale, void *out, float *lse,
+                             void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ----------------------------------------------------------------------------
+ * Expanded attention for prompts: keys and values of each head are laid out,
+ * requests packed one after another. Query i (head h) of request b, with ql and kl its
+ * lengths, sees the request's keys j < kl, and j <= kl - ql + i when causal:
+ *   s_j = scale * (q[0:128] . k[j, h] + q[128:192] . k_rope[j])
+ *   out = sum_j softmax(s)_j * v[j, h],  lse = log sum_j exp(s_j)
+ *   q        [num_tokens, num_heads, 192] contiguous
+ *   k, v     [num_keys, num_heads, 128]; element strides per token and head (multiples of
+ *            8, at most 2^24; the token stride may be that of a wider row)
+ *   k_rope   [num_keys, 64], token stride kr_stride: shared by the heads
+ *   q_seqlens, kv_seqlens  int64 [batch] on the device; negative counts as 0, and what
+ *            passes num_tokens or num_keys is cut off
+ *   out      [num_tokens, num_heads, 128], dtype; lse fp32 [num_tokens * num_heads]
+ * A query that sees nothing, and every row behind the last request, gets out = 0,
+ * lse = -inf. P is rounded to dtype before the second product, its sum is not.
+ * batch is at most 2^16.
+ * -------------------------------------------------------------------------- */
+int ck_latent_prefill(const void *q, const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                      const void *k_rope, int64_t kr_stride, const void *v, int64_t v_token_stride,
+                      int64_t v_head_stride, const int64_t *q_seqlens, const int64_t *kv_seqlens, int64_t batch,
+                      int64_t num_tokens, int64_t num_keys, int64_t num_heads, int dtype, float scale, int causal,
+                      void *out, float *lse, void *stream);
+
+/* ============================================================================
  * Health counter of the bounded waits inside the suffix and fused cascade
  * kernels (ck_suffix_decode, ck_cascade_decode, ck_cascade_decode_noalloc, and
  * ck_fa_fp32_stage1_decode).

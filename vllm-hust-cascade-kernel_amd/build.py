@@ -26,7 +26,8 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
 
 KERNEL_SOURCES = ["abi.hip", "lse_merge.hip", "fa_stage1.hip", "suffix_decode.hip", "cascade.hip",
-                  "gateup_swiglu.hip", "add_rms_norm.hip", "probe.hip"]
+                  "gateup_swiglu.hip", "add_rms_norm.hip", "latent_cache.hip", "latent_decode.hip",
+                  "latent_prefill.hip", "probe.hip"]
 
 HIP_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc",
@@ -55,6 +56,8 @@ def run(cmd, cwd=None):
 # leading scalar parameters, which kernarg preloading puts in SGPRs at wave
 # launch (kernels whose first parameter is a struct are left as they are).
 SOURCE_FLAGS = {"fa_stage1.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+                "latent_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+                "latent_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                 "suffix_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm", "-amdgpu-kernarg-preload-count=16"]}
 
 
@@ -88,7 +91,7 @@ def build_torch_ops():
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=cascade_torch",
            "-Wno-deprecated-declarations"] + incs + [
-        os.path.join(CSRC, "torch_ops.cpp"), "-o", tmp,
+        os.path.join(CSRC, "torch_ops.cpp"), os.path.join(CSRC, "torch_latent.cpp"), "-o", tmp,
         f"-L{LIBDIR}", "-lcascade_hip", f"-L{tlib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch",
         "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"]
     run(cmd)

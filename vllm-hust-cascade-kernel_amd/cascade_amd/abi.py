@@ -41,6 +41,15 @@ SIGNATURES = {
     "ck_cascade_decode_noalloc": (_int, [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64,
                                          _i64, _i64, _i64, _i64, _i64, _f32, _i64, _i64, _vp, _vp, _vp]),
     "ck_add_rms_norm_stats": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _i64, _f64, _vp]),
+    "ck_latent_cache_write": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _int, _f32, _int, _vp]),
+    "ck_latent_decode_plan": (_int, [_i64, _i64, _i64, _i64, _p64]),
+    "ck_latent_decode": (_int, [_vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _int, _f32, _vp, _vp, _vp,
+                                _i64, _vp]),
+    "ck_latent_cascade_decode_plan": (_int, [_i64, _i64, _i64, _i64, _p64]),
+    "ck_latent_cascade_decode": (_int, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64,
+                                        _int, _f32, _vp, _vp, _vp, _i64, _vp]),
+    "ck_latent_prefill": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
+                                 _int, _f32, _int, _vp, _vp, _vp]),
     "ck_wait_giveups": (_int, [ctypes.POINTER(ctypes.c_uint64), _int]),
     "ck_bw_probe": (_int, [_vp, _vp, _i64, _int, _vp, _i64, _vp]),
     "ck_mfma_probe": (_int, [_i64, _vp, _i64, ctypes.POINTER(ctypes.c_double), _vp]),
@@ -121,4 +130,17 @@ def cascade_plan(batch, num_heads, kv_heads, head_dim, prefix_cap, suffix_cap):
     w = ctypes.c_int64(0)
     check(lib().ck_cascade_decode_plan(batch, num_heads, kv_heads, head_dim, prefix_cap, suffix_cap,
                                        ctypes.byref(w)), "ck_cascade_decode_plan")
+    return w.value
+
+
+def latent_decode_plan(batch, q_len, num_heads, kv_cap):
+    w = ctypes.c_int64(0)
+    check(lib().ck_latent_decode_plan(batch, q_len, num_heads, kv_cap, ctypes.byref(w)), "ck_latent_decode_plan")
+    return w.value
+
+
+def latent_cascade_plan(batch, num_heads, prefix_cap, suffix_cap):
+    w = ctypes.c_int64(0)
+    check(lib().ck_latent_cascade_decode_plan(batch, num_heads, prefix_cap, suffix_cap, ctypes.byref(w)),
+          "ck_latent_cascade_decode_plan")
     return w.value

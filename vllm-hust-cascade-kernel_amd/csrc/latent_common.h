@@ -1,0 +1,67 @@
+// latent_common.h - what the latent-attention kernels share: the 16-bit element types,
+// their matrix products and the sizes of a cache row.
+#pragma once
+
+#include "ck_common.h"
+
+namespace ck {
+namespace lat {
+
+constexpr int kR = 512;          // latent dims: the values, and the first part of every key
+constexpr int kP = 64;           // rotated key dims
+constexpr int kRow = kR + kP;    // a cache row
+constexpr int kRowBytes = kRow * 2;
+constexpr int kPage = 128;       // tokens per page
+constexpr int kPageBytes = kPage * kRowBytes;
+
+// CK_DTYPE_BF16 or CK_DTYPE_F16: conversions (round to nearest even) and the products
+// D = A B + C of 16-bit operands with fp32 sums, fragments as raw 16 bytes per lane.
+template <int DT>
+struct Elem;
+
+template <>
+struct Elem<CK_DTYPE_BF16> {
+    static __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return pack_bf16x2(lo, hi); }
+    static __device__ __forceinline__ float lo(uint32_t w) { return bf16_lo(w); }
+    static __device__ __forceinline__ float hi(uint32_t w) { return bf16_hi(w); }
+    static __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+    // Probabilities enter the second product as 2^kBias p: bf16 has fp32's exponents.
+    static constexpr float kBias = 0.f;
+};
+
+template <>
+struct Elem<CK_DTYPE_F16> {
+    typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8;
+    static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+        typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
+        const f16x2v v = {(_Float16)lo, (_Float16)hi};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+    static __device__ __forceinline__ float lo(uint32_t w) {
+        return (float)__builtin_bit_cast(_Float16, (uint16_t)(w & 0xFFFFu));
+    }
+    static __device__ __forceinline__ float hi(uint32_t w) {
+        return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16));
+    }
+    static __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    }
+    // fp16's normal range ends at 2^-14: 2^7 p keeps all bits of p down to 2^-21, and with
+    // the running maximum at most 2^8 behind (kSlack) stays at or below 2^15 < 65504.
+    static constexpr float kBias = 7.f;
+};
+
+}  // namespace lat
+}  // namespace ck
