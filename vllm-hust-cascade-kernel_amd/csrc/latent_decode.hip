@@ -55,10 +55,14 @@ constexpr int kPhase = 128;  // tiles described in LDS at a time
 constexpr int kGroups = 256; // workgroups: one per CU
 constexpr float kSlack = 8.f;
 
+constexpr int kProducers = 4;  // waves that compute scores; the others own O
+
 constexpr int kLdsP = kSlots * kTileBytes;
 constexpr int kLdsDesc = kLdsP + 2 * kPBytes;
-constexpr int kLdsMax = kLdsDesc + kPhase * 16;  // fp32 [2][64]: row maxima, then row sums
-constexpr int kLdsFlag = kLdsMax + 2 * kRows * 4;
+constexpr int kLdsMax = kLdsDesc + kPhase * 16;      // fp32 [2 token halves][64]: row maxima of a tile
+constexpr int kLdsFac = kLdsMax + 2 * kRows * 4;     // fp32 [64]: what O is scaled by
+constexpr int kLdsSum = kLdsFac + kRows * 4;         // fp32 [2][3][64]: a closing segment's sums and reference points
+constexpr int kLdsFlag = kLdsSum + 2 * 3 * kRows * 4;
 constexpr int kLdsScan = kLdsFlag + 16;
 constexpr int kLds = kLdsScan + 64;
 static_assert(kLds <= 160 * 1024, "LDS");
@@ -118,164 +122,76 @@ __device__ __forceinline__ int64_t clamp_len(int64_t n, const DecodeArgs &a) {
     return n < 0 || a.num_blocks <= 0 ? 0 : n;
 }
 
-template <int DT>
-__global__ __launch_bounds__(kThreads) void latent_decode_kernel(DecodeArgs a) {
+// What a workgroup works on, the same in all its threads but for the thread's requests.
+struct Share {
+    int team, wg;
+    int units;           // prefix units, dealt round-robin
+    int64_t ptiles, unit_tiles;
+    int chunk;           // numbered chunk of the list: tiles [lo, hi)
+    int64_t lo, hi;
+    int b_lo, b_hi;      // this thread's requests
+    int64_t my_start;    // and the list's tiles before them
+};
+
+// One role of a workgroup: the producers compute a tile's scores and P, the consumers move
+// the tiles in and own O. Both walk the same tiles between the same barriers:
+//   interval t: consumers issue tile t + 3; all look at tile t's flag; producers: scores and
+//   P of tile t + 1; consumers: O += of tile t, wait for tile t + 2; barrier
+template <int DT, int NB, bool PRODUCER>
+__device__ __forceinline__ void role_loop(const DecodeArgs &a, const Share &w, CK_LDS char *smem) {
     using E = Elem<DT>;
-    extern __shared__ __attribute__((aligned(16))) char smem_raw[];
-    CK_LDS char *smem = (CK_LDS char *)smem_raw;
     CK_LDS int *desc = (CK_LDS int *)(smem + kLdsDesc);  // {page, item, first token, length}
     CK_LDS float *xmax = (CK_LDS float *)(smem + kLdsMax);
+    CK_LDS float *fac = (CK_LDS float *)(smem + kLdsFac);
     CK_LDS int *flag = (CK_LDS int *)(smem + kLdsFlag);
-    CK_LDS int *scan = (CK_LDS int *)(smem + kLdsScan);
-
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63;
     const int g = lane >> 4, n16 = lane & 15;
-    const int rb = wave & 3, tb = wave >> 2;
 
-    const uint32_t lw = xcd_remap(blockIdx.x, gridDim.x);
-    const int team = lw % a.teams;
-    const int wg = lw / a.teams;
-
-    // ---- the list: this thread's requests, their first tile, the total --------------------
-    const int per = (a.batch + kThreads - 1) / kThreads;
-    const int b_lo = min(tid * per, a.batch), b_hi = min(b_lo + per, a.batch);
-    auto tiles_of = [&](int b) { return (int)((clamp_len(a.lens[b], a) + kTok - 1) / kTok) * a.listed; };
-    int mine = 0;
-    for (int b = b_lo; b < b_hi; ++b) mine += tiles_of(b);
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int up = __shfl_up(incl, o);
-        if (lane >= o) incl += up;
-    }
-    if (lane == 63) scan[wave] = incl;
-    if (tid < 4) flag[tid] = 0;
-    __syncthreads();
-    int my_start = incl - mine, total = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        if (i < wave) my_start += scan[i];
-        total += scan[i];
-    }
-    if (wg == 0 && team == 0) {
-        int at = my_start;
-        for (int b = b_lo; b < b_hi; ++b) {
-            a.sums[b] = at;
-            at += tiles_of(b);
-        }
-        if (tid == 0) a.sums[a.batch] = total;
-    }
-
-    // ---- this workgroup's share ------------------------------------------------------------
-    int64_t ptiles = 0, unit_tiles = 0;
-    int units = 0;
-    if (a.merge) {
-        ptiles = prefix_tiles(a);
-        unit_tiles = (ptiles + a.psplits - 1) / a.psplits;
-        units = ptiles > 0 ? a.pmtiles * a.psplits : 0;
-    }
-    const ListMap map = list_map(total, a.chunks, a.min_tiles, units, unit_tiles);
-    const int chunk = wg < map.ra ? wg : wg - map.ra + map.na;
-    const bool has_list = wg < map.ra ? wg < map.na : wg - map.ra < map.nb;
-    const int64_t lo = has_list ? list_lo(map, chunk) : 0, hi = has_list ? list_lo(map, chunk + 1) : 0;
-
-    // ---- per-lane addresses ------------------------------------------------------------------
-    // DMA piece j of wave w is KB w + 8 j of the tile: LDS chunk L = 64 piece + lane
-    const int pieces = wave < 4 ? 5 : 4;
-    int dma_off[5], dma_row[5];
-#pragma unroll
-    for (int j = 0; j < 5; ++j) {
-        const int l = (wave + 8 * j) * 64 + lane;
-        const int r = l / (kRowBytes / 16), c = l - r * (kRowBytes / 16);
-        dma_row[j] = r;
-        dma_off[j] = r * kRowBytes + ((c & ~7) | ((c ^ swz(r)) & 7)) * 16;
-    }
+    // producer: rows 32 rh .. + 31 (two blocks of 16), tokens 16 tb .. + 15
+    const int rh = wave & 1, tb = (wave >> 1) & 1;
+    u32x4 qf[2][18];
+    f32x4 s[2];
+    float m_own[2], l_part[2];
+    int limit[2];  // tokens that this lane's rows see
     const int krow = 16 * tb + n16;
     const int k_addr = krow * kRowBytes + ((g ^ swz(krow)) & 7) * 16;  // even steps; odd ones ^ 64
-    int v_addr[2];  // db 0; db adds 2 chunks, XORed
+
+    // consumer: value dims 128 cw .. + 127 of all rows, and KB cw + 4 j of every tile
+    const int cw = wave & 3;
+    f32x4 oacc[8][NB];  // [16-dim block][16-row block]
+    int dma_off[9], dma_row[9], v_addr[2];
+    if constexpr (!PRODUCER) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        const int r = 8 * g + 4 * s + (n16 >> 2);
-        v_addr[s] = r * kRowBytes + wave * 128 + ((((n16 >> 1) & 1) ^ swz(r)) << 4) + (n16 & 1) * 8;
+        for (int j = 0; j < 9; ++j) {
+            const int l = (cw + 4 * j) * 64 + lane;  // 16-byte chunk of the tile in LDS
+            const int r = l / (kRowBytes / 16), c = l - r * (kRowBytes / 16);
+            dma_row[j] = r;
+            dma_off[j] = r * kRowBytes + ((c & ~7) | ((c ^ swz(r)) & 7)) * 16;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = 8 * g + 4 * h + (n16 >> 2);
+            v_addr[h] = r * kRowBytes + cw * 256 + ((((n16 >> 1) & 1) ^ swz(r)) << 4) + (n16 & 1) * 8;
+        }
     }
 
-    // ---- state -------------------------------------------------------------------------------
-    u32x4 qf[18];
-    f32x4 oacc[4][4];  // [16-dim block][16-row block]
-    float m_row[4];    // reference points of rows 16 i + n16
-    float l_part = 0.f;
-    int limit = 0;     // tokens that this lane's score row sees
-    int stamp = 0;     // tiles computed, for the flags
-
-    bool began_before = false;  // the segment's item began in an earlier chunk
+    // the segment at hand: both roles, each at its own tile
     int item = -1;
-    int64_t row0 = 0;  // the segment's first row in q, and its rows
-    int rows_n = 0;
+    int64_t row0 = 0;
+    int rows_n = 0, nblk = 0;  // rows, and this wave's 16-row blocks of them
+    bool began_before = false, ends = false, goes_on = false;
+    int parity = 0;  // of the segment, for its sums' place
+    int stamp = 0;   // tiles before this phase's
 
-    // Row sums and factors of the closing segment: inv[i], lse[i] (log2) of rows 16 i + n16.
-    auto finish = [&](float (&inv)[4], float (&lse2)[4]) {
-        float v = l_part + __shfl_xor(l_part, 16);
-        v += __shfl_xor(v, 32);
-        if (g == 0) xmax[tb * kRows + 16 * rb + n16] = v;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float l = xmax[16 * i + n16] + xmax[kRows + 16 * i + n16];
-            // l is 0 where no token was seen (or every score was -inf)
-            inv[i] = l == 0.f ? 0.f : 1.0f / l;
-            lse2[i] = l == 0.f ? -INFINITY : m_row[i] - E::kBias + log2f(l);
-        }
-    };
-    // rows 16 i + n16 < rows_n of this lane to part_o / part_lse
-    auto store_part = [&](float *po, float *pl) {
-        float inv[4], lse2[4];
-        finish(inv, lse2);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = 16 * i + n16;
-            if (row < rows_n) {
-#pragma unroll
-                for (int d = 0; d < 4; ++d)
-                    *reinterpret_cast<f32x4 *>(po + (int64_t)row * kR + 64 * wave + 16 * d + 4 * g) = oacc[d][i] * inv[i];
-                if (wave == 0 && g == 0) pl[row] = lse2[i];
-            }
-        }
-    };
-    auto store_final = [&]() {
-        float inv[4], lse2[4];
-        finish(inv, lse2);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = 16 * i + n16;
-            if (row < rows_n) {
-#pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const f32x4 o = oacc[d][i] * inv[i];
-                    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + (row0 + row) * kR + 64 * wave + 16 * d +
-                                               4 * g) = make_uint2(E::pack2(o[0], o[1]), E::pack2(o[2], o[3]));
-                }
-                if (wave == 0 && g == 0) a.lse[row0 + row] = lse2[i] * kLn2;
-            }
-        }
-    };
-    auto load_rows = [&]() {
-        const int row = 16 * rb + n16;
-#pragma unroll
-        for (int kk = 0; kk < 18; ++kk) {
-            qf[kk] = u32x4{0, 0, 0, 0};
-            if (row < rows_n) qf[kk] = *reinterpret_cast<const u32x4 *>(a.q + (row0 + row) * kRow + 32 * kk + 8 * g);
-        }
-    };
-
-    // ---- the work: prefix units, then the chunk of the list, kPhase tiles at a time -----------
     CK_LDS int *mark = (CK_LDS int *)(smem + kLdsP);  // in P's place: [kPhase] each
     CK_LDS int *seg_item = mark + kPhase, *seg_tile = seg_item + kPhase, *seg_len = seg_tile + kPhase;
-    int unit = wg;
-    int64_t at_prefix = 0, at_list = lo;  // within the unit; in the list
+    int unit = w.wg;
+    int64_t at_prefix = 0, at_list = w.lo;  // within the unit; in the list
     for (;;) {
-        const bool in_prefix = unit < units;
+        // ---- describe the next tiles, at most kPhase: a prefix unit's, then the list's -------
+        const bool in_prefix = unit < w.units;
         int n, sp = 0;
         bool last;
         const char *cache;
@@ -283,7 +199,7 @@ __global__ __launch_bounds__(kThreads) void latent_decode_kernel(DecodeArgs a) {
             // row tiles inner: workgroups side by side read the same prefix tiles
             const int mt = unit % a.pmtiles;
             sp = unit / a.pmtiles;
-            const int64_t p_lo = sp * unit_tiles + at_prefix, p_hi = min((sp + 1) * unit_tiles, ptiles);
+            const int64_t p_lo = sp * w.unit_tiles + at_prefix, p_hi = min((sp + 1) * w.unit_tiles, w.ptiles);
             n = (int)max((int64_t)0, min((int64_t)kPhase, p_hi - p_lo));
             last = p_lo + n >= p_hi;
             cache = reinterpret_cast<const char *>(a.pcache);
@@ -303,15 +219,15 @@ __global__ __launch_bounds__(kThreads) void latent_decode_kernel(DecodeArgs a) {
                 at_prefix = 0;
             }
             if (n == 0) continue;  // past a short prefix's end: the combine counts the splits the same way
-        } else if (at_list < hi) {
+        } else if (at_list < w.hi) {
             const int64_t ph = at_list;
-            n = (int)min((int64_t)kPhase, hi - ph);
-            last = ph + n >= hi;
+            n = (int)min((int64_t)kPhase, w.hi - ph);
+            last = ph + n >= w.hi;
             cache = reinterpret_cast<const char *>(a.cache);
             if (tid < kPhase) mark[tid] = 0;
             __syncthreads();
-            int64_t at = my_start;
-            for (int b = b_lo; b < b_hi && at < ph + n; ++b) {
+            int64_t at = w.my_start;
+            for (int b = w.b_lo; b < w.b_hi && at < ph + n; ++b) {
                 const int64_t len = clamp_len(a.lens[b], a);
                 const int each = (int)((len + kTok - 1) / kTok);
                 for (int m = 0; m < a.listed; ++m, at += each) {
@@ -339,151 +255,354 @@ __global__ __launch_bounds__(kThreads) void latent_decode_kernel(DecodeArgs a) {
                 desc[4 * tid + 2] = tile * kTok;
                 desc[4 * tid + 3] = seg_len[i];
             }
-            at_list += n;
         } else {
             break;
         }
+        if (!in_prefix) at_list += n;
         __syncthreads();
 
-        auto issue = [&](int t) {
-            const int page = __builtin_amdgcn_readfirstlane(desc[4 * t]);
-            const int first = __builtin_amdgcn_readfirstlane(desc[4 * t + 2]);
-            const ck_rsrc_t r = buf_rsrc(cache + (int64_t)max(page, 0) * kPageBytes + ((first / kTok) % kTilesPerPage) * kTileBytes,
-                                         kTileBytes);
-            CK_LDS char *dst = smem + (t & (kSlots - 1)) * kTileBytes + wave * 1024;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) dma16_buf(r, dma_off[j], 0, dst + j * 8192);
-            if (wave < 4) dma16_buf(r, dma_off[4], 0, dst + 4 * 8192);
+        // ---- a tile's item, length and first token; a new item's rows -------------------------
+        int first = 0, len = 0;
+        auto step_to = [&](int t) {  // true where tile t opens a segment
+            const u32x4 d = *reinterpret_cast<const CK_LDS u32x4 *>(desc + 4 * t);
+            const int it = __builtin_amdgcn_readfirstlane(d[1]);
+            first = __builtin_amdgcn_readfirstlane(d[2]);
+            len = __builtin_amdgcn_readfirstlane(d[3]);
+            goes_on = first + kTok < len;
+            ends = !goes_on || (last && t + 1 == n);
+            if (it == item) return false;
+            item = it;
+            began_before = first > 0;
+            if (!in_prefix) {
+                const int b = it / a.listed, first_row = (a.teams > 1 ? w.team : it - b * a.listed) * kRows;
+                row0 = (int64_t)b * a.rows + first_row;
+                rows_n = min(kRows, a.rows - first_row);
+            }
+            return true;
         };
-        // This wave's pieces of tile t are in; rows past the length or of an invalid page
-        // become zeros (0 * V must not be NaN, and an invalid page reads as zeros).
-        auto settle = [&](int t, int younger) {  // younger: tiles in flight behind it
-            if (younger <= 0) wait_vmcnt<0>();
-            else if (younger == 1) wave < 4 ? wait_vmcnt<5>() : wait_vmcnt<4>();
-            else wave < 4 ? wait_vmcnt<10>() : wait_vmcnt<8>();
-            const int page = __builtin_amdgcn_readfirstlane(desc[4 * t]);
-            const int z0 = page < 0 ? 0 : __builtin_amdgcn_readfirstlane(desc[4 * t + 3] - desc[4 * t + 2]);
-            if (z0 < kTok) {
-                CK_LDS char *dst = smem + (t & (kSlots - 1)) * kTileBytes + wave * 1024 + lane * 16;
-#pragma unroll
-                for (int j = 0; j < 5; ++j)
-                    if (j < pieces && dma_row[j] >= z0)
-                        *reinterpret_cast<CK_LDS u32x4 *>(dst + j * 8192) = u32x4{0, 0, 0, 0};
-            }
-        };
-        for (int t = 0; t < 3 && t < n; ++t) issue(t);
-        settle(0, min(n - 1, 2));
-        __syncthreads();
-        for (int t = 0; t < n; ++t) {
-            const int it = __builtin_amdgcn_readfirstlane(desc[4 * t + 1]);
-            const int first = __builtin_amdgcn_readfirstlane(desc[4 * t + 2]);
-            const int len = __builtin_amdgcn_readfirstlane(desc[4 * t + 3]);
-            if (it != item) {
-                item = it;
-                if (in_prefix) {
-                    limit = len;
-                } else {
-                    const int b = it / a.listed, first_row = (a.teams > 1 ? team : it - b * a.listed) * kRows;
-                    row0 = (int64_t)b * a.rows + first_row;
-                    rows_n = min(kRows, a.rows - first_row);
-                    limit = max(0, min(len, len - a.q_len + 1 + (first_row + 16 * rb + n16) / a.heads));
-                }
-                load_rows();
-                began_before = first > 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    m_row[i] = -INFINITY;
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) oacc[d][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-                }
-                l_part = 0.f;
-            }
-            CK_LDS char *tile = smem + (t & (kSlots - 1)) * kTileBytes;
-            f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int kk = 0; kk < 18; ++kk) {
-                const u32x4 kf = *reinterpret_cast<const CK_LDS u32x4 *>(tile + (k_addr ^ ((kk & 1) << 6)) + (kk >> 1) * 128);
-                s = E::mfma16(kf, qf[kk], s);
-            }
-            // lane (g, n): row 16 rb + n, tokens 16 tb + 4 g + r
-            const int tok0 = first + 16 * tb + 4 * g;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[r] = tok0 + r < limit ? s[r] * a.scale_log2 : -INFINITY;
-            const float smax = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-            const float m_own = rb == 0 ? m_row[0] : rb == 1 ? m_row[1] : rb == 2 ? m_row[2] : m_row[3];
-            ++stamp;
-            if (__builtin_amdgcn_ballot_w64(smax > m_own + kSlack) && lane == 0) flag[stamp & 1] = stamp;
-            CK_LDS char *pbuf = smem + kLdsP + (t & 1) * kPBytes;
-            float ls;
-            auto write_p = [&](float m) {
-                const float sub = (m == -INFINITY ? 0.f : m) - E::kBias;
-                float p[4];
-                ls = 0.f;
+
+        if constexpr (PRODUCER) {
+            auto write_p = [&](int t, int i) {
+                const float sub = (m_own[i] == -INFINITY ? 0.f : m_own[i]) - E::kBias;
+                float p[4], ls = 0.f;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    p[r] = exp2_fast(s[r] - sub);
+                    p[r] = exp2_fast(s[i][r] - sub);
                     ls += p[r];
                 }
-                *reinterpret_cast<CK_LDS u32x2 *>(pbuf + (16 * rb + n16) * kPPitch + tb * 32 + g * 8) =
-                    u32x2{E::pack2(p[0], p[1]), E::pack2(p[2], p[3])};
+                *reinterpret_cast<CK_LDS u32x2 *>(smem + kLdsP + (t & 1) * kPBytes + (32 * rh + 16 * i + n16) * kPPitch +
+                                                  tb * 32 + g * 8) = u32x2{E::pack2(p[0], p[1]), E::pack2(p[2], p[3])};
+                return ls;
             };
-            write_p(m_own);
-            if (t + 1 < n) settle(t + 1, t + 2 < n ? 1 : 0);
-            __syncthreads();  // P of tile t and tile t + 1 are in; every wave is done with tile t - 1
-            if (t + 3 < n) issue(t + 3);
-            if (__builtin_amdgcn_readfirstlane(flag[stamp & 1]) == stamp) {  // rare: move the reference points
-                float v = fmaxf(smax, __shfl_xor(smax, 16));
-                v = fmaxf(v, __shfl_xor(v, 32));
-                if (g == 0) xmax[tb * kRows + 16 * rb + n16] = v;
-                __syncthreads();
-                float m_new_own = 0.f, l_scale = 1.f;
+            float l_tile[2] = {0.f, 0.f};  // of tile t, not yet in l_part
+            // scores and P of tile t
+            auto scores = [&](int t) {
+                if (step_to(t)) {
+                    nblk = max(0, min(2, (rows_n + 15) / 16 - 2 * rh));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float mx = fmaxf(xmax[16 * i + n16], xmax[kRows + 16 * i + n16]);
-                    const float m_new = fmaxf(m_row[i], mx);
-                    const float f = m_new == -INFINITY ? 1.f : exp2_fast(m_row[i] - m_new);
-                    m_row[i] = m_new;
+                    for (int i = 0; i < 2; ++i) {
+                        const int row = 32 * rh + 16 * i + n16;
+                        m_own[i] = -INFINITY;
+                        l_part[i] = 0.f;
+                        const int from = (int)(row0 % a.rows);  // of the request
+                        limit[i] = in_prefix ? len : max(0, min(len, len - a.q_len + 1 + (from + row) / a.heads));
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) oacc[d][i] *= f;
-                    if (i == rb) {
-                        m_new_own = m_new;
-                        l_scale = f;
+                        for (int kk = 0; kk < 18; ++kk) {
+                            qf[i][kk] = u32x4{0, 0, 0, 0};
+                            if (row < rows_n)
+                                qf[i][kk] = *reinterpret_cast<const u32x4 *>(a.q + (row0 + row) * kRow + 32 * kk + 8 * g);
+                        }
                     }
                 }
-                l_part *= l_scale;
-                write_p(m_new_own);
+                if (nblk == 0) return;
+                const CK_LDS char *tile = smem + (t & (kSlots - 1)) * kTileBytes;
+                auto kfrag = [&](int kk) {
+                    return *reinterpret_cast<const CK_LDS u32x4 *>(tile + (k_addr ^ ((kk & 1) << 6)) + (kk >> 1) * 128);
+                };
+                constexpr int kAhead = 6;
+                u32x4 kf[kAhead];
+                s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < kAhead; ++kk) kf[kk] = kfrag(kk);
+                __builtin_amdgcn_sched_barrier(0);
+                if (nblk == 2) {
+#pragma unroll
+                    for (int kk = 0; kk < 18; ++kk) {
+                        s[0] = E::mfma16(kf[kk % kAhead], qf[0][kk], s[0]);
+                        s[1] = E::mfma16(kf[kk % kAhead], qf[1][kk], s[1]);
+                        if (kk + kAhead < 18) kf[kk % kAhead] = kfrag(kk + kAhead);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                } else {
+#pragma unroll
+                    for (int kk = 0; kk < 18; ++kk) {  // two chains of products
+                        s[kk & 1] = E::mfma16(kf[kk % kAhead], qf[0][kk], s[kk & 1]);
+                        if (kk + kAhead < 18) kf[kk % kAhead] = kfrag(kk + kAhead);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    s[0] += s[1];
+                }
+                // lane (g, n): row n of block i, tokens 16 tb + 4 g + r
+                const int tok0 = first + 16 * tb + 4 * g;
+                bool moves = false;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (i >= nblk) break;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        s[i][r] = tok0 + r < limit[i] ? s[i][r] * a.scale_log2 : -INFINITY;
+                        moves |= s[i][r] > m_own[i] + kSlack;
+                    }
+                    l_tile[i] = write_p(t, i);
+                }
+                if (__builtin_amdgcn_ballot_w64(moves) && lane == 0) flag[t & 1] = stamp + t + 1;
+            };
+
+            __syncthreads();  // tile 0 is in
+            scores(0);
+            __syncthreads();
+            for (int t = 0; t < n; ++t) {
+                if (__builtin_amdgcn_readfirstlane(flag[t & 1]) == stamp + t + 1) {  // rare: move the reference points
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float v = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
+                        v = fmaxf(v, __shfl_xor(v, 16));
+                        v = fmaxf(v, __shfl_xor(v, 32));
+                        if (g == 0 && i < nblk) xmax[tb * kRows + 32 * rh + 16 * i + n16] = v;
+                    }
+                    __syncthreads();
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (i >= nblk) break;
+                        const int row = 32 * rh + 16 * i + n16;
+                        const float m_new = fmaxf(m_own[i], fmaxf(xmax[row], xmax[kRows + row]));
+                        const float f = m_new == -INFINITY ? 1.f : exp2_fast(m_own[i] - m_new);
+                        m_own[i] = m_new;
+                        l_part[i] *= f;
+                        l_tile[i] = write_p(t, i);
+                        if (tb == 0 && g == 0) fac[row] = f;
+                    }
+                    __syncthreads();
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) l_part[i] += l_tile[i];
+                if (ends) {
+                    CK_LDS float *sums = (CK_LDS float *)(smem + kLdsSum) + parity * 3 * kRows;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float v = l_part[i] + __shfl_xor(l_part[i], 16);
+                        v += __shfl_xor(v, 32);
+                        const int row = 32 * rh + 16 * i + n16;
+                        if (g == 0 && i < nblk) {
+                            sums[tb * kRows + row] = v;
+                            if (tb == 0) sums[2 * kRows + row] = m_own[i];
+                        }
+                    }
+                    parity ^= 1;
+                    item = -1;
+                }
+                if (t + 1 < n) scores(t + 1);
                 __syncthreads();
             }
-            l_part += ls;
-            // O^T += C^T P^T over the tile's 32 tokens
-            u32x4 pf[4];
+        } else {
+            auto issue = [&](int t) {
+                const int page = __builtin_amdgcn_readfirstlane(desc[4 * t]);
+                const int from = __builtin_amdgcn_readfirstlane(desc[4 * t + 2]);
+                const ck_rsrc_t r = buf_rsrc(
+                    cache + (int64_t)max(page, 0) * kPageBytes + ((from / kTok) % kTilesPerPage) * kTileBytes, kTileBytes);
+                CK_LDS char *dst = smem + (t & (kSlots - 1)) * kTileBytes + cw * 1024;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                pf[i] = *reinterpret_cast<const CK_LDS u32x4 *>(pbuf + (16 * i + n16) * kPPitch + g * 16);
+                for (int j = 0; j < 9; ++j) dma16_buf(r, dma_off[j], 0, dst + j * 4096);
+            };
+            // This wave's pieces of tile t are in (`younger` tiles behind it may not be); rows
+            // past the length or of an invalid page become zeros: 0 * V must not be NaN,
+            // and an invalid page reads as zeros.
+            auto settle = [&](int t, int younger) {
+                if (younger <= 0) wait_vmcnt<0>();
+                else if (younger == 1) wait_vmcnt<9>();
+                else if (younger == 2) wait_vmcnt<18>();
+                else wait_vmcnt<27>();
+                const int page = __builtin_amdgcn_readfirstlane(desc[4 * t]);
+                const int z0 = page < 0 ? 0 : __builtin_amdgcn_readfirstlane(desc[4 * t + 3] - desc[4 * t + 2]);
+                if (z0 < kTok) {
+                    CK_LDS char *dst = smem + (t & (kSlots - 1)) * kTileBytes + cw * 1024 + lane * 16;
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                const uint2 v0 = lds_read_tr16(tile + (v_addr[0] ^ (d << 5)));
-                const uint2 v1 = lds_read_tr16(tile + (v_addr[1] ^ (d << 5)));
-                const u32x4 vf = {v0.x, v0.y, v1.x, v1.y};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) oacc[d][i] = E::mfma16(vf, pf[i], oacc[d][i]);
-            }
-            const bool goes_on = first + kTok < len;
-            if (!goes_on || (last && t + 1 == n)) {
-                if (in_prefix) {
-                    store_part(a.ppart_o + (sp * (int64_t)a.prows + row0) * kR, a.ppart_lse + sp * (int64_t)a.prows + row0);
-                } else if (a.merge || began_before || goes_on) {
-                    const int64_t slot = began_before || goes_on ? part_slot(began_before, chunk, a.teams, team)
-                                                                 : (int64_t)2 * a.chunks * a.teams + it;
-                    store_part(a.part_o + slot * a.slot_rows * kR, a.part_lse + slot * a.slot_rows);
-                } else {
-                    store_final();
+                    for (int j = 0; j < 9; ++j)
+                        if (dma_row[j] >= z0) *reinterpret_cast<CK_LDS u32x4 *>(dst + j * 4096) = u32x4{0, 0, 0, 0};
                 }
+            };
+            bool pending = false;  // the segment before tile t's is to be closed
+            // O of the closed segment: to its place in the workspace, or to the result
+            auto close = [&]() {
+                const CK_LDS float *sums = (const CK_LDS float *)(smem + kLdsSum) + parity * 3 * kRows;
+                const bool part = in_prefix || a.merge || began_before || goes_on;
+                float *po = nullptr, *pl = nullptr;
+                if (in_prefix) {
+                    po = a.ppart_o + (sp * (int64_t)a.prows + row0) * kR;
+                    pl = a.ppart_lse + sp * (int64_t)a.prows + row0;
+                } else if (part) {
+                    const int64_t slot = began_before || goes_on ? part_slot(began_before, w.chunk, a.teams, w.team)
+                                                                 : (int64_t)2 * a.chunks * a.teams + item;
+                    po = a.part_o + slot * a.slot_rows * kR;
+                    pl = a.part_lse + slot * a.slot_rows;
+                }
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    const int row = 16 * i + n16;
+                    if (row >= rows_n) continue;
+                    // l is 0 where no token was seen (or every score was -inf)
+                    const float l = sums[row] + sums[kRows + row];
+                    const float inv = l == 0.f ? 0.f : 1.0f / l;
+                    const float lse2 = l == 0.f ? -INFINITY : sums[2 * kRows + row] - E::kBias + log2f(l);
+                    if (part) {
+#pragma unroll
+                        for (int d = 0; d < 8; ++d)
+                            *reinterpret_cast<f32x4 *>(po + (int64_t)row * kR + 128 * cw + 16 * d + 4 * g) = oacc[d][i] * inv;
+                        if (cw == 0 && g == 0) pl[row] = lse2;
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < 8; ++d) {
+                            const f32x4 o = oacc[d][i] * inv;
+                            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + (row0 + row) * kR + 128 * cw +
+                                                       16 * d + 4 * g) = make_uint2(E::pack2(o[0], o[1]), E::pack2(o[2], o[3]));
+                        }
+                        if (cw == 0 && g == 0) a.lse[row0 + row] = lse2 * kLn2;
+                    }
+                }
+                parity ^= 1;
                 item = -1;
+            };
+            // O^T += C^T P^T of tile t
+            auto add = [&](int t) {
+                const CK_LDS char *tile = smem + (t & (kSlots - 1)) * kTileBytes;
+                const CK_LDS char *pbuf = smem + kLdsP + (t & 1) * kPBytes;
+                u32x4 pf[NB];
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+                    pf[i] = *reinterpret_cast<const CK_LDS u32x4 *>(pbuf + (16 * i + n16) * kPPitch + g * 16);
+                auto vfrag = [&](int d) {
+                    const uint2 v0 = lds_read_tr16(tile + (v_addr[0] ^ ((d & 3) << 5)) + (d >> 2) * 128);
+                    const uint2 v1 = lds_read_tr16(tile + (v_addr[1] ^ ((d & 3) << 5)) + (d >> 2) * 128);
+                    return u32x4{v0.x, v0.y, v1.x, v1.y};
+                };
+                constexpr int kAhead = 4;
+                u32x4 vf[kAhead];
+#pragma unroll
+                for (int d = 0; d < kAhead; ++d) vf[d] = vfrag(d);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) oacc[d][i] = E::mfma16(vf[d % kAhead], pf[i], oacc[d][i]);
+                    if (d + kAhead < 8) vf[d % kAhead] = vfrag(d + kAhead);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+
+            for (int t = 0; t < kSlots && t < n; ++t) issue(t);
+            settle(0, min(n - 1, 3));
+            __syncthreads();  // tile 0 is in
+            if (n > 1) settle(1, min(n - 2, 2));
+            __syncthreads();
+            for (int t = 0; t < n; ++t) {
+                if (t > 0 && t + 3 < n) issue(t + 3);
+                bool settled = t + 2 >= n;
+                if (pending) {
+                    // the tile's wait in front of the stores, which are counted with it
+                    if (!settled) settle(t + 2, min(n - 3 - t, 1));
+                    settled = true;
+                    close();
+                    pending = false;
+                }
+                if (step_to(t)) {
+                    nblk = (rows_n + 15) / 16;
+#pragma unroll
+                    for (int d = 0; d < 8; ++d)
+#pragma unroll
+                        for (int i = 0; i < NB; ++i) oacc[d][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+                if (__builtin_amdgcn_readfirstlane(flag[t & 1]) == stamp + t + 1) {
+                    __syncthreads();
+                    __syncthreads();  // the factors are in
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) {
+                        const float f = i < nblk ? fac[16 * i + n16] : 1.f;
+#pragma unroll
+                        for (int d = 0; d < 8; ++d) oacc[d][i] *= f;
+                    }
+                }
+                add(t);
+                if (!settled) settle(t + 2, min(n - 3 - t, 1));
+                pending = ends;
+                __syncthreads();
             }
+            if (pending) close();
         }
-        __syncthreads();  // the tables and the ring are free
+        stamp += n;
     }
+}
+
+// NB: 16-row blocks of the largest row tile
+template <int DT, int NB>
+__global__ __launch_bounds__(kThreads) void latent_decode_kernel(DecodeArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+    CK_LDS char *smem = (CK_LDS char *)smem_raw;
+    CK_LDS int *scan = (CK_LDS int *)(smem + kLdsScan);
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63;
+    Share w;
+    const uint32_t lw = xcd_remap(blockIdx.x, gridDim.x);
+    w.team = lw % a.teams;
+    w.wg = lw / a.teams;
+
+    // ---- the list: this thread's requests, their first tile, the total --------------------
+    const int per = (a.batch + kThreads - 1) / kThreads;
+    w.b_lo = min(tid * per, a.batch);
+    w.b_hi = min(w.b_lo + per, a.batch);
+    auto tiles_of = [&](int b) { return (int)((clamp_len(a.lens[b], a) + kTok - 1) / kTok) * a.listed; };
+    int mine = 0;
+    for (int b = w.b_lo; b < w.b_hi; ++b) mine += tiles_of(b);
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(incl, o);
+        if (lane >= o) incl += up;
+    }
+    if (lane == 63) scan[wave] = incl;
+    if (tid < 2) ((CK_LDS int *)(smem + kLdsFlag))[tid] = 0;
+    __syncthreads();
+    int start = incl - mine, total = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        if (i < wave) start += scan[i];
+        total += scan[i];
+    }
+    w.my_start = start;
+    if (w.wg == 0 && w.team == 0) {
+        for (int b = w.b_lo; b < w.b_hi; ++b) {
+            a.sums[b] = start;
+            start += tiles_of(b);
+        }
+        if (tid == 0) a.sums[a.batch] = total;
+    }
+
+    // ---- this workgroup's share ------------------------------------------------------------
+    w.ptiles = w.unit_tiles = 0;
+    w.units = 0;
+    if (a.merge) {
+        w.ptiles = prefix_tiles(a);
+        w.unit_tiles = (w.ptiles + a.psplits - 1) / a.psplits;
+        w.units = w.ptiles > 0 ? a.pmtiles * a.psplits : 0;
+    }
+    const ListMap map = list_map(total, a.chunks, a.min_tiles, w.units, w.unit_tiles);
+    w.chunk = w.wg < map.ra ? w.wg : w.wg - map.ra + map.na;
+    const bool has_list = w.wg < map.ra ? w.wg < map.na : w.wg - map.ra < map.nb;
+    w.lo = has_list ? list_lo(map, w.chunk) : 0;
+    w.hi = has_list ? list_lo(map, w.chunk + 1) : 0;
+
+    if (wave < kProducers) role_loop<DT, NB, true>(a, w, smem);
+    else role_loop<DT, NB, false>(a, w, smem);
 }
 
 // Folds the parts of every row that has some, in list order and after the prefix's, and
@@ -612,14 +731,20 @@ int make_plan(int64_t batch, int64_t q_len, int64_t heads, int64_t kv_cap, bool 
     return CK_OK;
 }
 
+template <int DT, int NB>
+int launch_decode(const DecodeArgs &a, hipStream_t s) {
+    static std::atomic<uint64_t> lds_set{0};
+    int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(&latent_decode_kernel<DT, NB>), kLds, lds_set);
+    if (rc != CK_OK) return rc;
+    hipLaunchKernelGGL((latent_decode_kernel<DT, NB>), dim3((unsigned)(a.teams * a.chunks)), dim3(kThreads), kLds, s, a);
+    CK_RETURN_LAUNCH();
+}
+
 template <int DT>
 int launch(const DecodeArgs &a, hipStream_t s) {
-    static std::atomic<uint64_t> lds_set{0};
-    int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(&latent_decode_kernel<DT>), kLds, lds_set);
+    const int rows = a.merge ? kRows : a.rows;  // of the largest row tile
+    int rc = rows <= 16 ? launch_decode<DT, 1>(a, s) : rows <= 32 ? launch_decode<DT, 2>(a, s) : launch_decode<DT, 4>(a, s);
     if (rc != CK_OK) return rc;
-    hipLaunchKernelGGL((latent_decode_kernel<DT>), dim3((unsigned)(a.teams * a.chunks)), dim3(kThreads), kLds, s, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return static_cast<int>(e);
     hipLaunchKernelGGL((latent_combine_kernel<DT>), dim3((unsigned)ceil_div((int64_t)a.batch * a.rows, 2)), dim3(256), 0,
                        s, a);
     CK_RETURN_LAUNCH();
