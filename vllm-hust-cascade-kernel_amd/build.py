@@ -11,6 +11,7 @@ link, one g++ invocation for the torch layer.
 import argparse
 import concurrent.futures as cf
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -67,11 +68,35 @@ def compile_hip(src):
     return obj
 
 
+# latent_decode.hip keeps its output accumulators in the accumulation registers, which only
+# its inline assembly names. That is sound as long as the compiler keeps nothing of its own
+# there (it would, were it short of vector registers), so the build looks.
+OWN_ACC_REGISTERS = ["latent_decode.hip"]
+
+
+def check_acc_registers(src):
+    asm = os.path.join(OBJDIR, os.path.splitext(src)[0] + ".s")
+    run([HIPCC] + HIP_FLAGS + SOURCE_FLAGS.get(src, []) + ["--cuda-device-only", "-S", os.path.join(CSRC, src), "-o", asm])
+    inline = False
+    with open(asm) as f:
+        for line in f:
+            code = line.split(";")[0]
+            if "#ASMSTART" in line or "#ASMEND" in line:
+                inline = "#ASMSTART" in line
+            elif not inline and not code.lstrip().startswith(".") and re.search(r"[\s,]a(\d|\[)", code):
+                raise RuntimeError(f"{src}: the compiler uses an accumulation register of its own: {line.strip()}")
+            elif "scratch_" in code:
+                raise RuntimeError(f"{src}: the compiler spills: {line.strip()}")
+
+
 def build_kernels(jobs):
     os.makedirs(OBJDIR, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+        checks = [ex.submit(check_acc_registers, src) for src in OWN_ACC_REGISTERS]
         objs = list(ex.map(compile_hip, KERNEL_SOURCES))
+        for c in checks:
+            c.result()
     out = os.path.join(LIBDIR, "libcascade_hip.so")
     tmp = out + ".tmp"
     run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp] + objs)

@@ -45,33 +45,37 @@ typedef __attribute__((__vector_size__(2 * sizeof(unsigned)))) unsigned u32x2;
 constexpr int kTok = 32;                      // tokens per tile
 constexpr int kTilesPerPage = kPage / kTok;
 constexpr int kTileBytes = kTok * kRowBytes;  // 36864
+// A tile in LDS: 32 rows of the latent, 66 16-byte chunks apart, then 32 of the rotated
+// dims, 8 chunks apart. A 16-byte read is served in groups of 16 lanes that are 8 rows of one
+// chunk and the 8 others of the next one, a transpose read in groups of 8 rows x 2 chunks: with
+// rows 2 bank groups apart both touch every bank group once, without any swizzle (and so with
+// one address register). The rotated dims' rows, which a DMA writes without gaps, are XORed.
+constexpr int kPitch = kR * 2 + 32;
+constexpr int kRopeAt = kTok * kPitch;
+constexpr int kSlotBytes = kRopeAt + kTok * kP * 2;
 constexpr int kSlots = 4;
-constexpr int kRows = 64;   // query rows per workgroup
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;  // 4 waves, one per SIMD, each with all of its 512 registers
+constexpr int kWaveRows = 32;   // query rows per wave, two blocks of 16
+constexpr int kRows = 128;      // query rows per workgroup
 constexpr int kWaves = kThreads / 64;
-constexpr int kPPitch = 80;  // bytes per row of P (32 tokens; odd in 16-byte units, so rows spread over the banks)
-constexpr int kPBytes = kRows * kPPitch;
-constexpr int kPhase = 128;  // tiles described in LDS at a time
-constexpr int kGroups = 256; // workgroups: one per CU
+constexpr int kPieces = 9;    // DMAs per wave and tile: 8 rows of the latent, and their rotated dims
+constexpr int kPhase = 256;   // tiles described in LDS at a time
+constexpr int kGroups = 256;  // workgroups: one per CU
 constexpr float kSlack = 8.f;
 
-constexpr int kProducers = 4;  // waves that compute scores; the others own O
-
-constexpr int kLdsP = kSlots * kTileBytes;
-constexpr int kLdsDesc = kLdsP + 2 * kPBytes;
-constexpr int kLdsMax = kLdsDesc + kPhase * 16;      // fp32 [2 token halves][64]: row maxima of a tile
-constexpr int kLdsFac = kLdsMax + 2 * kRows * 4;     // fp32 [64]: what O is scaled by
-constexpr int kLdsSum = kLdsFac + kRows * 4;         // fp32 [2][3][64]: a closing segment's sums and reference points
-constexpr int kLdsFlag = kLdsSum + 2 * 3 * kRows * 4;
-constexpr int kLdsScan = kLdsFlag + 16;
-constexpr int kLds = kLdsScan + 64;
+constexpr int kLdsZero = kSlots * kSlotBytes;  // a row of zeros
+constexpr int kLdsDesc = kLdsZero + kPitch;
+constexpr int kLdsPlace = kLdsDesc + kPhase * 16;
+constexpr int kLdsScan = kLdsPlace + kPhase * 8;
+constexpr int kLdsStart = kLdsScan + 64;  // each thread's place in the list
+constexpr int kLds = kLdsStart + kThreads * 4;
+static_assert(kPhase == kThreads, "a tile per thread");
 static_assert(kLds <= 160 * 1024, "LDS");
 
-// XOR of a token's 16-byte chunks inside a 128-byte group. A row is 9 such groups, so row r
-// starts in bank half r % 2; with bits 1, 3, 2 of r here, 16 consecutive rows' chunks lie in
-// 16 distinct bank groups (score reads), and so do 4 consecutive rows x 2 chunks of rows
-// r and r + 8 (transpose reads).
-__device__ __forceinline__ int swz(int r) { return ((r & 2) << 1) | ((r >> 2) & 2) | ((r >> 2) & 1); }
+// XOR of the 8 chunks of row r's rotated dims (128 bytes: bit 0 of r is the bank half).
+__device__ __forceinline__ int swz(int r) {
+    return ((r & 2) << 1) | ((((r >> 2) ^ (r >> 3)) & 1) << 1) | ((r >> 3) & 1);
+}
 
 struct DecodeArgs {
     const uint16_t *q;      // [batch * q_len, heads, 576]
@@ -84,8 +88,9 @@ struct DecodeArgs {
     int q_len;
     int heads;
     int rows;     // per request: q_len * heads
-    int teams;    // 64-row tiles of a request given to workgroups of their own
-    int listed;   // 64-row tiles of a request listed one after another (teams == 1)
+    int head_groups;  // 32-row groups of a token's heads, one per wave: its rows see the same tokens
+    int teams;    // row tiles of a request given to workgroups of their own
+    int listed;   // row tiles of a request listed one after another (teams == 1)
     int chunks;   // workgroups per team
     int min_tiles;  // least tiles per chunk
     float scale_log2;
@@ -109,132 +114,254 @@ struct DecodeArgs {
     float *ppart_lse;  // [psplits][prows], log2
 };
 
-__device__ __forceinline__ int64_t prefix_tiles(const DecodeArgs &a) {
-    int64_t n = a.plen[0];
-    const int64_t cap = a.pcols * kPage;
+__device__ __forceinline__ int64_t clamp_len(int64_t n, int64_t cols, int64_t num_blocks) {
+    const int64_t cap = cols * kPage;
     if (n > cap) n = cap;
-    if (n < 0 || a.pblocks <= 0) n = 0;
-    return (n + kTok - 1) / kTok;
+    return n < 0 || num_blocks <= 0 ? 0 : n;
 }
-__device__ __forceinline__ int64_t clamp_len(int64_t n, const DecodeArgs &a) {
-    const int64_t cap = a.bt_cols * kPage;
-    if (n > cap) n = cap;
-    return n < 0 || a.num_blocks <= 0 ? 0 : n;
+__device__ __forceinline__ int64_t prefix_tiles(const int64_t *len, int64_t cols, int64_t num_blocks) {
+    return (clamp_len(*len, cols, num_blocks) + kTok - 1) / kTok;
 }
 
-// What a workgroup works on, the same in all its threads but for the thread's requests.
-struct Share {
-    int team, wg;
-    int units;           // prefix units, dealt round-robin
-    int64_t ptiles, unit_tiles;
-    int chunk;           // numbered chunk of the list: tiles [lo, hi)
-    int64_t lo, hi;
-    int b_lo, b_hi;      // this thread's requests
-    int64_t my_start;    // and the list's tiles before them
-};
+// A value that is the same in all lanes, into scalar registers (divisions leave it in vector ones).
+__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t scalar(int64_t x) {
+    return ((int64_t)scalar((int)(x >> 32)) << 32) | (uint32_t)scalar((int)x);
+}
 
-// One role of a workgroup: the producers compute a tile's scores and P, the consumers move
-// the tiles in and own O. Both walk the same tiles between the same barriers:
-//   interval t: consumers issue tile t + 3; all look at tile t's flag; producers: scores and
-//   P of tile t + 1; consumers: O += of tile t, wait for tile t + 2; barrier
-template <int DT, int NB, bool PRODUCER>
-__device__ __forceinline__ void role_loop(const DecodeArgs &a, const Share &w, CK_LDS char *smem) {
+// The largest of three; a NaN among them is passed over.
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    return r;
+}
+
+// op over the four lanes n, 16 + n, 32 + n, 48 + n, in each of them: exchanging the odd rows of
+// 16 lanes (then the upper half) of x with the even ones (the lower half) of x leaves one
+// operand in each result.
+template <class Op>
+__device__ __forceinline__ float over_groups(float x, Op &&op) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+typedef const __attribute__((address_space(4))) DecodeArgs *KernArgs;
+__device__ __forceinline__ KernArgs args_again(KernArgs a) {
+    asm volatile("" : "+s"(a));
+    return a;
+}
+
+// 16 bytes per lane from r at voff + soff to LDS at base + IMM + 16 * lane, as dma16_buf, with
+// the place in two scalar instructions: they issue in the shadow of a product, where a vector
+// instruction and its trip to the scalar registers would hold the wave up.
+template <int IMM>
+__device__ __forceinline__ void dma_tile(const ck_rsrc_t &r, int voff, int soff, int base) {
+    asm volatile("s_add_i32 m0, %0, %c1\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds"
+                 :
+                 : "s"(base), "i"(IMM), "v"(voff), "s"(r), "s"(soff)
+                 : "memory", "m0", "scc");
+}
+
+// ---- O: the accumulation registers -----------------------------------------------------------
+// O^T of a wave's 32 rows is 512 dims x 32 rows of fp32, all 256 accumulation registers of a
+// lane: block (db, i) of 16 dims x 16 rows is a[8 db + 4 i .. + 3]. The compiler cannot hold
+// values there that vector instructions also touch (it moves them to vector registers, which
+// Q fills), so O is kept out of its sight: only the statements below name these registers. It
+// has no use of its own for them, as long as it spills nothing (the build checks that).
+// acc_ready stands between the last write of an operand and the first product, acc_done
+// between the last product and a read (a product takes 4 passes of 4 cycles).
+constexpr int acc_at(int db, int i) { return 8 * db + 4 * i; }
+
+__device__ __forceinline__ void acc_zero() {
+    static_for<256>([](auto n) __attribute__((always_inline)) { asm volatile("v_accvgpr_write_b32 a%c0, 0" ::"i"(int(n))); });
+    asm volatile("" ::: "a255");  // all of them belong to the kernel
+}
+__device__ __forceinline__ void acc_ready(u32x4 &x, u32x4 &y) { asm volatile("s_nop 7" : "+v"(x), "+v"(y)); }
+__device__ __forceinline__ void acc_done() { asm volatile("s_nop 15\n\ts_nop 15"); }
+template <int DT, int DB, int I>
+__device__ __forceinline__ void acc_mfma(u32x4 a, u32x4 b) {
+    constexpr int n = acc_at(DB, I);
+    if constexpr (DT == CK_DTYPE_BF16)
+        asm volatile("v_mfma_f32_16x16x32_bf16 a[%c0:%c1], %2, %3, a[%c0:%c1]" ::"i"(n), "i"(n + 3), "v"(a), "v"(b));
+    else
+        asm volatile("v_mfma_f32_16x16x32_f16 a[%c0:%c1], %2, %3, a[%c0:%c1]" ::"i"(n), "i"(n + 3), "v"(a), "v"(b));
+}
+template <int N>
+__device__ __forceinline__ float acc_read1() {
+    float x;
+    asm volatile("v_accvgpr_read_b32 %0, a%c1" : "=v"(x) : "i"(N));
+    return x;
+}
+template <int DB, int I>
+__device__ __forceinline__ f32x4 acc_read() {
+    constexpr int n = acc_at(DB, I);
+    return f32x4{acc_read1<n>(), acc_read1<n + 1>(), acc_read1<n + 2>(), acc_read1<n + 3>()};
+}
+// Rows of block i times f_i.
+__device__ __forceinline__ void acc_scale(float f0, float f1) {
+    static_for<256>([&](auto n) __attribute__((always_inline)) {
+        const float x = acc_read1<n>() * ((n / 4) % 2 ? f1 : f0);
+        asm volatile("v_accvgpr_write_b32 a%c0, %1" ::"i"(int(n)), "v"(x));
+    });
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(DecodeArgs) {
     using E = Elem<DT>;
+    // The arguments, read where they are used: held in scalar registers throughout they would
+    // spill, into vector registers that Q and O need.
+    const KernArgs first_args = args_again((KernArgs)__builtin_amdgcn_kernarg_segment_ptr());
+    extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+    CK_LDS char *smem = (CK_LDS char *)smem_raw;
     CK_LDS int *desc = (CK_LDS int *)(smem + kLdsDesc);  // {page, item, first token, length}
-    CK_LDS float *xmax = (CK_LDS float *)(smem + kLdsMax);
-    CK_LDS float *fac = (CK_LDS float *)(smem + kLdsFac);
-    CK_LDS int *flag = (CK_LDS int *)(smem + kLdsFlag);
-    const int tid = threadIdx.x;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int lane = tid & 63;
-    const int g = lane >> 4, n16 = lane & 15;
+    CK_LDS u32x2 *place = (CK_LDS u32x2 *)(smem + kLdsPlace);  // a described tile's bytes into its pool
+    CK_LDS int *scan = (CK_LDS int *)(smem + kLdsScan);
+    CK_LDS int *bad = scan + kWaves;  // the last phase with an invalid page
+    const int wave = scalar((int)threadIdx.x >> 6);
+    const int lane = __lane_id();
+    const int first_tid = 64 * wave + lane;
 
-    // producer: rows 32 rh .. + 31 (two blocks of 16), tokens 16 tb .. + 15
-    const int rh = wave & 1, tb = (wave >> 1) & 1;
-    u32x4 qf[2][18];
-    f32x4 s[2];
-    float m_own[2], l_part[2];
-    int limit[2];  // tokens that this lane's rows see
-    const int krow = 16 * tb + n16;
-    const int k_addr = krow * kRowBytes + ((g ^ swz(krow)) & 7) * 16;  // even steps; odd ones ^ 64
+    const uint32_t lw = xcd_remap(blockIdx.x, gridDim.x);
+    const int wg = scalar((int)(lw / first_args->teams)), team = (int)lw - wg * first_args->teams;
 
-    // consumer: value dims 128 cw .. + 127 of all rows, and KB cw + 4 j of every tile
-    const int cw = wave & 3;
-    f32x4 oacc[8][NB];  // [16-dim block][16-row block]
-    int dma_off[9], dma_row[9], v_addr[2];
-    if constexpr (!PRODUCER) {
+    // ---- the list: this thread's requests, their first tile, the total --------------------
+    auto first_request = [](KernArgs a, int t) {
+        return (int)min((int64_t)t * ((a->batch + kThreads - 1) / kThreads), (int64_t)a->batch);
+    };
+    auto tiles_of = [](KernArgs a, int b) { return (int)((clamp_len(a->lens[b], a->bt_cols, a->num_blocks) + kTok - 1) / kTok); };
+    CK_LDS int *starts = (CK_LDS int *)(smem + kLdsStart);
+    int total = 0;
+    {
+        int mine = 0;
+        for (int b = first_request(first_args, first_tid); b < first_request(first_args, first_tid + 1); ++b) mine += tiles_of(first_args, b) * first_args->listed;
+        int incl = mine;
 #pragma unroll
-        for (int j = 0; j < 9; ++j) {
-            const int l = (cw + 4 * j) * 64 + lane;  // 16-byte chunk of the tile in LDS
-            const int r = l / (kRowBytes / 16), c = l - r * (kRowBytes / 16);
-            dma_row[j] = r;
-            dma_off[j] = r * kRowBytes + ((c & ~7) | ((c ^ swz(r)) & 7)) * 16;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int up = __shfl_up(incl, o);
+            if (lane >= o) incl += up;
         }
+        if (lane == 63) scan[wave] = incl;
+        if (first_tid == 0) *bad = 0;
+        __syncthreads();
+        int start = incl - mine;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = 8 * g + 4 * h + (n16 >> 2);
-            v_addr[h] = r * kRowBytes + cw * 256 + ((((n16 >> 1) & 1) ^ swz(r)) << 4) + (n16 & 1) * 8;
+        for (int i = 0; i < kWaves; ++i) {
+            if (i < wave) start += scan[i];
+            total += scan[i];
         }
+        starts[first_tid] = start;
+        total = scalar(total);
     }
 
-    // the segment at hand: both roles, each at its own tile
-    int item = -1;
-    int64_t row0 = 0;
-    int rows_n = 0, nblk = 0;  // rows, and this wave's 16-row blocks of them
-    bool began_before = false, ends = false, goes_on = false;
-    int parity = 0;  // of the segment, for its sums' place
-    int stamp = 0;   // tiles before this phase's
+    // ---- this workgroup's share ------------------------------------------------------------
+    int64_t ptiles = 0, unit_tiles = 0;
+    int units = 0;
+    if (first_args->merge) {
+        ptiles = scalar(prefix_tiles(first_args->plen, first_args->pcols, first_args->pblocks));
+        unit_tiles = scalar((ptiles + first_args->psplits - 1) / first_args->psplits);
+        units = ptiles > 0 ? first_args->pmtiles * first_args->psplits : 0;
+    }
+    const ListMap map = list_map(total, first_args->chunks, first_args->min_tiles, units, unit_tiles);
+    const int chunk = scalar(wg < map.ra ? wg : wg - map.ra + map.na);
+    const bool has_list = scalar((int)(wg < map.ra ? wg < map.na : wg - map.ra < map.nb));
+    const int64_t lo = has_list ? scalar(list_lo(map, chunk)) : 0, hi = has_list ? scalar(list_lo(map, chunk + 1)) : 0;
 
-    CK_LDS int *mark = (CK_LDS int *)(smem + kLdsP);  // in P's place: [kPhase] each
+    // ---- per-lane addresses ------------------------------------------------------------------
+    for (int i = first_tid; i < kPitch / 4; i += kThreads) ((CK_LDS int *)(smem + kLdsZero))[i] = 0;
+
+    // The lane again, for addresses that are not to be held over the steps: there are no registers
+    // for them beside Q (O has the accumulation registers).
+    struct Lane {
+        int id, g, n16;
+        __device__ __forceinline__ explicit Lane(int l) {
+            asm volatile("" : "+v"(l));
+            id = l;
+            g = l >> 4;
+            n16 = l & 15;
+        }
+    };
+    // Those that are: of a key's latent part and rotated part (first 32 dims; the others ^ 64),
+    // of a value's, and of the DMAs (rows 8 wave .. + 7 of the latent, one each, and their rotated
+    // dims together).
+    const int k_addr = (lane & 15) * kPitch + (lane >> 4) * 16;
+    const int r_addr = kRopeAt + (lane & 15) * (kP * 2) + (((lane >> 4) ^ swz(lane & 15)) & 7) * 16;
+    const int v_row = 4 * (lane >> 4) + ((lane & 15) >> 2), v_addr = v_row * kPitch + (lane & 3) * 8;
+    const int rope_row = 8 * wave + (lane >> 3);
+    const int rope_off = rope_row * kRowBytes + kR * 2 + ((lane & 7) ^ swz(rope_row)) * 16;
+
+    // ---- a segment: an item's tiles in this workgroup -----------------------------------------
+    struct Segment {
+        int64_t row0;  // row i of the wave is row row0 + i of q, i < rows_n
+        int rows_n;
+        int limit;     // tokens that the wave's rows see
+        int item;
+        int began_before;
+    };
+    Segment seg = {0, 0, 0, -1, 0};
+    const float scale_log2 = first_args->scale_log2;
+    u32x4 qf[2][18];
+    float m_row[2], sub[2], l_part[2];  // per row: reference point, what scores are lowered by, sum of p
+
+    CK_LDS int *mark = (CK_LDS int *)smem;  // in the ring's place: [kPhase] each
     CK_LDS int *seg_item = mark + kPhase, *seg_tile = seg_item + kPhase, *seg_len = seg_tile + kPhase;
-    int unit = w.wg;
-    int64_t at_prefix = 0, at_list = w.lo;  // within the unit; in the list
+    int unit = wg, phase = 0;
+    int64_t at_prefix = 0, at_list = lo;  // within the unit; in the list
     for (;;) {
+        const KernArgs a = args_again(first_args);
+        const int tid = 64 * wave + Lane(lane).id;  // again: its places in the tables are not to be held either
         // ---- describe the next tiles, at most kPhase: a prefix unit's, then the list's -------
-        const bool in_prefix = unit < w.units;
+        const bool in_prefix = unit < units;
+        ++phase;
+        auto describe = [&](int page, int64_t blocks, int item, int64_t tile, int len) {
+            const bool ok = page >= 0 && page < blocks;
+            const int64_t at = ok ? (int64_t)page * kPageBytes + (tile % kTilesPerPage) * kTileBytes : 0;
+            *reinterpret_cast<CK_LDS u32x4 *>(desc + 4 * tid) =
+                u32x4{ok ? 1u : 0u, (unsigned)item, (unsigned)(tile * kTok), (unsigned)len};
+            place[tid] = u32x2{(unsigned)at, (unsigned)(at >> 32)};
+            if (!ok) *bad = phase;
+        };
         int n, sp = 0;
+        int64_t prefix_row0 = 0;
         bool last;
         const char *cache;
         if (in_prefix) {
             // row tiles inner: workgroups side by side read the same prefix tiles
-            const int mt = unit % a.pmtiles;
-            sp = unit / a.pmtiles;
-            const int64_t p_lo = sp * w.unit_tiles + at_prefix, p_hi = min((sp + 1) * w.unit_tiles, w.ptiles);
+            sp = scalar(unit / a->pmtiles);
+            const int mt = unit - sp * a->pmtiles;
+            const int64_t p_lo = sp * unit_tiles + at_prefix, p_hi = min((sp + 1) * unit_tiles, ptiles);
             n = (int)max((int64_t)0, min((int64_t)kPhase, p_hi - p_lo));
             last = p_lo + n >= p_hi;
-            cache = reinterpret_cast<const char *>(a.pcache);
-            row0 = (int64_t)mt * kRows;
-            rows_n = (int)min((int64_t)kRows, a.prows - row0);
+            cache = reinterpret_cast<const char *>(a->pcache);
+            prefix_row0 = (int64_t)mt * kRows + kWaveRows * wave;  // rows of all sequences, one after another
             if (tid < n) {
                 const int64_t tile = p_lo + tid;
-                const int page = a.pbt[tile / kTilesPerPage];
-                desc[4 * tid] = page >= 0 && page < a.pblocks ? page : -1;
-                desc[4 * tid + 1] = unit;
-                desc[4 * tid + 2] = (int)(tile * kTok);
-                desc[4 * tid + 3] = (int)min(a.plen[0], a.pcols * kPage);
+                describe(a->pbt[tile / kTilesPerPage], a->pblocks, unit, tile, (int)min(a->plen[0], a->pcols * kPage));
             }
             at_prefix += n;
             if (last) {
-                unit += a.chunks;
+                unit += a->chunks;
                 at_prefix = 0;
             }
             if (n == 0) continue;  // past a short prefix's end: the combine counts the splits the same way
-        } else if (at_list < w.hi) {
+        } else if (at_list < hi) {
             const int64_t ph = at_list;
-            n = (int)min((int64_t)kPhase, w.hi - ph);
-            last = ph + n >= w.hi;
-            cache = reinterpret_cast<const char *>(a.cache);
-            if (tid < kPhase) mark[tid] = 0;
+            n = (int)min((int64_t)kPhase, hi - ph);
+            last = ph + n >= hi;
+            at_list += n;
+            cache = reinterpret_cast<const char *>(a->cache);
+            mark[tid] = 0;
             __syncthreads();
-            int64_t at = w.my_start;
-            for (int b = w.b_lo; b < w.b_hi && at < ph + n; ++b) {
-                const int64_t len = clamp_len(a.lens[b], a);
+            int64_t at = starts[tid];
+            for (int b = first_request(a, tid); b < first_request(a, tid + 1) && at < ph + n; ++b) {
+                const int64_t len = clamp_len(a->lens[b], a->bt_cols, a->num_blocks);
                 const int each = (int)((len + kTok - 1) / kTok);
-                for (int m = 0; m < a.listed; ++m, at += each) {
+                for (int m = 0; m < a->listed; ++m, at += each) {
                     if (each > 0 && at < ph + n && at + each > ph) {
                         const int i = (int)(max(at, ph) - ph);
                         mark[i] = 1;
-                        seg_item[i] = b * a.listed + m;
+                        seg_item[i] = b * a->listed + m;
                         seg_tile[i] = (int)(max(at, ph) - at);
                         seg_len[i] = (int)len;
                     }
@@ -242,367 +369,348 @@ __device__ __forceinline__ void role_loop(const DecodeArgs &a, const Share &w, C
             }
             __syncthreads();
             // the last segment start at or before tile tid
-            const uint64_t lo_mask = __builtin_amdgcn_ballot_w64(mark[lane] != 0);
-            const uint64_t hi_mask = __builtin_amdgcn_ballot_w64(mark[64 + lane] != 0);
+            const Lane l(lane);
+            int i = -1;
+            for (int w = 0; w <= wave; ++w) {
+                uint64_t m = __builtin_amdgcn_ballot_w64(mark[64 * w + l.id] != 0);
+                if (w == wave) m &= ~0ull >> (63 - l.id);
+                if (m) i = 64 * w + 63 - __clzll(m);
+            }
             if (tid < n) {
-                const uint64_t upto = ~0ull >> (63 - lane);
-                const int i = tid < 64 ? 63 - __clzll(lo_mask & upto)
-                              : hi_mask & upto ? 127 - __clzll(hi_mask & upto) : 63 - __clzll(lo_mask);
                 const int it = seg_item[i], tile = seg_tile[i] + tid - i;
-                const int page = a.bt[(int64_t)(it / a.listed) * a.bt_cols + tile / kTilesPerPage];
-                desc[4 * tid] = page >= 0 && page < a.num_blocks ? page : -1;
-                desc[4 * tid + 1] = it;
-                desc[4 * tid + 2] = tile * kTok;
-                desc[4 * tid + 3] = seg_len[i];
+                describe(a->bt[(int64_t)(it / a->listed) * a->bt_cols + tile / kTilesPerPage], a->num_blocks, it, tile,
+                         seg_len[i]);
             }
         } else {
             break;
         }
-        if (!in_prefix) at_list += n;
         __syncthreads();
 
-        // ---- a tile's item, length and first token; a new item's rows -------------------------
-        int first = 0, len = 0;
-        auto step_to = [&](int t) {  // true where tile t opens a segment
-            const u32x4 d = *reinterpret_cast<const CK_LDS u32x4 *>(desc + 4 * t);
-            const int it = __builtin_amdgcn_readfirstlane(d[1]);
-            first = __builtin_amdgcn_readfirstlane(d[2]);
-            len = __builtin_amdgcn_readfirstlane(d[3]);
-            goes_on = first + kTok < len;
-            ends = !goes_on || (last && t + 1 == n);
-            if (it == item) return false;
-            item = it;
-            began_before = first > 0;
-            if (!in_prefix) {
-                const int b = it / a.listed, first_row = (a.teams > 1 ? w.team : it - b * a.listed) * kRows;
-                row0 = (int64_t)b * a.rows + first_row;
-                rows_n = min(kRows, a.rows - first_row);
-            }
-            return true;
+        // ---- the tiles ------------------------------------------------------------------------
+        struct Tile {
+            int ok, item, first, len;  // ok: of a page in the pool
+        };
+        auto tile_at = [&](int t) {  // past the last, it again
+            const u32x4 d = *reinterpret_cast<const CK_LDS u32x4 *>(desc + 4 * min(t, n - 1));
+            return Tile{scalar((int)d[0]), scalar((int)d[1]), scalar((int)d[2]), scalar((int)d[3])};
+        };
+        const bool all_ok = scalar(*bad) != phase;
+        // This wave's moves of tile t into its slot. A resource without bytes moves nothing but
+        // zeros, so that every step issues the same number.
+        struct Moves {
+            ck_rsrc_t r;
+            int base;
+        };
+        auto place_at = [&](int t) { return place[min(t, n - 1)]; };
+        auto moves_of = [&](u32x2 at, int t, bool ok) {
+            const uint64_t from = (uint64_t)(uintptr_t)cache + (((uint64_t)(uint32_t)scalar((int)at[1]) << 32) | (uint32_t)scalar((int)at[0]));
+            Moves m;
+            m.r[0] = (int)(uint32_t)from;
+            m.r[1] = (int)((uint32_t)(from >> 32) & 0xffffu);
+            m.r[2] = t < n && ok ? kTileBytes : 0;
+            m.r[3] = 0x00020000;
+            m.base = scalar((int)(uintptr_t)smem + (t & (kSlots - 1)) * kSlotBytes + 8 * wave * kPitch);
+            return m;
+        };
+        const int rows_at = scalar(8 * wave * kRowBytes);
+        auto move = [&](const Moves &m, auto j) __attribute__((always_inline)) {
+            if constexpr (j < 8) dma_tile<j * kPitch>(m.r, lane * 16, rows_at + j * kRowBytes, m.base);
+            else dma_tile<kRopeAt>(m.r, rope_off, 0, m.base - 8 * wave * kPitch + wave * 1024);
+        };
+        // An invalid page reads as zeros: this wave's part of it, once the DMAs are through.
+        auto blank = [&](int t) {
+            CK_LDS char *dst = smem + (t & (kSlots - 1)) * kSlotBytes + Lane(lane).id * 16;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<CK_LDS u32x4 *>(dst + (8 * wave + j) * kPitch) = u32x4{0, 0, 0, 0};
+            *reinterpret_cast<CK_LDS u32x4 *>(dst + kRopeAt + wave * 1024) = u32x4{0, 0, 0, 0};
         };
 
-        if constexpr (PRODUCER) {
-            auto write_p = [&](int t, int i) {
-                const float sub = (m_own[i] == -INFINITY ? 0.f : m_own[i]) - E::kBias;
-                float p[4], ls = 0.f;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    p[r] = exp2_fast(s[i][r] - sub);
-                    ls += p[r];
-                }
-                *reinterpret_cast<CK_LDS u32x2 *>(smem + kLdsP + (t & 1) * kPBytes + (32 * rh + 16 * i + n16) * kPPitch +
-                                                  tb * 32 + g * 8) = u32x2{E::pack2(p[0], p[1]), E::pack2(p[2], p[3])};
-                return ls;
-            };
-            float l_tile[2] = {0.f, 0.f};  // of tile t, not yet in l_part
-            // scores and P of tile t
-            auto scores = [&](int t) {
-                if (step_to(t)) {
-                    nblk = max(0, min(2, (rows_n + 15) / 16 - 2 * rh));
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int row = 32 * rh + 16 * i + n16;
-                        m_own[i] = -INFINITY;
-                        l_part[i] = 0.f;
-                        const int from = (int)(row0 % a.rows);  // of the request
-                        limit[i] = in_prefix ? len : max(0, min(len, len - a.q_len + 1 + (from + row) / a.heads));
-#pragma unroll
-                        for (int kk = 0; kk < 18; ++kk) {
-                            qf[i][kk] = u32x4{0, 0, 0, 0};
-                            if (row < rows_n)
-                                qf[i][kk] = *reinterpret_cast<const u32x4 *>(a.q + (row0 + row) * kRow + 32 * kk + 8 * g);
-                        }
-                    }
-                }
-                if (nblk == 0) return;
-                const CK_LDS char *tile = smem + (t & (kSlots - 1)) * kTileBytes;
-                auto kfrag = [&](int kk) {
-                    return *reinterpret_cast<const CK_LDS u32x4 *>(tile + (k_addr ^ ((kk & 1) << 6)) + (kk >> 1) * 128);
-                };
-                constexpr int kAhead = 6;
-                u32x4 kf[kAhead];
-                s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kk = 0; kk < kAhead; ++kk) kf[kk] = kfrag(kk);
-                __builtin_amdgcn_sched_barrier(0);
-                if (nblk == 2) {
-#pragma unroll
-                    for (int kk = 0; kk < 18; ++kk) {
-                        s[0] = E::mfma16(kf[kk % kAhead], qf[0][kk], s[0]);
-                        s[1] = E::mfma16(kf[kk % kAhead], qf[1][kk], s[1]);
-                        if (kk + kAhead < 18) kf[kk % kAhead] = kfrag(kk + kAhead);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                } else {
-#pragma unroll
-                    for (int kk = 0; kk < 18; ++kk) {  // two chains of products
-                        s[kk & 1] = E::mfma16(kf[kk % kAhead], qf[0][kk], s[kk & 1]);
-                        if (kk + kAhead < 18) kf[kk % kAhead] = kfrag(kk + kAhead);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                    s[0] += s[1];
-                }
-                // lane (g, n): row n of block i, tokens 16 tb + 4 g + r
-                const int tok0 = first + 16 * tb + 4 * g;
-                bool moves = false;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if (i >= nblk) break;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        s[i][r] = tok0 + r < limit[i] ? s[i][r] * a.scale_log2 : -INFINITY;
-                        moves |= s[i][r] > m_own[i] + kSlack;
-                    }
-                    l_tile[i] = write_p(t, i);
-                }
-                if (__builtin_amdgcn_ballot_w64(moves) && lane == 0) flag[t & 1] = stamp + t + 1;
-            };
-
-            __syncthreads();  // tile 0 is in
-            scores(0);
-            __syncthreads();
-            for (int t = 0; t < n; ++t) {
-                if (__builtin_amdgcn_readfirstlane(flag[t & 1]) == stamp + t + 1) {  // rare: move the reference points
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        float v = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
-                        v = fmaxf(v, __shfl_xor(v, 16));
-                        v = fmaxf(v, __shfl_xor(v, 32));
-                        if (g == 0 && i < nblk) xmax[tb * kRows + 32 * rh + 16 * i + n16] = v;
-                    }
-                    __syncthreads();
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        if (i >= nblk) break;
-                        const int row = 32 * rh + 16 * i + n16;
-                        const float m_new = fmaxf(m_own[i], fmaxf(xmax[row], xmax[kRows + row]));
-                        const float f = m_new == -INFINITY ? 1.f : exp2_fast(m_own[i] - m_new);
-                        m_own[i] = m_new;
-                        l_part[i] *= f;
-                        l_tile[i] = write_p(t, i);
-                        if (tb == 0 && g == 0) fac[row] = f;
-                    }
-                    __syncthreads();
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i) l_part[i] += l_tile[i];
-                if (ends) {
-                    CK_LDS float *sums = (CK_LDS float *)(smem + kLdsSum) + parity * 3 * kRows;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        float v = l_part[i] + __shfl_xor(l_part[i], 16);
-                        v += __shfl_xor(v, 32);
-                        const int row = 32 * rh + 16 * i + n16;
-                        if (g == 0 && i < nblk) {
-                            sums[tb * kRows + row] = v;
-                            if (tb == 0) sums[2 * kRows + row] = m_own[i];
-                        }
-                    }
-                    parity ^= 1;
-                    item = -1;
-                }
-                if (t + 1 < n) scores(t + 1);
-                __syncthreads();
+        // The segment that tile d begins or goes on with.
+        auto segment_of = [&](const Tile &d) {
+            const KernArgs a = args_again(first_args);
+            Segment x = {prefix_row0, 0, d.len, d.item, d.first > 0};
+            if (in_prefix) {
+                x.rows_n = (int)max((int64_t)0, min((int64_t)kWaveRows, a->prows - prefix_row0));
+                if (x.rows_n == 0) x.row0 = 0;
+                return x;
             }
-        } else {
-            auto issue = [&](int t) {
-                const int page = __builtin_amdgcn_readfirstlane(desc[4 * t]);
-                const int from = __builtin_amdgcn_readfirstlane(desc[4 * t + 2]);
-                const ck_rsrc_t r = buf_rsrc(
-                    cache + (int64_t)max(page, 0) * kPageBytes + ((from / kTok) % kTilesPerPage) * kTileBytes, kTileBytes);
-                CK_LDS char *dst = smem + (t & (kSlots - 1)) * kTileBytes + cw * 1024;
+            const int b = scalar(d.item / a->listed);
+            const int group = (a->teams > 1 ? team : d.item - b * a->listed) * 4 + wave;  // of the request
+            const int tok = scalar(group / a->head_groups), head = kWaveRows * (group - tok * a->head_groups);
+            x.rows_n = tok < a->q_len ? min(kWaveRows, a->heads - head) : 0;
+            x.row0 = x.rows_n > 0 ? ((int64_t)b * a->q_len + tok) * a->heads + head : 0;
+            x.limit = max(0, min(d.len, d.len - a->q_len + 1 + tok));
+            return x;
+        };
+        auto load_q = [&](const Segment &x) {  // a row past the last repeats it: it is not stored
+            const KernArgs a = args_again(first_args);
+            const Lane l(lane);
 #pragma unroll
-                for (int j = 0; j < 9; ++j) dma16_buf(r, dma_off[j], 0, dst + j * 4096);
+            for (int i = 0; i < 2; ++i) {
+                const uint16_t *q = a->q + (x.row0 + min(16 * i + l.n16, max(0, x.rows_n - 1))) * kRow + 8 * l.g;
+#pragma unroll
+                for (int kk = 0; kk < 18; ++kk) qf[i][kk] = *reinterpret_cast<const u32x4 *>(q + 32 * kk);
+            }
+        };
+        auto start = [&]() {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                m_row[i] = -INFINITY;
+                sub[i] = -E::kBias;
+                l_part[i] = 0.f;
+            }
+            acc_zero();
+        };
+
+        // S^T = X Q^T of tile t: tokens 4 g + r and 16 + 4 g + r of rows n16 and 16 + n16.
+        // between(f) is placed after the f-th pair of products: what fits in their shadow.
+        f32x4 s[2][2];  // [16 tokens][16 rows]
+        float v[2];     // the rows' largest score in the lane
+        auto scores = [&](int t, f32x4 (&x)[2][2], auto &&between) __attribute__((always_inline)) {
+            const CK_LDS char *tile = smem + (t & (kSlots - 1)) * kSlotBytes;
+            auto kfrag = [&](int f) {
+                const int kk = f >> 1;
+                const CK_LDS char *at = kk < 16 ? tile + k_addr + kk * 64 + (f & 1) * 16 * kPitch
+                                                : tile + (r_addr ^ ((kk & 1) << 6)) + (f & 1) * 16 * kP * 2;
+                return *reinterpret_cast<const CK_LDS u32x4 *>(at);
             };
-            // This wave's pieces of tile t are in (`younger` tiles behind it may not be); rows
-            // past the length or of an invalid page become zeros: 0 * V must not be NaN,
-            // and an invalid page reads as zeros.
-            auto settle = [&](int t, int younger) {
-                if (younger <= 0) wait_vmcnt<0>();
-                else if (younger == 1) wait_vmcnt<9>();
-                else if (younger == 2) wait_vmcnt<18>();
-                else wait_vmcnt<27>();
-                const int page = __builtin_amdgcn_readfirstlane(desc[4 * t]);
-                const int z0 = page < 0 ? 0 : __builtin_amdgcn_readfirstlane(desc[4 * t + 3] - desc[4 * t + 2]);
-                if (z0 < kTok) {
-                    CK_LDS char *dst = smem + (t & (kSlots - 1)) * kTileBytes + cw * 1024 + lane * 16;
+            constexpr int kAhead = 4;
+            u32x4 kf[kAhead];
 #pragma unroll
-                    for (int j = 0; j < 9; ++j)
-                        if (dma_row[j] >= z0) *reinterpret_cast<CK_LDS u32x4 *>(dst + j * 4096) = u32x4{0, 0, 0, 0};
+            for (int f = 0; f < 4; ++f) x[f >> 1][f & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int f = 0; f < kAhead; ++f) kf[f] = kfrag(f);
+            __builtin_amdgcn_sched_barrier(0);
+            static_for<36>([&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) x[f & 1][i] = E::mfma16(kf[f % kAhead], qf[i][f >> 1], x[f & 1][i]);
+                if (f + kAhead < 36) kf[f % kAhead] = kfrag(f + kAhead);
+                between(f);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+        auto hide = [&](int sees) {  // scores of tokens that the rows do not see
+            if (sees < kTok) {
+                const Lane l(lane);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (16 * h + 4 * l.g + r >= sees) s[h][0][r] = s[h][1][r] = -INFINITY;
+            }
+        };
+        auto largest = [&](const f32x4 (&x)[2][2], int i) {
+            v[i] = max3(max3(max3(x[0][i][0], x[0][i][1], x[0][i][2]), x[0][i][3], x[1][i][0]), x[1][i][1],
+                        fmaxf(x[1][i][2], x[1][i][3])) * scale_log2;
+        };
+        auto nothing = [](int) {};
+        // Whether a score passes its row's reference point by more than 2^kSlack.
+        auto moves = [&]() {
+            return __builtin_amdgcn_ballot_w64(v[0] > m_row[0] + kSlack || v[1] > m_row[1] + kSlack) != 0;
+        };
+        u32x4 pf[2];  // P^T of a tile: the scores' token order is the operand's
+        auto p_of = [&](int e) __attribute__((always_inline)) {  // two of the lane's 16 probabilities
+            const int i = e / 4, h = e / 2 % 2, r = e % 2;
+            const float p0 = exp2_fast(fmaf(s[h][i][2 * r], scale_log2, -sub[i]));
+            const float p1 = exp2_fast(fmaf(s[h][i][2 * r + 1], scale_log2, -sub[i]));
+            l_part[i] += p0;
+            l_part[i] += p1;
+            pf[i][2 * h + r] = E::pack2(p0, p1);
+        };
+        // O^T += C^T P^T of a tile whose rows 4 g + n16 / 4 (+ 16) are at v0 (v1).
+        auto products = [&](const CK_LDS char *v0, const CK_LDS char *v1, auto &&between) __attribute__((always_inline)) {
+            auto vfrag = [&](int db) {
+                const uint2 x = lds_read_tr16(v0 + db * 32), y = lds_read_tr16(v1 + db * 32);
+                return u32x4{x.x, x.y, y.x, y.y};
+            };
+            constexpr int kAhead = 4;
+            u32x4 vf[kAhead];
+#pragma unroll
+            for (int db = 0; db < kAhead; ++db) vf[db] = vfrag(db);
+            __builtin_amdgcn_sched_barrier(0);
+            acc_ready(pf[0], pf[1]);
+            static_for<32>([&](auto db) __attribute__((always_inline)) {
+                acc_mfma<DT, db, 0>(vf[db % kAhead], pf[0]);
+                acc_mfma<DT, db, 1>(vf[db % kAhead], pf[1]);
+                if (db + kAhead < 32) vf[db % kAhead] = vfrag(db + kAhead);
+                between(db);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+
+        // ---- the phase's first tiles ------------------------------------------------------------
+        for (int t = 0; t < 3; ++t) {
+            const Moves m = moves_of(place_at(t), t, tile_at(t).ok);
+            static_for<kPieces>([&](auto j) __attribute__((always_inline)) { move(m, j); });
+        }
+        {
+            const Tile d = tile_at(0);
+            if (d.item != seg.item) {
+                seg = segment_of(d);
+                start();
+            }
+            load_q(seg);  // in each phase, so that it is not held while the tiles are described
+            wait_vmcnt<0>();
+            if (!d.ok) blank(0);
+            __syncthreads();
+            if (seg.rows_n > 0) {
+                scores(0, s, nothing);
+                hide(seg.limit - d.first);
+                largest(s, 0);
+                largest(s, 1);
+            }
+        }
+        bool stored = false;  // the last step ended with 32 stores of this wave or more
+        for (int t = 0; t < n; ++t) {
+            // ---- a step in general ----------------------------------------------------------------
+            // Tile t + 1 is in, in every wave; tile t + 3 takes the place of tile t - 1. The scores
+            // of tile t are there.
+            const Tile d0 = tile_at(t), d1 = tile_at(t + 1);
+            if (stored) wait_vmcnt<kPieces + 32>();
+            else wait_vmcnt<kPieces>();
+            if (!d1.ok) blank(t + 1);
+            __syncthreads();
+            stored = false;
+            const bool goes_on = d0.first + kTok < d0.len;
+            const bool ends = !goes_on || (last && t + 1 == n);
+            const bool carries = !ends && t + 1 < n;  // tile t + 1 is the segment's too
+            const bool opens = ends && t + 1 < n;     // tile t + 1 opens another
+            Segment next = seg;
+            if (opens) {  // Q's registers are free since the scores of tile t
+                next = segment_of(d1);
+                load_q(next);
+            }
+            if (seg.rows_n > 0) {
+                if (moves()) {
+                    float scale[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float m_new = fmaxf(m_row[i], over_groups(v[i], [](float x, float y) { return fmaxf(x, y); }));
+                        scale[i] = m_new == -INFINITY ? 1.f : exp2_fast(m_row[i] - m_new);
+                        m_row[i] = m_new;
+                        sub[i] = (m_new == -INFINITY ? 0.f : m_new) - E::kBias;
+                        l_part[i] *= scale[i];
+                    }
+                    acc_scale(scale[0], scale[1]);
                 }
-            };
-            bool pending = false;  // the segment before tile t's is to be closed
-            // O of the closed segment: to its place in the workspace, or to the result
-            auto close = [&]() {
-                const CK_LDS float *sums = (const CK_LDS float *)(smem + kLdsSum) + parity * 3 * kRows;
-                const bool part = in_prefix || a.merge || began_before || goes_on;
-                float *po = nullptr, *pl = nullptr;
+                static_for<8>([&](auto e) __attribute__((always_inline)) { p_of(e); });
+                // Tokens that the rows do not see (past the length they may hold anything) are read
+                // as zeros: 0 * inf must not reach O.
+                const int sees = seg.limit - d0.first;
+                const CK_LDS char *at = smem + (t & (kSlots - 1)) * kSlotBytes + v_addr;
+                products(v_row < sees ? at : smem + kLdsZero, v_row + 16 < sees ? at + 16 * kPitch : smem + kLdsZero, nothing);
+            }
+            // Q, and tile t + 2: before the moves and stores below. Whether the step opens a segment
+            // or not: at Q's use in the plain steps the compiler would wait otherwise.
+            wait_vmcnt<0>();
+            {
+                const Moves m = moves_of(place_at(t + 3), t + 3, tile_at(t + 3).ok);
+                static_for<kPieces>([&](auto j) __attribute__((always_inline)) { move(m, j); });
+            }
+            if (carries && seg.rows_n > 0) {
+                scores(t + 1, s, nothing);
+                hide(seg.limit - d1.first);
+                largest(s, 0);
+                largest(s, 1);
+            }
+
+            // ---- the segment's end ------------------------------------------------------------------
+            if (ends) {
+                const KernArgs a = args_again(first_args);
+                float *po = nullptr, *pl = nullptr;  // the wave's first row of its part
                 if (in_prefix) {
-                    po = a.ppart_o + (sp * (int64_t)a.prows + row0) * kR;
-                    pl = a.ppart_lse + sp * (int64_t)a.prows + row0;
-                } else if (part) {
-                    const int64_t slot = began_before || goes_on ? part_slot(began_before, w.chunk, a.teams, w.team)
-                                                                 : (int64_t)2 * a.chunks * a.teams + item;
-                    po = a.part_o + slot * a.slot_rows * kR;
-                    pl = a.part_lse + slot * a.slot_rows;
+                    po = a->ppart_o + (sp * (int64_t)a->prows + seg.row0) * kR;
+                    pl = a->ppart_lse + sp * (int64_t)a->prows + seg.row0;
+                } else if (a->merge || seg.began_before || goes_on) {
+                    const int64_t slot = seg.began_before || goes_on ? part_slot(seg.began_before, chunk, a->teams, team)
+                                                                     : (int64_t)2 * a->chunks * a->teams + seg.item;
+                    po = a->part_o + (slot * a->slot_rows + kWaveRows * wave) * kR;
+                    pl = a->part_lse + slot * a->slot_rows + kWaveRows * wave;
                 }
-#pragma unroll
-                for (int i = 0; i < NB; ++i) {
-                    const int row = 16 * i + n16;
-                    if (row >= rows_n) continue;
-                    // l is 0 where no token was seen (or every score was -inf)
-                    const float l = sums[row] + sums[kRows + row];
-                    const float inv = l == 0.f ? 0.f : 1.0f / l;
-                    const float lse2 = l == 0.f ? -INFINITY : sums[2 * kRows + row] - E::kBias + log2f(l);
-                    if (part) {
-#pragma unroll
-                        for (int d = 0; d < 8; ++d)
-                            *reinterpret_cast<f32x4 *>(po + (int64_t)row * kR + 128 * cw + 16 * d + 4 * g) = oacc[d][i] * inv;
-                        if (cw == 0 && g == 0) pl[row] = lse2;
+                const Lane l(lane);
+                acc_done();
+                static_for<2>([&](auto i) __attribute__((always_inline)) {
+                    const float sum = over_groups(l_part[i], [](float x, float y) { return x + y; });
+                    // 0 where no token was seen (or every score was -inf)
+                    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+                    const float lse2 = sum == 0.f ? -INFINITY : m_row[i] - E::kBias + log2f(sum);
+                    const int row = 16 * i + l.n16;
+                    if (row >= seg.rows_n) return;
+                    if (po != nullptr) {
+                        float *o = po + row * kR + 4 * l.g;
+                        static_for<32>([&](auto db) __attribute__((always_inline)) {
+                            *reinterpret_cast<f32x4 *>(o + 16 * db) = acc_read<db, i>() * inv;
+                        });
+                        if (l.g == 0) pl[row] = lse2;
                     } else {
-#pragma unroll
-                        for (int d = 0; d < 8; ++d) {
-                            const f32x4 o = oacc[d][i] * inv;
-                            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + (row0 + row) * kR + 128 * cw +
-                                                       16 * d + 4 * g) = make_uint2(E::pack2(o[0], o[1]), E::pack2(o[2], o[3]));
-                        }
-                        if (cw == 0 && g == 0) a.lse[row0 + row] = lse2 * kLn2;
+                        uint16_t *out = static_cast<uint16_t *>(a->out) + (seg.row0 + row) * kR + 4 * l.g;
+                        static_for<32>([&](auto db) __attribute__((always_inline)) {
+                            const f32x4 o = acc_read<db, i>() * inv;
+                            *reinterpret_cast<uint2 *>(out + 16 * db) = make_uint2(E::pack2(o[0], o[1]), E::pack2(o[2], o[3]));
+                        });
+                        if (l.g == 0) a->lse[seg.row0 + row] = lse2 * kLn2;
+                    }
+                });
+                stored = seg.rows_n > 0;
+                seg.item = -1;
+                if (opens) {
+                    seg = next;
+                    start();
+                    if (seg.rows_n > 0) {
+                        scores(t + 1, s, nothing);
+                        hide(seg.limit - d1.first);
+                        largest(s, 0);
+                        largest(s, 1);
                     }
                 }
-                parity ^= 1;
-                item = -1;
-            };
-            // O^T += C^T P^T of tile t
-            auto add = [&](int t) {
-                const CK_LDS char *tile = smem + (t & (kSlots - 1)) * kTileBytes;
-                const CK_LDS char *pbuf = smem + kLdsP + (t & 1) * kPBytes;
-                u32x4 pf[NB];
-#pragma unroll
-                for (int i = 0; i < NB; ++i)
-                    pf[i] = *reinterpret_cast<const CK_LDS u32x4 *>(pbuf + (16 * i + n16) * kPPitch + g * 16);
-                auto vfrag = [&](int d) {
-                    const uint2 v0 = lds_read_tr16(tile + (v_addr[0] ^ ((d & 3) << 5)) + (d >> 2) * 128);
-                    const uint2 v1 = lds_read_tr16(tile + (v_addr[1] ^ ((d & 3) << 5)) + (d >> 2) * 128);
-                    return u32x4{v0.x, v0.y, v1.x, v1.y};
-                };
-                constexpr int kAhead = 4;
-                u32x4 vf[kAhead];
-#pragma unroll
-                for (int d = 0; d < kAhead; ++d) vf[d] = vfrag(d);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int d = 0; d < 8; ++d) {
-#pragma unroll
-                    for (int i = 0; i < NB; ++i) oacc[d][i] = E::mfma16(vf[d % kAhead], pf[i], oacc[d][i]);
-                    if (d + kAhead < 8) vf[d % kAhead] = vfrag(d + kAhead);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            };
-
-            for (int t = 0; t < kSlots && t < n; ++t) issue(t);
-            settle(0, min(n - 1, 3));
-            __syncthreads();  // tile 0 is in
-            if (n > 1) settle(1, min(n - 2, 2));
-            __syncthreads();
-            for (int t = 0; t < n; ++t) {
-                if (t > 0 && t + 3 < n) issue(t + 3);
-                bool settled = t + 2 >= n;
-                if (pending) {
-                    // the tile's wait in front of the stores, which are counted with it
-                    if (!settled) settle(t + 2, min(n - 3 - t, 1));
-                    settled = true;
-                    close();
-                    pending = false;
-                }
-                if (step_to(t)) {
-                    nblk = (rows_n + 15) / 16;
-#pragma unroll
-                    for (int d = 0; d < 8; ++d)
-#pragma unroll
-                        for (int i = 0; i < NB; ++i) oacc[d][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-                }
-                if (__builtin_amdgcn_readfirstlane(flag[t & 1]) == stamp + t + 1) {
-                    __syncthreads();
-                    __syncthreads();  // the factors are in
-#pragma unroll
-                    for (int i = 0; i < NB; ++i) {
-                        const float f = i < nblk ? fac[16 * i + n16] : 1.f;
-#pragma unroll
-                        for (int d = 0; d < 8; ++d) oacc[d][i] *= f;
-                    }
-                }
-                add(t);
-                if (!settled) settle(t + 2, min(n - 3 - t, 1));
-                pending = ends;
-                __syncthreads();
             }
-            if (pending) close();
+
+            // ---- plain steps: whole tiles of one segment, no reference point moves ---------------------
+            // One run of code without branches (one between products costs as much as two of them),
+            // and as few other instructions as the products' shadow holds: alone on its SIMD, a
+            // wave issues one in four cycles, three beside each product. P of tile t is made and tile
+            // t + 3 is moved beside the scores of tile t + 1, the largest of those is taken
+            // beside the products of tile t.
+            if (!carries || stored || seg.rows_n == 0 || !all_ok || moves()) continue;
+            // the last step whose tile and next are seen whole
+            const int end = min(n - 1, t + 1 + max(0, (seg.limit - d1.first) / kTok - 1));
+            bool moved = false;
+            while (t + 1 < end && !moved) {
+                ++t;
+                const u32x2 at3 = place_at(t + 3);
+                wait_vmcnt<kPieces>();
+                __syncthreads();
+                f32x4 s2[2][2];
+                Moves m;
+                scores(t + 1, s2, [&](auto f) __attribute__((always_inline)) {
+                    if constexpr (f == 0) m = moves_of(at3, t + 3, true);
+                    if constexpr (f >= 4 && f < 31 && f % 3 == 1) move(m, std::integral_constant<int, f / 3 - 1>{});
+                    if constexpr (f >= 2 && f < 34 && f % 4 == 2) p_of((f - 2) / 4);
+                });
+                const CK_LDS char *tile = smem + (t & (kSlots - 1)) * kSlotBytes + v_addr;
+                products(tile, tile + 16 * kPitch, [&](auto db) __attribute__((always_inline)) {
+                    if constexpr (db == 4) largest(s2, 0);
+                    if constexpr (db == 8) largest(s2, 1);
+                    if constexpr (db == 12) moved = moves();
+                    if constexpr (db >= 16 && db < 20) s[(db - 16) / 2][db % 2] = s2[(db - 16) / 2][db % 2];
+                });
+            }
         }
-        stamp += n;
+        wait_vmcnt<0>();  // the empty moves too
+        __syncthreads();  // the tables and the ring are free
     }
-}
 
-// NB: 16-row blocks of the largest row tile
-template <int DT, int NB>
-__global__ __launch_bounds__(kThreads) void latent_decode_kernel(DecodeArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char smem_raw[];
-    CK_LDS char *smem = (CK_LDS char *)smem_raw;
-    CK_LDS int *scan = (CK_LDS int *)(smem + kLdsScan);
-    const int tid = threadIdx.x;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int lane = tid & 63;
-    Share w;
-    const uint32_t lw = xcd_remap(blockIdx.x, gridDim.x);
-    w.team = lw % a.teams;
-    w.wg = lw / a.teams;
-
-    // ---- the list: this thread's requests, their first tile, the total --------------------
-    const int per = (a.batch + kThreads - 1) / kThreads;
-    w.b_lo = min(tid * per, a.batch);
-    w.b_hi = min(w.b_lo + per, a.batch);
-    auto tiles_of = [&](int b) { return (int)((clamp_len(a.lens[b], a) + kTok - 1) / kTok) * a.listed; };
-    int mine = 0;
-    for (int b = w.b_lo; b < w.b_hi; ++b) mine += tiles_of(b);
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int up = __shfl_up(incl, o);
-        if (lane >= o) incl += up;
-    }
-    if (lane == 63) scan[wave] = incl;
-    if (tid < 2) ((CK_LDS int *)(smem + kLdsFlag))[tid] = 0;
-    __syncthreads();
-    int start = incl - mine, total = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        if (i < wave) start += scan[i];
-        total += scan[i];
-    }
-    w.my_start = start;
-    if (w.wg == 0 && w.team == 0) {
-        for (int b = w.b_lo; b < w.b_hi; ++b) {
-            a.sums[b] = start;
-            start += tiles_of(b);
+    if (wg == 0 && team == 0) {
+        const KernArgs a = args_again(first_args);
+        const int tid = 64 * wave + Lane(lane).id;
+        int at = starts[tid];
+        for (int b = first_request(a, tid); b < first_request(a, tid + 1); ++b) {
+            a->sums[b] = at;
+            at += tiles_of(a, b) * a->listed;
         }
-        if (tid == 0) a.sums[a.batch] = total;
+        if (tid == 0) a->sums[a->batch] = total;
     }
-
-    // ---- this workgroup's share ------------------------------------------------------------
-    w.ptiles = w.unit_tiles = 0;
-    w.units = 0;
-    if (a.merge) {
-        w.ptiles = prefix_tiles(a);
-        w.unit_tiles = (w.ptiles + a.psplits - 1) / a.psplits;
-        w.units = w.ptiles > 0 ? a.pmtiles * a.psplits : 0;
-    }
-    const ListMap map = list_map(total, a.chunks, a.min_tiles, w.units, w.unit_tiles);
-    w.chunk = w.wg < map.ra ? w.wg : w.wg - map.ra + map.na;
-    const bool has_list = w.wg < map.ra ? w.wg < map.na : w.wg - map.ra < map.nb;
-    w.lo = has_list ? list_lo(map, w.chunk) : 0;
-    w.hi = has_list ? list_lo(map, w.chunk + 1) : 0;
-
-    if (wave < kProducers) role_loop<DT, NB, true>(a, w, smem);
-    else role_loop<DT, NB, false>(a, w, smem);
 }
 
 // Folds the parts of every row that has some, in list order and after the prefix's, and
@@ -616,14 +724,16 @@ __global__ __launch_bounds__(256) void latent_combine_kernel(DecodeArgs a) {
     const int d4 = 4 * (threadIdx.x & 127);
     if (r >= (int64_t)a.batch * a.rows) return;
     const int b = (int)(r / a.rows), rr = (int)(r - (int64_t)b * a.rows);
-    const int mt = rr / kRows, row = rr - mt * kRows;
+    const int tok = rr / a.heads, head = rr - tok * a.heads;
+    const int group = tok * a.head_groups + head / kWaveRows;
+    const int mt = group / 4, row = (group - 4 * mt) * kWaveRows + head % kWaveRows;
     const int team = a.teams > 1 ? mt : 0, m = a.teams > 1 ? 0 : mt;
     const int64_t all = a.sums[b + 1] - a.sums[b], each = all / a.listed, s0 = a.sums[b] + m * each;
 
     int psplits = 0, units = 0;
     int64_t unit_tiles = 0;
     if (a.merge) {
-        const int64_t ptiles = prefix_tiles(a);
+        const int64_t ptiles = prefix_tiles(a.plen, a.pcols, a.pblocks);
         unit_tiles = (ptiles + a.psplits - 1) / a.psplits;
         if (ptiles > 0) {
             units = a.pmtiles * a.psplits;
@@ -690,7 +800,7 @@ int64_t pad256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 // Sizes of a call: the list's and the prefix's partition, and the workspace.
 struct LatentPlan {
-    int64_t rows, mtiles, teams, listed, chunks, slot_rows, slots;
+    int64_t rows, head_groups, mtiles, teams, listed, chunks, slot_rows, slots;
     int64_t prows, pmtiles, psplits;
     int64_t off_lse, off_o, off_plse, off_po, ws_bytes;
 };
@@ -702,13 +812,15 @@ int make_plan(int64_t batch, int64_t q_len, int64_t heads, int64_t kv_cap, bool 
         prefix_cap > ((int64_t)1 << 30) || batch * q_len > ((int64_t)1 << 31) / heads)
         return CK_E_INVALID_ARG;
     p->rows = q_len * heads;
-    p->mtiles = ceil_div(p->rows, kRows);
+    p->head_groups = ceil_div(heads, kWaveRows);
+    const int64_t groups = q_len * p->head_groups;
+    p->mtiles = ceil_div(groups, 4);
     p->teams = merge ? 1 : p->mtiles;
     p->listed = merge ? p->mtiles : 1;
     p->chunks = p->teams >= kGroups ? 1 : kGroups / p->teams;
     // the list's places and the sums are 32-bit
     if (batch * p->listed * ceil_div(kv_cap, kTok) >= (int64_t)1 << 31) return CK_E_INVALID_ARG;
-    p->slot_rows = p->rows < kRows ? p->rows : kRows;
+    p->slot_rows = kWaveRows * (groups < 4 ? groups : 4);
     p->slots = 2 * p->chunks * p->teams + (merge ? batch * p->listed : 0);
     p->prows = merge ? batch * heads : 0;
     p->pmtiles = ceil_div(p->prows, kRows);
@@ -731,20 +843,14 @@ int make_plan(int64_t batch, int64_t q_len, int64_t heads, int64_t kv_cap, bool 
     return CK_OK;
 }
 
-template <int DT, int NB>
-int launch_decode(const DecodeArgs &a, hipStream_t s) {
-    static std::atomic<uint64_t> lds_set{0};
-    int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(&latent_decode_kernel<DT, NB>), kLds, lds_set);
-    if (rc != CK_OK) return rc;
-    hipLaunchKernelGGL((latent_decode_kernel<DT, NB>), dim3((unsigned)(a.teams * a.chunks)), dim3(kThreads), kLds, s, a);
-    CK_RETURN_LAUNCH();
-}
-
 template <int DT>
 int launch(const DecodeArgs &a, hipStream_t s) {
-    const int rows = a.merge ? kRows : a.rows;  // of the largest row tile
-    int rc = rows <= 16 ? launch_decode<DT, 1>(a, s) : rows <= 32 ? launch_decode<DT, 2>(a, s) : launch_decode<DT, 4>(a, s);
+    static std::atomic<uint64_t> lds_set{0};
+    int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(&latent_decode_kernel<DT>), kLds, lds_set);
     if (rc != CK_OK) return rc;
+    hipLaunchKernelGGL((latent_decode_kernel<DT>), dim3((unsigned)(a.teams * a.chunks)), dim3(kThreads), kLds, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return static_cast<int>(e);
     hipLaunchKernelGGL((latent_combine_kernel<DT>), dim3((unsigned)ceil_div((int64_t)a.batch * a.rows, 2)), dim3(256), 0,
                        s, a);
     CK_RETURN_LAUNCH();
@@ -806,6 +912,7 @@ int run(const void *q, const void *cache, const int32_t *block_table, int64_t bt
     a.part_lse = reinterpret_cast<float *>(ws + p.off_lse);
     a.part_o = reinterpret_cast<float *>(ws + p.off_o);
     a.slot_rows = (int)p.slot_rows;
+    a.head_groups = (int)p.head_groups;
     a.merge = prefix != nullptr;
     if (prefix) {
         a.pcache = static_cast<const uint16_t *>(prefix->cache);
