@@ -475,17 +475,18 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                                                 : tile + (r_addr ^ ((kk & 1) << 6)) + (f & 1) * 16 * kP * 2;
                 return *reinterpret_cast<const CK_LDS u32x4 *>(at);
             };
-            constexpr int kAhead = 4;
-            u32x4 kf[kAhead];
+            constexpr int kAhead = 4, kHeld = kAhead + 1;
+            u32x4 kf[kHeld];
 #pragma unroll
             for (int f = 0; f < 4; ++f) x[f >> 1][f & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int f = 0; f < kAhead; ++f) kf[f] = kfrag(f);
             __builtin_amdgcn_sched_barrier(0);
             static_for<36>([&](auto f) __attribute__((always_inline)) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) x[f & 1][i] = E::mfma16(kf[f % kAhead], qf[i][f >> 1], x[f & 1][i]);
-                if (f + kAhead < 36) kf[f % kAhead] = kfrag(f + kAhead);
+                x[f & 1][0] = E::mfma16(kf[f % kHeld], qf[0][f >> 1], x[f & 1][0]);
+                if (f + kAhead < 36) kf[(f + kAhead) % kHeld] = kfrag(f + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
+                x[f & 1][1] = E::mfma16(kf[f % kHeld], qf[1][f >> 1], x[f & 1][1]);
                 between(f);
                 __builtin_amdgcn_sched_barrier(0);
             });
@@ -520,20 +521,24 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
         };
         // O^T += C^T P^T of a tile whose rows 4 g + n16 / 4 (+ 16) are at v0 (v1).
         auto products = [&](const CK_LDS char *v0, const CK_LDS char *v1, auto &&between) __attribute__((always_inline)) {
-            auto vfrag = [&](int db) {
-                const uint2 x = lds_read_tr16(v0 + db * 32), y = lds_read_tr16(v1 + db * 32);
-                return u32x4{x.x, x.y, y.x, y.y};
-            };
-            constexpr int kAhead = 4;
-            u32x4 vf[kAhead];
+            constexpr int kAhead = 4, kHeld = kAhead + 1;
+            uint2 va[kHeld], vb[kHeld];
 #pragma unroll
-            for (int db = 0; db < kAhead; ++db) vf[db] = vfrag(db);
+            for (int db = 0; db < kAhead; ++db) {
+                va[db] = lds_read_tr16(v0 + db * 32);
+                vb[db] = lds_read_tr16(v1 + db * 32);
+            }
             __builtin_amdgcn_sched_barrier(0);
             acc_ready(pf[0], pf[1]);
             static_for<32>([&](auto db) __attribute__((always_inline)) {
-                acc_mfma<DT, db, 0>(vf[db % kAhead], pf[0]);
-                acc_mfma<DT, db, 1>(vf[db % kAhead], pf[1]);
-                if (db + kAhead < 32) vf[db % kAhead] = vfrag(db + kAhead);
+                constexpr int at = (db + kAhead) % kHeld;
+                const uint2 x = va[db % kHeld], y = vb[db % kHeld];
+                const u32x4 c = {x.x, x.y, y.x, y.y};
+                acc_mfma<DT, db, 0>(c, pf[0]);
+                if (db + kAhead < 32) va[at] = lds_read_tr16(v0 + (db + kAhead) * 32);
+                __builtin_amdgcn_sched_barrier(0);
+                acc_mfma<DT, db, 1>(c, pf[1]);
+                if (db + kAhead < 32) vb[at] = lds_read_tr16(v1 + (db + kAhead) * 32);
                 between(db);
                 __builtin_amdgcn_sched_barrier(0);
             });
