@@ -61,6 +61,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kPieces = 9;    // DMAs per wave and tile: 8 rows of the latent, and their rotated dims
 constexpr int kPhase = 256;   // tiles described in LDS at a time
 constexpr int kGroups = 256;  // workgroups: one per CU
+constexpr int kMinPlaces = 4;  // least places of the list per chunk
 constexpr float kSlack = 8.f;
 
 constexpr int kLdsZero = kSlots * kSlotBytes;  // a row of zeros
@@ -68,7 +69,8 @@ constexpr int kLdsDesc = kLdsZero + kPitch;
 constexpr int kLdsPlace = kLdsDesc + kPhase * 16;
 constexpr int kLdsScan = kLdsPlace + kPhase * 8;
 constexpr int kLdsStart = kLdsScan + 64;  // each thread's place in the list
-constexpr int kLds = kLdsStart + kThreads * 4;
+constexpr int kLdsLen = kLdsStart + kThreads * 4;  // and its first request's length
+constexpr int kLds = kLdsLen + kThreads * 4;
 static_assert(kPhase == kThreads, "a tile per thread");
 static_assert(kLds <= 160 * 1024, "LDS");
 
@@ -92,13 +94,12 @@ struct DecodeArgs {
     int teams;    // row tiles of a request given to workgroups of their own
     int listed;   // row tiles of a request listed one after another (teams == 1)
     int chunks;   // workgroups per team
-    int min_tiles;  // least tiles per chunk
     float scale_log2;
     void *out;    // [batch * q_len, heads, 512]
     float *lse;   // [batch * q_len * heads]
     float *part_o;    // [slots][slot_rows][512]
     float *part_lse;  // [slots][slot_rows], log2
-    int32_t *sums;    // [batch + 1]: tiles of the list before each request
+    int32_t *sums;    // [batch + 2]: the list's places before each request and in all; the prefix's splits
     int slot_rows;
     int merge;        // 1: every part goes to the workspace (a prefix is folded in)
     // shared prefix (merge == 1)
@@ -109,9 +110,9 @@ struct DecodeArgs {
     int64_t pblocks;
     int prows;    // batch * heads
     int pmtiles;
-    int psplits;
-    float *ppart_o;    // [psplits][prows][512]
-    float *ppart_lse;  // [psplits][prows], log2
+    int most_splits;
+    float *ppart_o;    // [splits][prows][512]
+    float *ppart_lse;  // [splits][prows], log2
 };
 
 __device__ __forceinline__ int64_t clamp_len(int64_t n, int64_t cols, int64_t num_blocks) {
@@ -119,9 +120,8 @@ __device__ __forceinline__ int64_t clamp_len(int64_t n, int64_t cols, int64_t nu
     if (n > cap) n = cap;
     return n < 0 || num_blocks <= 0 ? 0 : n;
 }
-__device__ __forceinline__ int64_t prefix_tiles(const int64_t *len, int64_t cols, int64_t num_blocks) {
-    return (clamp_len(*len, cols, num_blocks) + kTok - 1) / kTok;
-}
+__device__ __forceinline__ int tiles_of(int64_t len) { return (int)((len + kTok - 1) / kTok); }
+__device__ __forceinline__ int places_of(int64_t len) { return len > 0 ? tiles_of(len) + kItemPlaces : 0; }
 
 // A value that is the same in all lanes, into scalar registers (divisions leave it in vector ones).
 __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -230,12 +230,17 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     auto first_request = [](KernArgs a, int t) {
         return (int)min((int64_t)t * ((a->batch + kThreads - 1) / kThreads), (int64_t)a->batch);
     };
-    auto tiles_of = [](KernArgs a, int b) { return (int)((clamp_len(a->lens[b], a->bt_cols, a->num_blocks) + kTok - 1) / kTok); };
-    CK_LDS int *starts = (CK_LDS int *)(smem + kLdsStart);
+    auto len_of = [](KernArgs a, int b) { return (int)clamp_len(a->lens[b], a->bt_cols, a->num_blocks); };
+    CK_LDS int *starts = (CK_LDS int *)(smem + kLdsStart), *len0 = (CK_LDS int *)(smem + kLdsLen);
     int total = 0;
     {
         int mine = 0;
-        for (int b = first_request(first_args, first_tid); b < first_request(first_args, first_tid + 1); ++b) mine += tiles_of(first_args, b) * first_args->listed;
+        const int b0 = first_request(first_args, first_tid), b1 = first_request(first_args, first_tid + 1);
+        for (int b = b0; b < b1; ++b) {
+            const int len = len_of(first_args, b);
+            if (b == b0) len0[first_tid] = len;
+            mine += places_of(len) * first_args->listed;
+        }
         int incl = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -256,17 +261,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     }
 
     // ---- this workgroup's share ------------------------------------------------------------
-    int64_t ptiles = 0, unit_tiles = 0;
-    int units = 0;
+    int ptiles = 0, unit_tiles = 0, units = 0, splits = 0;
     if (first_args->merge) {
-        ptiles = scalar(prefix_tiles(first_args->plen, first_args->pcols, first_args->pblocks));
-        unit_tiles = scalar((ptiles + first_args->psplits - 1) / first_args->psplits);
-        units = ptiles > 0 ? first_args->pmtiles * first_args->psplits : 0;
+        ptiles = scalar(tiles_of(clamp_len(*first_args->plen, first_args->pcols, first_args->pblocks)));
+        if (ptiles > 0) {
+            splits = scalar(prefix_splits(first_args->pmtiles, ptiles, total, kGroups, min(first_args->most_splits, ptiles)));
+            unit_tiles = scalar((ptiles + splits - 1) / splits);
+            units = first_args->pmtiles * splits;
+        }
     }
-    const ListMap map = list_map(total, first_args->chunks, first_args->min_tiles, units, unit_tiles);
-    const int chunk = scalar(wg < map.ra ? wg : wg - map.ra + map.na);
-    const bool has_list = scalar((int)(wg < map.ra ? wg < map.na : wg - map.ra < map.nb));
-    const int64_t lo = has_list ? scalar(list_lo(map, chunk)) : 0, hi = has_list ? scalar(list_lo(map, chunk + 1)) : 0;
+    const ListMap map = list_map(total, first_args->chunks, kMinPlaces, units, unit_tiles + kItemPlaces);
+    const int chunk = scalar(wg < map.ra ? wg : wg - map.ra + map.a.chunks);
+    const bool has_list = scalar((int)(wg < map.ra ? wg < map.a.chunks : wg - map.ra < map.b.chunks));
+    const int lo = has_list ? scalar(list_lo(map, chunk)) : 0, hi = has_list ? scalar(list_lo(map, chunk + 1)) : 0;
 
     // ---- per-lane addresses ------------------------------------------------------------------
     for (int i = first_tid; i < kPitch / 4; i += kThreads) ((CK_LDS int *)(smem + kLdsZero))[i] = 0;
@@ -302,24 +309,25 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     Segment seg = {0, 0, 0, -1, 0};
     const float scale_log2 = first_args->scale_log2;
     u32x4 qf[2][18];
+    bool fresh = false;  // O is zero
     float m_row[2], sub[2], l_part[2];  // per row: reference point, what scores are lowered by, sum of p
 
     CK_LDS int *mark = (CK_LDS int *)smem;  // in the ring's place: [kPhase] each
-    CK_LDS int *seg_item = mark + kPhase, *seg_tile = seg_item + kPhase, *seg_len = seg_tile + kPhase;
+    CK_LDS int *seg_item = mark + kPhase, *seg_at = seg_item + kPhase, *seg_len = seg_at + kPhase;
     int unit = wg, phase = 0;
-    int64_t at_prefix = 0, at_list = lo;  // within the unit; in the list
+    int at_prefix = 0, at_list = lo;  // within the unit; in the list
     for (;;) {
         const KernArgs a = args_again(first_args);
         const int tid = 64 * wave + Lane(lane).id;  // again: its places in the tables are not to be held either
         // ---- describe the next tiles, at most kPhase: a prefix unit's, then the list's -------
         const bool in_prefix = unit < units;
         ++phase;
-        auto describe = [&](int page, int64_t blocks, int item, int64_t tile, int len) {
+        auto describe = [&](int i, int page, int64_t blocks, int item, int tile, int len) {
             const bool ok = page >= 0 && page < blocks;
             const int64_t at = ok ? (int64_t)page * kPageBytes + (tile % kTilesPerPage) * kTileBytes : 0;
-            *reinterpret_cast<CK_LDS u32x4 *>(desc + 4 * tid) =
+            *reinterpret_cast<CK_LDS u32x4 *>(desc + 4 * i) =
                 u32x4{ok ? 1u : 0u, (unsigned)item, (unsigned)(tile * kTok), (unsigned)len};
-            place[tid] = u32x2{(unsigned)at, (unsigned)(at >> 32)};
+            place[i] = u32x2{(unsigned)at, (unsigned)(at >> 32)};
             if (!ok) *bad = phase;
         };
         int n, sp = 0;
@@ -330,14 +338,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             // row tiles inner: workgroups side by side read the same prefix tiles
             sp = scalar(unit / a->pmtiles);
             const int mt = unit - sp * a->pmtiles;
-            const int64_t p_lo = sp * unit_tiles + at_prefix, p_hi = min((sp + 1) * unit_tiles, ptiles);
-            n = (int)max((int64_t)0, min((int64_t)kPhase, p_hi - p_lo));
+            const int p_lo = sp * unit_tiles + at_prefix, p_hi = min((sp + 1) * unit_tiles, ptiles);
+            n = max(0, min(kPhase, p_hi - p_lo));
             last = p_lo + n >= p_hi;
             cache = reinterpret_cast<const char *>(a->pcache);
             prefix_row0 = (int64_t)mt * kRows + kWaveRows * wave;  // rows of all sequences, one after another
             if (tid < n) {
-                const int64_t tile = p_lo + tid;
-                describe(a->pbt[tile / kTilesPerPage], a->pblocks, unit, tile, (int)min(a->plen[0], a->pcols * kPage));
+                const int tile = p_lo + tid;
+                describe(tid, a->pbt[tile / kTilesPerPage], a->pblocks, unit, tile, (int)min(a->plen[0], a->pcols * kPage));
             }
             at_prefix += n;
             if (last) {
@@ -346,45 +354,54 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             }
             if (n == 0) continue;  // past a short prefix's end: the combine counts the splits the same way
         } else if (at_list < hi) {
-            const int64_t ph = at_list;
-            n = (int)min((int64_t)kPhase, hi - ph);
-            last = ph + n >= hi;
-            at_list += n;
+            const int ph = at_list, places = min(kPhase, hi - ph);
+            last = ph + places >= hi;
+            at_list += places;
             cache = reinterpret_cast<const char *>(a->cache);
             mark[tid] = 0;
             __syncthreads();
-            int64_t at = starts[tid];
-            for (int b = first_request(a, tid); b < first_request(a, tid + 1) && at < ph + n; ++b) {
-                const int64_t len = clamp_len(a->lens[b], a->bt_cols, a->num_blocks);
-                const int each = (int)((len + kTok - 1) / kTok);
+            int at = starts[tid];
+            const int b0 = first_request(a, tid), b1 = first_request(a, tid + 1);
+            for (int b = b0; b < b1 && at < ph + places; ++b) {
+                const int len = b == b0 ? len0[tid] : len_of(a, b);
+                const int each = places_of(len);
                 for (int m = 0; m < a->listed; ++m, at += each) {
-                    if (each > 0 && at < ph + n && at + each > ph) {
-                        const int i = (int)(max(at, ph) - ph);
+                    if (each > 0 && at < ph + places && at + each > ph) {
+                        const int i = max(at, ph) - ph;
                         mark[i] = 1;
                         seg_item[i] = b * a->listed + m;
-                        seg_tile[i] = (int)(max(at, ph) - at);
-                        seg_len[i] = (int)len;
+                        seg_at[i] = max(at, ph) - at;
+                        seg_len[i] = len;
                     }
                 }
             }
             __syncthreads();
-            // the last segment start at or before tile tid
+            // Place i's item is that of the last mark at or before it. Each mark past the first is
+            // followed by kItemPlaces empty places, which the tiles close up over.
             const Lane l(lane);
-            int i = -1;
-            for (int w = 0; w <= wave; ++w) {
-                uint64_t m = __builtin_amdgcn_ballot_w64(mark[64 * w + l.id] != 0);
-                if (w == wave) m &= ~0ull >> (63 - l.id);
-                if (m) i = 64 * w + 63 - __clzll(m);
+            int item_at = 0, last_at = 0, marks = 0, all_marks = 0;  // marks: up to this place
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const uint64_t all = __builtin_amdgcn_ballot_w64(mark[64 * w + l.id] != 0);
+                const uint64_t mine = w < wave ? all : w == wave ? all & (~0ull >> (63 - l.id)) : 0;
+                if (mine) item_at = 64 * w + 63 - __clzll(mine);
+                if (all) last_at = 64 * w + 63 - __clzll(all);
+                marks += __popcll(mine);
+                all_marks += __popcll(all);
             }
-            if (tid < n) {
-                const int it = seg_item[i], tile = seg_tile[i] + tid - i;
-                describe(a->bt[(int64_t)(it / a->listed) * a->bt_cols + tile / kTilesPerPage], a->num_blocks, it, tile,
-                         seg_len[i]);
+            const int skipped = kItemPlaces - min(kItemPlaces, seg_at[0]);  // of the first mark
+            n = scalar(places - kItemPlaces * (all_marks - 1) - skipped + max(0, kItemPlaces - (seg_at[last_at] + places - last_at)));
+            const int off = seg_at[item_at] + tid - item_at;
+            if (tid < places && off >= kItemPlaces) {
+                const int it = seg_item[item_at], tile = off - kItemPlaces;
+                describe(tid - kItemPlaces * (marks - 1) - skipped,
+                         a->bt[(int64_t)(it / a->listed) * a->bt_cols + tile / kTilesPerPage], a->num_blocks, it, tile, seg_len[item_at]);
             }
         } else {
             break;
         }
         __syncthreads();
+        if (n == 0) continue;  // empty places
 
         // ---- the tiles ------------------------------------------------------------------------
         struct Tile {
@@ -461,6 +478,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                 l_part[i] = 0.f;
             }
             acc_zero();
+            fresh = true;
         };
 
         // S^T = X Q^T of tile t: tokens 4 g + r and 16 + 4 g + r of rows n16 and 16 + n16.
@@ -545,18 +563,17 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
         };
 
         // ---- the phase's first tiles ------------------------------------------------------------
-        for (int t = 0; t < 3; ++t) {
-            const Moves m = moves_of(place_at(t), t, tile_at(t).ok);
-            static_for<kPieces>([&](auto j) __attribute__((always_inline)) { move(m, j); });
-        }
         {
             const Tile d = tile_at(0);
-            if (d.item != seg.item) {
-                seg = segment_of(d);
-                start();
-            }
+            const bool opens = d.item != seg.item;
+            if (opens) seg = segment_of(d);
             load_q(seg);  // in each phase, so that it is not held while the tiles are described
-            wait_vmcnt<0>();
+            for (int t = 0; t < 3; ++t) {
+                const Moves m = moves_of(place_at(t), t, tile_at(t).ok);
+                static_for<kPieces>([&](auto j) __attribute__((always_inline)) { move(m, j); });
+            }
+            if (opens) start();
+            wait_vmcnt<2 * kPieces>();
             if (!d.ok) blank(0);
             __syncthreads();
             if (seg.rows_n > 0) {
@@ -597,8 +614,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                         sub[i] = (m_new == -INFINITY ? 0.f : m_new) - E::kBias;
                         l_part[i] *= scale[i];
                     }
-                    acc_scale(scale[0], scale[1]);
+                    if (!fresh) acc_scale(scale[0], scale[1]);
                 }
+                fresh = false;
                 static_for<8>([&](auto e) __attribute__((always_inline)) { p_of(e); });
                 // Tokens that the rows do not see (past the length they may hold anything) are read
                 // as zeros: 0 * inf must not reach O.
@@ -712,92 +730,105 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
         int at = starts[tid];
         for (int b = first_request(a, tid); b < first_request(a, tid + 1); ++b) {
             a->sums[b] = at;
-            at += tiles_of(a, b) * a->listed;
+            at += places_of(len_of(a, b)) * a->listed;
         }
-        if (tid == 0) a->sums[a->batch] = total;
+        if (tid == 0) {
+            a->sums[a->batch] = total;
+            a->sums[a->batch + 1] = splits;
+        }
     }
 }
 
 // Folds the parts of every row that has some, in list order and after the prefix's, and
-// writes rows that see nothing. 128 threads a row, 4 dims each; parts are loaded kBatch at a
-// time, independent of each other.
+// writes rows that see nothing. A wave takes a row: lane p holds the weight of the p-th of 64
+// parts, then 4 + 4 dims of each part in turn, loaded kBatch at a time.
 template <int DT>
 __global__ __launch_bounds__(256) void latent_combine_kernel(DecodeArgs a) {
     using E = Elem<DT>;
-    constexpr int kBatch = 8;
-    const int64_t r = (int64_t)blockIdx.x * 2 + (threadIdx.x >> 7);
-    const int d4 = 4 * (threadIdx.x & 127);
-    if (r >= (int64_t)a.batch * a.rows) return;
-    const int b = (int)(r / a.rows), rr = (int)(r - (int64_t)b * a.rows);
-    const int tok = rr / a.heads, head = rr - tok * a.heads;
+    constexpr int kBatch = 6;
+    const int lane = __lane_id();
+    const int r = scalar((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    if (r >= a.batch * a.rows) return;
+    const int b = scalar(r / a.rows), rr = r - b * a.rows;
+    const int tok = scalar(rr / a.heads), head = rr - tok * a.heads;
     const int group = tok * a.head_groups + head / kWaveRows;
     const int mt = group / 4, row = (group - 4 * mt) * kWaveRows + head % kWaveRows;
     const int team = a.teams > 1 ? mt : 0, m = a.teams > 1 ? 0 : mt;
-    const int64_t all = a.sums[b + 1] - a.sums[b], each = all / a.listed, s0 = a.sums[b] + m * each;
+    const int places = scalar((a.sums[b + 1] - a.sums[b]) / a.listed);
 
-    int psplits = 0, units = 0;
-    int64_t unit_tiles = 0;
+    int ptiles = 0, unit_tiles = 0, splits = 0, units = 0;
     if (a.merge) {
-        const int64_t ptiles = prefix_tiles(a.plen, a.pcols, a.pblocks);
-        unit_tiles = (ptiles + a.psplits - 1) / a.psplits;
+        ptiles = tiles_of(clamp_len(*a.plen, a.pcols, a.pblocks));
         if (ptiles > 0) {
-            units = a.pmtiles * a.psplits;
-            psplits = (int)((ptiles + unit_tiles - 1) / unit_tiles);
+            const int dealt = a.sums[a.batch + 1];
+            unit_tiles = scalar((ptiles + dealt - 1) / dealt);
+            units = a.pmtiles * dealt;
+            splits = scalar((ptiles + unit_tiles - 1) / unit_tiles);  // that hold tiles
         }
     }
     int c0 = 0, parts = 0;
     bool whole = false;
-    if (each > 0) {
-        const ListMap map = list_map(a.sums[a.batch], a.chunks, a.min_tiles, units, unit_tiles);
-        c0 = list_chunk(map, s0);
-        parts = list_chunk(map, s0 + each - 1) - c0 + 1;
+    if (places > 0) {
+        const ListMap map = list_map(a.sums[a.batch], a.chunks, kMinPlaces, units, unit_tiles + kItemPlaces);
+        const int at = a.sums[b] + m * places;
+        c0 = scalar(list_chunk(map, at + kItemPlaces));
+        parts = scalar(list_chunk(map, at + places - 1)) - c0 + 1;
         whole = parts == 1;
         if (whole && !a.merge) return;  // written by its workgroup
     }
-    const int total = psplits + parts;
+    const int total = splits + parts;
+    // a part's row, in rows of its workspace
+    auto part_row = [&](int p) -> int64_t {
+        if (p < splits) return (int64_t)p * a.prows + r;
+        const int c = c0 + p - splits;
+        const int64_t slot = whole ? (int64_t)2 * a.chunks * a.teams + b * a.listed + m : part_slot(c > c0, c, a.teams, team);
+        return slot * a.slot_rows + row;
+    };
     float mx = -INFINITY, sum = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int p0 = 0; p0 < total; p0 += kBatch) {
-        float ls[kBatch];
-        f32x4 o[kBatch];
+    f32x4 acc[2] = {};
+    for (int p0 = 0; p0 < total; p0 += 64) {
+        const int count = min(64, total - p0), p = p0 + min(lane, count - 1);
+        float ls = (p < splits ? a.ppart_lse : a.part_lse)[part_row(p)];
+        if (lane >= count) ls = -INFINITY;
+        float mb = fmaxf(mx, ls);
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            const int p = min(p0 + j, total - 1);  // past the last part: it again, at weight 0
-            const float *po, *pl;
-            if (p < psplits) {
-                pl = a.ppart_lse + (int64_t)p * a.prows + r;
-                po = a.ppart_o + ((int64_t)p * a.prows + r) * kR;
-            } else {
-                const int c = c0 + p - psplits;
-                const int64_t slot = whole ? (int64_t)2 * a.chunks * a.teams + b * a.listed + m
-                                           : part_slot(c > c0, c, a.teams, team);
-                pl = a.part_lse + slot * a.slot_rows + row;
-                po = a.part_o + (slot * a.slot_rows + row) * kR;
-            }
-            ls[j] = p0 + j < total ? *pl : -INFINITY;
-            o[j] = *reinterpret_cast<const f32x4 *>(po + d4);
-        }
-        float mb = mx;
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) mb = fmaxf(mb, ls[j]);
+        for (int o = 1; o < 64; o <<= 1) mb = fmaxf(mb, __shfl_xor(mb, o));
         const float mu = mb == -INFINITY ? 0.f : mb;
-        const float f = exp2_fast(mx - mu);
-        acc *= f;
-        sum *= f;
+        const float f = exp2_fast(mx - mu), w = exp2_fast(ls - mu);  // a part that saw nothing holds zeros
+        float ws = w;
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            // a part that saw nothing holds zeros
-            const float w = exp2_fast(ls[j] - mu);
-            if (p0 + j < total) acc += o[j] * w;
-            sum += w;
-        }
+        for (int o = 1; o < 64; o <<= 1) ws += __shfl_xor(ws, o);
+        sum = sum * f + ws;
+        acc[0] *= f;
+        acc[1] *= f;
         mx = mb;
+        for (int q0 = 0; q0 < count; q0 += kBatch) {
+            f32x4 o[kBatch][2];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                if (q0 + j >= count) break;
+                const int q = p0 + q0 + j;
+                const float *po = (q < splits ? a.ppart_o : a.part_o) + part_row(q) * kR + 4 * lane;
+                o[j][0] = *reinterpret_cast<const f32x4 *>(po);
+                o[j][1] = *reinterpret_cast<const f32x4 *>(po + kR / 2);
+            }
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                if (q0 + j >= count) break;
+                const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), q0 + j));
+                acc[0] += o[j][0] * wj;
+                acc[1] += o[j][1] * wj;
+            }
+        }
     }
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    acc *= inv;
-    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + r * kR + d4) =
-        make_uint2(E::pack2(acc[0], acc[1]), E::pack2(acc[2], acc[3]));
-    if (d4 == 0) a.lse[r] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        acc[i] *= inv;
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + (int64_t)r * kR + i * (kR / 2) + 4 * lane) =
+            make_uint2(E::pack2(acc[i][0], acc[i][1]), E::pack2(acc[i][2], acc[i][3]));
+    }
+    if (lane == 0) a.lse[r] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
 }
 
 int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
@@ -814,7 +845,7 @@ int make_plan(int64_t batch, int64_t q_len, int64_t heads, int64_t kv_cap, bool 
               LatentPlan *p) {
     if (batch < 0 || q_len < 1 || heads < 1 || kv_cap < 0 || prefix_cap < 0) return CK_E_INVALID_ARG;
     if (batch > (1 << 24) || q_len > (1 << 24) || heads > (1 << 16) || kv_cap > ((int64_t)1 << 30) ||
-        prefix_cap > ((int64_t)1 << 30) || batch * q_len > ((int64_t)1 << 31) / heads)
+        prefix_cap > ((int64_t)1 << 30) || batch * q_len >= ((int64_t)1 << 31) / heads)
         return CK_E_INVALID_ARG;
     p->rows = q_len * heads;
     p->head_groups = ceil_div(heads, kWaveRows);
@@ -824,18 +855,18 @@ int make_plan(int64_t batch, int64_t q_len, int64_t heads, int64_t kv_cap, bool 
     p->listed = merge ? p->mtiles : 1;
     p->chunks = p->teams >= kGroups ? 1 : kGroups / p->teams;
     // the list's places and the sums are 32-bit
-    if (batch * p->listed * ceil_div(kv_cap, kTok) >= (int64_t)1 << 31) return CK_E_INVALID_ARG;
+    if (batch * p->listed * (ceil_div(kv_cap, kTok) + kItemPlaces) >= (int64_t)1 << 31) return CK_E_INVALID_ARG;
     p->slot_rows = kWaveRows * (groups < 4 ? groups : 4);
     p->slots = 2 * p->chunks * p->teams + (merge ? batch * p->listed : 0);
     p->prows = merge ? batch * heads : 0;
     p->pmtiles = ceil_div(p->prows, kRows);
     p->psplits = 0;
     if (merge && p->pmtiles > 0) {
-        p->psplits = p->pmtiles >= kGroups ? 1 : kGroups / p->pmtiles;
-        const int64_t most = ceil_div(prefix_cap, 4 * kTok);
+        p->psplits = p->pmtiles >= 2 * kGroups ? 1 : 2 * kGroups / p->pmtiles;  // two rounds
+        const int64_t most = ceil_div(prefix_cap, 2 * kTok);  // of two tiles at least
         if (p->psplits > most) p->psplits = most < 1 ? 1 : most;
     }
-    int64_t at = pad256((batch + 1) * 4);
+    int64_t at = pad256((batch + 2) * 4);
     p->off_lse = at;
     at += pad256(p->slots * p->slot_rows * 4);
     p->off_plse = at;
@@ -856,7 +887,7 @@ int launch(const DecodeArgs &a, hipStream_t s) {
     hipLaunchKernelGGL((latent_decode_kernel<DT>), dim3((unsigned)(a.teams * a.chunks)), dim3(kThreads), kLds, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return static_cast<int>(e);
-    hipLaunchKernelGGL((latent_combine_kernel<DT>), dim3((unsigned)ceil_div((int64_t)a.batch * a.rows, 2)), dim3(256), 0,
+    hipLaunchKernelGGL((latent_combine_kernel<DT>), dim3((unsigned)ceil_div((int64_t)a.batch * a.rows, 4)), dim3(256), 0,
                        s, a);
     CK_RETURN_LAUNCH();
 }
@@ -909,7 +940,6 @@ int run(const void *q, const void *cache, const int32_t *block_table, int64_t bt
     a.teams = (int)p.teams;
     a.listed = (int)p.listed;
     a.chunks = (int)p.chunks;
-    a.min_tiles = 4;
     a.scale_log2 = scale * kLog2e;
     a.out = out;
     a.lse = lse;
@@ -927,7 +957,7 @@ int run(const void *q, const void *cache, const int32_t *block_table, int64_t bt
         a.pblocks = prefix->num_blocks;
         a.prows = (int)p.prows;
         a.pmtiles = (int)p.pmtiles;
-        a.psplits = (int)p.psplits;
+        a.most_splits = (int)p.psplits;
         a.ppart_lse = reinterpret_cast<float *>(ws + p.off_plse);
         a.ppart_o = reinterpret_cast<float *>(ws + p.off_po);
     }
