@@ -62,6 +62,7 @@ constexpr int kPieces = 9;    // DMAs per wave and tile: 8 rows of the latent, a
 constexpr int kPhase = 256;   // tiles described in LDS at a time
 constexpr int kGroups = 256;  // workgroups: one per CU
 constexpr int kMinPlaces = 4;  // least places of the list per chunk
+constexpr int kFoldBlocks = 256;
 constexpr float kSlack = 8.f;
 
 constexpr int kLdsZero = kSlots * kSlotBytes;  // a row of zeros
@@ -97,7 +98,10 @@ struct DecodeArgs {
     float scale_log2;
     void *out;    // [batch * q_len, heads, 512]
     float *lse;   // [batch * q_len * heads]
-    float *part_o;    // [slots][slot_rows][512]
+    // Parts are kept by blocks of 16 rows as the lanes hold them, [128 x 4 dims][16 rows][4]:
+    // neighbouring lanes then store and load neighbouring bytes. Lanes in different rows (2 KB
+    // apart) took a cycle each, 16000 of them for a workgroup's 256 KB.
+    float *part_o;    // [slots][slot_rows / 16][128][16][4]
     float *part_lse;  // [slots][slot_rows], log2
     int32_t *sums;    // [batch + 2]: the list's places before each request and in all; the prefix's splits
     int slot_rows;
@@ -109,10 +113,11 @@ struct DecodeArgs {
     int64_t pcols;
     int64_t pblocks;
     int prows;    // batch * heads
+    int prows_up;  // in whole row tiles
     int pmtiles;
     int most_splits;
-    float *ppart_o;    // [splits][prows][512]
-    float *ppart_lse;  // [splits][prows], log2
+    float *ppart_o;    // [splits][prows_up / 16][128][16][4]
+    float *ppart_lse;  // [splits][prows_up], log2
 };
 
 __device__ __forceinline__ int64_t clamp_len(int64_t n, int64_t cols, int64_t num_blocks) {
@@ -145,6 +150,16 @@ __device__ __forceinline__ float over_groups(float x, Op &&op) {
     x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Of a row's 32 dims, x its dims 4 g .. + 3 and y its dims 16 + 4 g .. + 3 in lane group g:
+// 8 neighbouring ones, from dim 16 (g & 1) + 8 (g >> 1) on, rounded once to 16 bits.
+template <int DT>
+__device__ __forceinline__ u32x4 eight_dims(f32x4 x, f32x4 y) {
+    using E = Elem<DT>;
+    const auto lo = __builtin_amdgcn_permlane16_swap(E::pack2(x[0], x[1]), E::pack2(y[0], y[1]), false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap(E::pack2(x[2], x[3]), E::pack2(y[2], y[3]), false, false);
+    return u32x4{lo[0], hi[0], lo[1], hi[1]};
 }
 
 typedef const __attribute__((address_space(4))) DecodeArgs *KernArgs;
@@ -460,15 +475,45 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             x.limit = max(0, min(d.len, d.len - a->q_len + 1 + tok));
             return x;
         };
+        // Q comes in pieces of 256 contiguous bytes for 16 lanes (an operand's own place, 64 lanes in
+        // 16 rows, costs a cycle a lane: 9200 of them for a workgroup's 128 rows) and is turned
+        // into operands through LDS: piece (m, e), rows 4 e .. + 3, dims 128 m .. + 127, waits in the
+        // registers of operand (e / 4, 4 m + e % 4); the rotated dims in 8 rows x 128 bytes.
         auto load_q = [&](const Segment &x) {  // a row past the last repeats it: it is not stored
             const KernArgs a = args_again(first_args);
             const Lane l(lane);
+            const int end = x.rows_n - 1;
+            const uint16_t *q = a->q + x.row0 * kRow;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint16_t *q = a->q + (x.row0 + min(16 * i + l.n16, max(0, x.rows_n - 1))) * kRow + 8 * l.g;
+            for (int m = 0; m < 4; ++m)
 #pragma unroll
-                for (int kk = 0; kk < 18; ++kk) qf[i][kk] = *reinterpret_cast<const u32x4 *>(q + 32 * kk);
+                for (int e = 0; e < 8; ++e)
+                    qf[e >> 2][4 * m + (e & 3)] =
+                        *reinterpret_cast<const u32x4 *>(q + min(4 * e + l.g, end) * kRow + 128 * m + 8 * l.n16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                qf[e >> 1][16 + (e & 1)] =
+                    *reinterpret_cast<const u32x4 *>(q + min(8 * e + (l.id >> 3), end) * kRow + kR + 8 * (l.id & 7));
+        };
+        // Through the wave's own 8 rows of the slot of tile t, which nothing moves to or reads now.
+        auto turn_q = [&](int t) {
+            const Lane l(lane);
+            CK_LDS char *at = smem + (t & (kSlots - 1)) * kSlotBytes + 8 * wave * kPitch;
+            auto piece = [&](int row, int chunk) {  // of [32][16] chunks: the 16 of a row XORed
+                return reinterpret_cast<CK_LDS u32x4 *>(at + row * 256 + ((chunk ^ row) & 15) * 16);
+            };
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) *piece(4 * e + l.g, l.n16) = qf[e >> 2][4 * m + (e & 3)];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qf[e >> 2][4 * m + (e & 3)] = *piece(16 * (e >> 2) + l.n16, 4 * (e & 3) + l.g);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *piece(8 * e + (l.id >> 3), l.id & 7) = qf[e >> 1][16 + (e & 1)];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qf[e >> 1][16 + (e & 1)] = *piece(16 * (e >> 1) + l.n16, 4 * (e & 1) + l.g);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // before the next move there
         };
         auto start = [&]() {
 #pragma unroll
@@ -567,13 +612,17 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             const Tile d = tile_at(0);
             const bool opens = d.item != seg.item;
             if (opens) seg = segment_of(d);
-            load_q(seg);  // in each phase, so that it is not held while the tiles are described
-            for (int t = 0; t < 3; ++t) {
+            auto move_tile = [&](int t) {
                 const Moves m = moves_of(place_at(t), t, tile_at(t).ok);
                 static_for<kPieces>([&](auto j) __attribute__((always_inline)) { move(m, j); });
-            }
+            };
+            move_tile(0);
+            if (seg.rows_n > 0) load_q(seg);  // in each phase, so that it is not held while the tiles are described
             if (opens) start();
-            wait_vmcnt<2 * kPieces>();
+            wait_vmcnt<0>();
+            if (seg.rows_n > 0) turn_q(3);
+            move_tile(1);
+            move_tile(2);
             if (!d.ok) blank(0);
             __syncthreads();
             if (seg.rows_n > 0) {
@@ -583,14 +632,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                 largest(s, 1);
             }
         }
-        bool stored = false;  // the last step ended with 32 stores of this wave or more
+        bool stored = false;  // the last step ended with stores, not to be waited for yet
         for (int t = 0; t < n; ++t) {
             // ---- a step in general ----------------------------------------------------------------
             // Tile t + 1 is in, in every wave; tile t + 3 takes the place of tile t - 1. The scores
             // of tile t are there.
             const Tile d0 = tile_at(t), d1 = tile_at(t + 1);
-            if (stored) wait_vmcnt<kPieces + 32>();
-            else wait_vmcnt<kPieces>();
+            if (!stored) wait_vmcnt<kPieces>();  // such a step waited for it before its stores
             if (!d1.ok) blank(t + 1);
             __syncthreads();
             stored = false;
@@ -601,7 +649,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             Segment next = seg;
             if (opens) {  // Q's registers are free since the scores of tile t
                 next = segment_of(d1);
-                load_q(next);
+                if (next.rows_n > 0) load_q(next);
             }
             if (seg.rows_n > 0) {
                 if (moves()) {
@@ -627,6 +675,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             // Q, and tile t + 2: before the moves and stores below. Whether the step opens a segment
             // or not: at Q's use in the plain steps the compiler would wait otherwise.
             wait_vmcnt<0>();
+            if (opens && next.rows_n > 0) turn_q(t + 3);
             {
                 const Moves m = moves_of(place_at(t + 3), t + 3, tile_at(t + 3).ok);
                 static_for<kPieces>([&](auto j) __attribute__((always_inline)) { move(m, j); });
@@ -643,13 +692,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                 const KernArgs a = args_again(first_args);
                 float *po = nullptr, *pl = nullptr;  // the wave's first row of its part
                 if (in_prefix) {
-                    po = a->ppart_o + (sp * (int64_t)a->prows + seg.row0) * kR;
-                    pl = a->ppart_lse + sp * (int64_t)a->prows + seg.row0;
+                    const int64_t row = sp * (int64_t)a->prows_up + seg.row0;
+                    po = a->ppart_o + row * kR;
+                    pl = a->ppart_lse + row;
                 } else if (a->merge || seg.began_before || goes_on) {
                     const int64_t slot = seg.began_before || goes_on ? part_slot(seg.began_before, chunk, a->teams, team)
                                                                      : (int64_t)2 * a->chunks * a->teams + seg.item;
-                    po = a->part_o + (slot * a->slot_rows + kWaveRows * wave) * kR;
-                    pl = a->part_lse + slot * a->slot_rows + kWaveRows * wave;
+                    const int64_t row = slot * a->slot_rows + kWaveRows * wave;
+                    po = a->part_o + row * kR;
+                    pl = a->part_lse + row;
                 }
                 const Lane l(lane);
                 acc_done();
@@ -659,20 +710,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
                     const float lse2 = sum == 0.f ? -INFINITY : m_row[i] - E::kBias + log2f(sum);
                     const int row = 16 * i + l.n16;
-                    if (row >= seg.rows_n) return;
+                    const bool is_row = row < seg.rows_n;
                     if (po != nullptr) {
-                        float *o = po + row * kR + 4 * l.g;
-                        static_for<32>([&](auto db) __attribute__((always_inline)) {
-                            *reinterpret_cast<f32x4 *>(o + 16 * db) = acc_read<db, i>() * inv;
-                        });
-                        if (l.g == 0) pl[row] = lse2;
+                        if (is_row) {
+                            float *o = po + 16 * i * kR + 4 * l.id;
+                            static_for<32>([&](auto db) __attribute__((always_inline)) {
+                                *reinterpret_cast<f32x4 *>(o + 256 * db) = acc_read<db, i>() * inv;
+                            });
+                            if (l.g == 0) pl[row] = lse2;
+                        }
                     } else {
-                        uint16_t *out = static_cast<uint16_t *>(a->out) + (seg.row0 + row) * kR + 4 * l.g;
-                        static_for<32>([&](auto db) __attribute__((always_inline)) {
-                            const f32x4 o = acc_read<db, i>() * inv;
-                            *reinterpret_cast<uint2 *>(out + 16 * db) = make_uint2(E::pack2(o[0], o[1]), E::pack2(o[2], o[3]));
+                        uint16_t *out = static_cast<uint16_t *>(a->out) + (seg.row0 + row) * kR + 16 * (l.g & 1) + 8 * (l.g >> 1);
+                        static_for<16>([&](auto p) __attribute__((always_inline)) {
+                            const u32x4 o = eight_dims<DT>(acc_read<2 * p, i>() * inv, acc_read<2 * p + 1, i>() * inv);
+                            if (is_row) *reinterpret_cast<u32x4 *>(out + 32 * p) = o;
                         });
-                        if (l.g == 0) a->lse[seg.row0 + row] = lse2 * kLn2;
+                        if (is_row && l.g == 0) a->lse[seg.row0 + row] = lse2 * kLn2;
                     }
                 });
                 stored = seg.rows_n > 0;
@@ -740,19 +793,21 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
 }
 
 // Folds the parts of every row that has some, in list order and after the prefix's, and
-// writes rows that see nothing. A wave takes a row: lane p holds the weight of the p-th of 64
-// parts, then 4 + 4 dims of each part in turn, loaded kBatch at a time.
-template <int DT>
+// writes rows that see nothing. A workgroup takes 16 heads of a token, a lane one row and 4 dims
+// of each 16, the part's own layout; kAhead parts are loaded independently of each other. Where
+// the blocks fill the CUs (SHARE false) a wave has 8 x 16 dims of all parts; where they do not, the
+// dims go over 8 workgroups and the parts over 4 waves, which are joined through LDS.
+template <int DT, bool SHARE>
 __global__ __launch_bounds__(256) void latent_combine_kernel(DecodeArgs a) {
-    using E = Elem<DT>;
-    constexpr int kBatch = 6;
-    const int lane = __lane_id();
-    const int r = scalar((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
-    if (r >= a.batch * a.rows) return;
-    const int b = scalar(r / a.rows), rr = r - b * a.rows;
-    const int tok = scalar(rr / a.heads), head = rr - tok * a.heads;
-    const int group = tok * a.head_groups + head / kWaveRows;
-    const int mt = group / 4, row = (group - 4 * mt) * kWaveRows + head % kWaveRows;
+    constexpr int kDb = SHARE ? 4 : 8, kAhead = SHARE ? 4 : 2, kStep = SHARE ? 4 : 1;
+    const int lane = __lane_id(), g = lane >> 4, n16 = lane & 15, wave = scalar((int)threadIdx.x >> 6);
+    const int head_blocks = (a.heads + 15) / 16;
+    const int token = scalar((int)(blockIdx.x / head_blocks)), hb = (int)blockIdx.x - token * head_blocks;
+    const int b = scalar(token / a.q_len), tok = token - b * a.q_len;
+    const int db0 = SHARE ? blockIdx.y * kDb : wave * kDb;
+    const int head = 16 * hb + n16;
+    const int group = tok * a.head_groups + hb / 2, mt = group / 4;
+    const int row = (group - 4 * mt) * kWaveRows + 16 * (hb & 1) + n16;
     const int team = a.teams > 1 ? mt : 0, m = a.teams > 1 ? 0 : mt;
     const int places = scalar((a.sums[b + 1] - a.sums[b]) / a.listed);
 
@@ -777,58 +832,87 @@ __global__ __launch_bounds__(256) void latent_combine_kernel(DecodeArgs a) {
         if (whole && !a.merge) return;  // written by its workgroup
     }
     const int total = splits + parts;
-    // a part's row, in rows of its workspace
-    auto part_row = [&](int p) -> int64_t {
-        if (p < splits) return (int64_t)p * a.prows + r;
-        const int c = c0 + p - splits;
-        const int64_t slot = whole ? (int64_t)2 * a.chunks * a.teams + b * a.listed + m : part_slot(c > c0, c, a.teams, team);
-        return slot * a.slot_rows + row;
-    };
+    const int64_t prow = (int64_t)b * a.heads + min(head, a.heads - 1);  // of the prefix's rows
+    const float *prefix_o = a.ppart_o + ((prow >> 4) * 128 + 4 * db0 + g) * 64 + (prow & 15) * 4;
     float mx = -INFINITY, sum = 0.f;
-    f32x4 acc[2] = {};
-    for (int p0 = 0; p0 < total; p0 += 64) {
-        const int count = min(64, total - p0), p = p0 + min(lane, count - 1);
-        float ls = (p < splits ? a.ppart_lse : a.part_lse)[part_row(p)];
-        if (lane >= count) ls = -INFINITY;
-        float mb = fmaxf(mx, ls);
+    f32x4 acc[kDb] = {};
+    for (int p0 = SHARE ? wave : 0; p0 < total; p0 += kStep * kAhead) {
+        float ls[kAhead];
+        f32x4 o[kAhead][kDb];
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) mb = fmaxf(mb, __shfl_xor(mb, o));
+        for (int j = 0; j < kAhead; ++j) {
+            const int p = min(p0 + j * kStep, total - 1);  // past the last part: it again, not added
+            const float *po;
+            if (p < splits) {
+                ls[j] = a.ppart_lse[(int64_t)p * a.prows_up + prow];
+                po = prefix_o + (int64_t)p * a.prows_up * kR;
+            } else {
+                const int c = c0 + p - splits;
+                const int64_t slot = whole ? (int64_t)2 * a.chunks * a.teams + b * a.listed + m : part_slot(c > c0, c, a.teams, team);
+                ls[j] = a.part_lse[slot * a.slot_rows + row];
+                po = a.part_o + (slot * a.slot_rows + row - n16) * kR + db0 * 256 + 4 * lane;
+            }
+#pragma unroll
+            for (int d = 0; d < kDb; ++d) o[j][d] = *reinterpret_cast<const f32x4 *>(po + d * 256);
+        }
+        float mb = mx;
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            if (p0 + j * kStep >= total) ls[j] = -INFINITY;
+            mb = fmaxf(mb, ls[j]);
+        }
         const float mu = mb == -INFINITY ? 0.f : mb;
-        const float f = exp2_fast(mx - mu), w = exp2_fast(ls - mu);  // a part that saw nothing holds zeros
-        float ws = w;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) ws += __shfl_xor(ws, o);
-        sum = sum * f + ws;
-        acc[0] *= f;
-        acc[1] *= f;
+        const float f = exp2_fast(mx - mu);
         mx = mb;
-        for (int q0 = 0; q0 < count; q0 += kBatch) {
-            f32x4 o[kBatch][2];
+        sum *= f;
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-                if (q0 + j >= count) break;
-                const int q = p0 + q0 + j;
-                const float *po = (q < splits ? a.ppart_o : a.part_o) + part_row(q) * kR + 4 * lane;
-                o[j][0] = *reinterpret_cast<const f32x4 *>(po);
-                o[j][1] = *reinterpret_cast<const f32x4 *>(po + kR / 2);
-            }
+        for (int d = 0; d < kDb; ++d) acc[d] *= f;
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-                if (q0 + j >= count) break;
-                const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), q0 + j));
-                acc[0] += o[j][0] * wj;
-                acc[1] += o[j][1] * wj;
+        for (int j = 0; j < kAhead; ++j)
+            if (p0 + j * kStep < total) {
+                const float w = exp2_fast(ls[j] - mu);  // a part that saw nothing holds zeros
+                sum += w;
+#pragma unroll
+                for (int d = 0; d < kDb; ++d) acc[d] += o[j][d] * w;
             }
+    }
+    const int64_t r = (int64_t)token * a.heads + head;
+    uint16_t *out = static_cast<uint16_t *>(a.out) + r * kR;
+    if constexpr (SHARE) {
+        __shared__ f32x4 part[4][kDb][64];
+        __shared__ float part_mx[4][16], part_sum[4][16];
+#pragma unroll
+        for (int d = 0; d < kDb; ++d) part[wave][d][lane] = acc[d];
+        if (g == 0) {
+            part_mx[wave][n16] = mx;
+            part_sum[wave][n16] = sum;
+        }
+        __syncthreads();
+        // a wave each of the four 16 dims
+        mx = fmaxf(fmaxf(part_mx[0][n16], part_mx[1][n16]), fmaxf(part_mx[2][n16], part_mx[3][n16]));
+        const float mu = mx == -INFINITY ? 0.f : mx;
+        sum = 0.f;
+        f32x4 x = {};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = exp2_fast(part_mx[w][n16] - mu);  // a wave without a part: zeros
+            sum += part_sum[w][n16] * f;
+            x += part[w][wave][lane] * f;
+        }
+        x *= sum == 0.f ? 0.f : 1.0f / sum;
+        using E = Elem<DT>;
+        if (head < a.heads)
+            *reinterpret_cast<uint2 *>(out + 16 * (db0 + wave) + 4 * g) = make_uint2(E::pack2(x[0], x[1]), E::pack2(x[2], x[3]));
+    } else {
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+        for (int d = 0; d < kDb; d += 2) {
+            const u32x4 x = eight_dims<DT>(acc[d] * inv, acc[d + 1] * inv);
+            if (head < a.heads) *reinterpret_cast<u32x4 *>(out + 16 * (db0 + d + (g & 1)) + 8 * (g >> 1)) = x;
         }
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        acc[i] *= inv;
-        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + (int64_t)r * kR + i * (kR / 2) + 4 * lane) =
-            make_uint2(E::pack2(acc[i][0], acc[i][1]), E::pack2(acc[i][2], acc[i][3]));
-    }
-    if (lane == 0) a.lse[r] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+    if (db0 == 0 && wave == 0 && g == 0 && head < a.heads)
+        a.lse[r] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
 }
 
 int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
@@ -837,7 +921,7 @@ int64_t pad256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 // Sizes of a call: the list's and the prefix's partition, and the workspace.
 struct LatentPlan {
     int64_t rows, head_groups, mtiles, teams, listed, chunks, slot_rows, slots;
-    int64_t prows, pmtiles, psplits;
+    int64_t prows, prows_up, pmtiles, psplits;
     int64_t off_lse, off_o, off_plse, off_po, ws_bytes;
 };
 
@@ -860,6 +944,7 @@ int make_plan(int64_t batch, int64_t q_len, int64_t heads, int64_t kv_cap, bool 
     p->slots = 2 * p->chunks * p->teams + (merge ? batch * p->listed : 0);
     p->prows = merge ? batch * heads : 0;
     p->pmtiles = ceil_div(p->prows, kRows);
+    p->prows_up = p->pmtiles * kRows;
     p->psplits = 0;
     if (merge && p->pmtiles > 0) {
         p->psplits = p->pmtiles >= 2 * kGroups ? 1 : 2 * kGroups / p->pmtiles;  // two rounds
@@ -870,11 +955,11 @@ int make_plan(int64_t batch, int64_t q_len, int64_t heads, int64_t kv_cap, bool 
     p->off_lse = at;
     at += pad256(p->slots * p->slot_rows * 4);
     p->off_plse = at;
-    at += pad256(p->psplits * p->prows * 4);
+    at += pad256(p->psplits * p->prows_up * 4);
     p->off_o = at;
     at += p->slots * p->slot_rows * kR * 4;
     p->off_po = at;
-    at += p->psplits * p->prows * kR * 4;
+    at += p->psplits * p->prows_up * kR * 4;
     p->ws_bytes = at;
     return CK_OK;
 }
@@ -887,8 +972,11 @@ int launch(const DecodeArgs &a, hipStream_t s) {
     hipLaunchKernelGGL((latent_decode_kernel<DT>), dim3((unsigned)(a.teams * a.chunks)), dim3(kThreads), kLds, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return static_cast<int>(e);
-    hipLaunchKernelGGL((latent_combine_kernel<DT>), dim3((unsigned)ceil_div((int64_t)a.batch * a.rows, 4)), dim3(256), 0,
-                       s, a);
+    const int64_t blocks = (int64_t)a.batch * a.q_len * ceil_div(a.heads, 16);
+    if (blocks >= kFoldBlocks)
+        hipLaunchKernelGGL((latent_combine_kernel<DT, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((latent_combine_kernel<DT, true>), dim3((unsigned)blocks, 32 / 4), dim3(256), 0, s, a);
     CK_RETURN_LAUNCH();
 }
 
@@ -956,6 +1044,7 @@ int run(const void *q, const void *cache, const int32_t *block_table, int64_t bt
         a.pcols = prefix->cols;
         a.pblocks = prefix->num_blocks;
         a.prows = (int)p.prows;
+        a.prows_up = (int)p.prows_up;
         a.pmtiles = (int)p.pmtiles;
         a.most_splits = (int)p.psplits;
         a.ppart_lse = reinterpret_cast<float *>(ws + p.off_plse);
