@@ -390,6 +390,28 @@ def test_prefill_lengths_past_the_ends():
     assert (out == 0).all() and (lse == -math.inf).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_prefill_hidden_keys_may_hold_anything(dtype, bad):
+    """Keys and values that a query does not see, in its own tiles and in the next request's,
+    change nothing of it; those that do see them show it."""
+    g = _gen(34)
+    ql, kl, at = [100, 70], [100, 70], 65
+    q, k, kr, v = _prompt(g, ql, kl, 2, dtype)
+    good = OPS.latent_prefill(q, k, kr, v, _i64(ql), _i64(kl), SCALE)
+    v[at, 0, 5] = bad
+    v[100:, 1] = bad
+    k[100:, 1] = bad
+    out, lse = OPS.latent_prefill(q, k, kr, v, _i64(ql), _i64(kl), SCALE)
+    assert torch.equal(out[:at], good[0][:at]) and torch.equal(lse[:at * 2], good[1][:at * 2])
+    assert torch.equal(out[:100, 1], good[0][:100, 1])
+    assert not torch.isfinite(out[at:100, 0, 5]).any()
+    rest = [d for d in range(128) if d != 5]
+    assert torch.equal(out[:100, 0][:, rest], good[0][:100, 0][:, rest])
+    if not math.isnan(bad):
+        assert (out[at:100, 0, 5] == bad).all()
+
+
 def test_prefill_rising_scores():
     g = _gen(35)
     q, k, kr, v = _prompt(g, [300], [300], 1, BF)

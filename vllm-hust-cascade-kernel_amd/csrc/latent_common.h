@@ -63,5 +63,29 @@ struct Elem<CK_DTYPE_F16> {
     static constexpr float kBias = 7.f;
 };
 
+// A value that is the same in all lanes, into scalar registers (divisions leave it in vector ones).
+__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t scalar(int64_t x) {
+    return ((int64_t)scalar((int)(x >> 32)) << 32) | (uint32_t)scalar((int)x);
+}
+
+// The largest of three; a NaN among them is passed over.
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    return r;
+}
+
+// 16 bytes per lane from r at voff + soff to LDS at base + IMM + 16 * lane, as dma16_buf, with
+// the place in two scalar instructions: they issue in the shadow of a product, where a vector
+// instruction and its trip to the scalar registers would hold the wave up.
+template <int IMM>
+__device__ __forceinline__ void dma_tile(const ck_rsrc_t &r, int voff, int soff, int base) {
+    asm volatile("s_add_i32 m0, %0, %c1\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds"
+                 :
+                 : "s"(base), "i"(IMM), "v"(voff), "s"(r), "s"(soff)
+                 : "memory", "m0", "scc");
+}
+
 }  // namespace lat
 }  // namespace ck

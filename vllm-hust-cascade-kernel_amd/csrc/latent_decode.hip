@@ -128,19 +128,6 @@ __device__ __forceinline__ int64_t clamp_len(int64_t n, int64_t cols, int64_t nu
 __device__ __forceinline__ int tiles_of(int64_t len) { return (int)((len + kTok - 1) / kTok); }
 __device__ __forceinline__ int places_of(int64_t len) { return len > 0 ? tiles_of(len) + kItemPlaces : 0; }
 
-// A value that is the same in all lanes, into scalar registers (divisions leave it in vector ones).
-__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t scalar(int64_t x) {
-    return ((int64_t)scalar((int)(x >> 32)) << 32) | (uint32_t)scalar((int)x);
-}
-
-// The largest of three; a NaN among them is passed over.
-__device__ __forceinline__ float max3(float x, float y, float z) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
-    return r;
-}
-
 // op over the four lanes n, 16 + n, 32 + n, 48 + n, in each of them: exchanging the odd rows of
 // 16 lanes (then the upper half) of x with the even ones (the lower half) of x leaves one
 // operand in each result.
@@ -166,17 +153,6 @@ typedef const __attribute__((address_space(4))) DecodeArgs *KernArgs;
 __device__ __forceinline__ KernArgs args_again(KernArgs a) {
     asm volatile("" : "+s"(a));
     return a;
-}
-
-// 16 bytes per lane from r at voff + soff to LDS at base + IMM + 16 * lane, as dma16_buf, with
-// the place in two scalar instructions: they issue in the shadow of a product, where a vector
-// instruction and its trip to the scalar registers would hold the wave up.
-template <int IMM>
-__device__ __forceinline__ void dma_tile(const ck_rsrc_t &r, int voff, int soff, int base) {
-    asm volatile("s_add_i32 m0, %0, %c1\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds"
-                 :
-                 : "s"(base), "i"(IMM), "v"(voff), "s"(r), "s"(soff)
-                 : "memory", "m0", "scc");
 }
 
 // ---- O: the accumulation registers -----------------------------------------------------------

@@ -31,9 +31,16 @@ typedef __attribute__((__vector_size__(2 * sizeof(unsigned)))) unsigned u32x2;
 constexpr int kD = 128;            // a head's key part, and its value
 constexpr int kQ = kD + kP;        // query row
 constexpr int kTok = 64;           // keys per tile
-constexpr int kKBytes = kTok * kD * 2;
-constexpr int kRBytes = kTok * kP * 2;
-constexpr int kStage = 2 * kKBytes + kRBytes;  // keys | rotated | values: 40 KB
+// A tile in LDS. Keys: pieces of 4 rows (1 KB, one DMA) 1088 bytes apart, chunk c (16 bytes) of
+// the piece's row i at c ^ i: the 16 rows that a 16-byte read is served for lie in 16 bank groups, and
+// all chunks of a row are two registers and immediates away. Rotated part: pieces of 8 rows 1056
+// bytes apart, chunk c at c ^ (i / 2 % 2). Values: pieces of 4 rows, chunk c at c ^ 4 i, for the
+// transpose reads, which take 4 rows x 64 bytes.
+constexpr int kKPiece = 1024 + 64, kRPiece = 1024 + 32, kVPiece = 1024;
+constexpr int kRAt = kTok / 4 * kKPiece;
+constexpr int kVAt = kRAt + kTok / 8 * kRPiece;
+constexpr int kStage = kVAt + kTok / 4 * kVPiece;  // 41 KB
+static_assert(kRAt % 256 == 0 && kVAt % 256 == 0 && kStage % 256 == 0, "addresses are XORed below bit 8");
 constexpr int kSlots = 3;
 constexpr int kLds = kSlots * kStage + 256;
 constexpr float kSlack = 8.f;
@@ -57,34 +64,24 @@ struct PrefillArgs {
     float *lse;
 };
 
-// 16-byte chunk c of row r: keys and values (256-byte rows) and the rotated part (128-byte
-// rows). Over 16 consecutive rows one chunk lies in 16 distinct bank groups, over 4
-// consecutive rows a 64-byte group in 16.
-__device__ __forceinline__ int swz(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
-__device__ __forceinline__ int kv_off(int r, int c) { return r * (kD * 2) + ((c ^ swz(r)) << 4); }
-__device__ __forceinline__ int rope_off(int r, int c) { return r * (kP * 2) + ((c ^ ((r >> 1) & 7)) << 4); }
+// The 16-bit halves of w that are infinite or NaN, as 0x8000 each: without their sign those are
+// the largest, kGap below the sign bit.
+template <int DT>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    constexpr uint32_t kGap = DT == CK_DTYPE_BF16 ? 0x00800080u : 0x04000400u;
+    return ((w & 0x7fff7fffu) + kGap) & 0x80008000u;
+}
 
-// Sum of x over the threads before this one, and over all (in *total); NW waves.
-template <int NW>
-__device__ __forceinline__ int64_t block_scan(int64_t x, CK_LDS int64_t *room, int64_t *total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int64_t incl = x;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t up = __shfl_up(incl, o);
-        if (lane >= o) incl += up;
-    }
-    __syncthreads();
-    if (lane == 63) room[wave] = incl;
-    __syncthreads();
-    int64_t before = incl - x, all = 0;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-        if (i < wave) before += room[i];
-        all += room[i];
-    }
-    *total = all;
-    return before;
+// Sums of x over the lanes up to each, none above `most`.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x, uint32_t most) {
+    auto add = [&](uint32_t y) { x = min(x + y, most); };
+    add(__builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, false));  // from 1, 2, 4, 8 lanes below in the row
+    add(__builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, false));  // the row before's last, in rows 1 and 3
+    add(__builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, false));  // lane 31's, in the upper half
+    return x;
 }
 
 template <int DT, int NW>
@@ -93,82 +90,79 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     constexpr int kRows = NW * 32;
     constexpr int kBlk = 16 / NW;   // 1-KB DMAs of the keys (and of the values) per wave and tile
     constexpr int kRBlk = 8 / NW;   // and of the rotated part
-    constexpr int kDmas = 2 * kBlk + kRBlk;
     extern __shared__ __attribute__((aligned(16))) char smem_raw[];
     CK_LDS char *smem = (CK_LDS char *)smem_raw;
-    CK_LDS int64_t *room = (CK_LDS int64_t *)(smem + kSlots * kStage);  // [0, 8): scans; [8, 13): the tile
+    CK_LDS int *odd = (CK_LDS int *)(smem + kSlots * kStage);
 
     const int tid = threadIdx.x;
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63;
     const int hh = lane >> 5, n32 = lane & 31;
 
+    // Heads in pairs, a pair's row tiles longest first: an XCD's CUs end together, and its L2 holds
+    // two heads' keys and values.
     const uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
-    const int head = w / a.tiles;
-    const int64_t tile = w % a.tiles;
+    const int pair = scalar((int)(w / (uint32_t)(2 * a.tiles))), in_pair = (int)w - pair * 2 * a.tiles;
+    const bool two = 2 * pair + 1 < a.heads;
+    const int head = 2 * pair + (two ? in_pair & 1 : 0);
+    const uint32_t tile = two ? in_pair >> 1 : in_pair;
 
-    // ---- which request's rows ---------------------------------------------------------------
-    // Thread t looks at requests [t per, t per + per); a pseudo request without keys follows
-    // the last one and takes the rows left.
-    auto len_of = [](const int64_t *lens, int b, int64_t most) {
-        const int64_t n = lens[b];
-        return n < 0 ? (int64_t)0 : n > most ? most : n;
-    };
-    const int per = (a.batch + NW * 64 - 1) / (NW * 64);
-    const int b_lo = min(tid * per, a.batch), b_hi = min(b_lo + per, a.batch);
-    int64_t ql_sum = 0, kl_sum = 0, q_all, k_all, t_all;
-    for (int b = b_lo; b < b_hi; ++b) {
-        ql_sum += len_of(a.q_lens, b, a.tokens);
-        kl_sum += len_of(a.kv_lens, b, a.keys);
-    }
-    int64_t q_at = block_scan<NW>(ql_sum, room, &q_all), k_at = block_scan<NW>(kl_sum, room, &k_all);
-    // rows [min(q_at, tokens), min(q_at + ql, tokens)): what passes the end is cut off
-    auto cut = [](int64_t at, int64_t n, int64_t most) { return min(at + n, most) - min(at, most); };
-    int64_t mine = 0;
+    // ---- which request's rows: each wave by itself, 64 requests at a time ---------------------
+    // What passes the last token or key is cut off; behind the last request follow rows without keys.
+    int64_t q0, k0 = 0;
+    int ql, kl = 0, row0;
     {
-        int64_t at = q_at;
-        for (int b = b_lo; b < b_hi; ++b) {
-            const int64_t n = len_of(a.q_lens, b, a.tokens);
-            mine += (cut(at, n, a.tokens) + kRows - 1) / kRows;
-            at += n;
-        }
-    }
-    int64_t t_at = block_scan<NW>(mine, room, &t_all);
-    if (tile >= t_all) {
-        if (tid == 0) {
-            const int64_t from = min(q_all, a.tokens);
-            room[8] = from;
-            room[9] = a.tokens - from;
-            room[10] = 0;
-            room[11] = 0;
-            room[12] = tile - t_all;
-        }
-    } else {
-        for (int b = b_lo; b < b_hi; ++b) {
-            const int64_t n = len_of(a.q_lens, b, a.tokens), m = len_of(a.kv_lens, b, a.keys);
-            const int64_t rows = cut(q_at, n, a.tokens), nt = (rows + kRows - 1) / kRows;
-            if (tile >= t_at && tile < t_at + nt) {
-                room[8] = q_at;
-                room[9] = rows;
-                room[10] = min(k_at, a.keys);
-                room[11] = cut(k_at, m, a.keys);
-                room[12] = nt - 1 - (tile - t_at);
+        const uint32_t tokens = (uint32_t)a.tokens, keys = (uint32_t)a.keys;
+        auto len_of = [](const int64_t *lens, int b, uint32_t most) {
+            const int64_t n = lens[b];
+            return n < 0 ? 0u : n > most ? most : (uint32_t)n;
+        };
+        uint32_t q_end = 0, k_end = 0, t_end = 0;
+        bool found = false;
+        for (int b0 = 0; b0 < a.batch && !found; b0 += 64) {
+            const int b = b0 + lane;
+            uint32_t n = 0, m = 0;
+            if (b < a.batch) {
+                n = len_of(a.q_lens, b, tokens);
+                m = len_of(a.kv_lens, b, keys);
             }
-            q_at += n;
-            k_at += m;
-            t_at += nt;
+            const uint32_t q_to = min(wave_scan(n, tokens) + q_end, tokens), k_to = min(wave_scan(m, keys) + k_end, keys);
+            // where the request begins: where the one before ends
+            uint32_t q_at = __builtin_amdgcn_update_dpp(0u, q_to, 0x138, 0xf, 0xf, false);  // the lane below's
+            uint32_t k_at = __builtin_amdgcn_update_dpp(0u, k_to, 0x138, 0xf, 0xf, false);
+            if (lane == 0) {
+                q_at = q_end;
+                k_at = k_end;
+            }
+            const uint32_t nt = (q_to - q_at + kRows - 1) / kRows;
+            const uint32_t t_to = wave_scan(nt, ~0u >> 1) + t_end;
+            const uint64_t hit = __builtin_amdgcn_ballot_w64(tile < t_to);
+            if (hit) {
+                const int from = (int)__ffsll((unsigned long long)hit) - 1;
+                auto of = [&](uint32_t x) { return (int)__builtin_amdgcn_readlane(x, from); };
+                q0 = of(q_at);
+                ql = of(q_to - q_at);
+                k0 = of(k_at);
+                kl = of(k_to - k_at);
+                row0 = (of(t_to) - 1 - (int)tile) * kRows;  // the last first: under a causal mask the longest
+                found = true;
+            }
+            q_end = __builtin_amdgcn_readlane(q_to, 63);
+            k_end = __builtin_amdgcn_readlane(k_to, 63);
+            t_end = __builtin_amdgcn_readlane(t_to, 63);
+        }
+        if (!found) {
+            q0 = q_end;
+            ql = (int)(tokens - q_end);
+            row0 = (int)(tile - t_end) * kRows;
         }
     }
-    __syncthreads();
-    const int64_t q0 = room[8], k0 = room[10];
-    const int ql = __builtin_amdgcn_readfirstlane((int)room[9]), kl = __builtin_amdgcn_readfirstlane((int)room[11]);
-    const int row0 = __builtin_amdgcn_readfirstlane((int)room[12]) * kRows;
     if (row0 >= ql) return;  // the same in every thread
 
     const int wrow0 = row0 + wid * 32;
     const int i_q = wrow0 + n32;
     const bool row_valid = i_q < ql;
-    const int64_t qrow = (q0 + i_q) * a.heads + head;
+    const int64_t qrow = (q0 + min(i_q, ql - 1)) * a.heads + head;
     // keys seen by this lane's query, by the wave's first and last, and by the workgroup's last
     auto seen = [&](int i) { return a.causal ? max(0, min(kl, kl - ql + 1 + i)) : kl; };
     const int limit = row_valid ? seen(i_q) : 0;
@@ -177,41 +171,67 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     const int most = seen(min(row0 + kRows - 1, ql - 1));
     const int ntiles = (most + kTok - 1) / kTok;
 
-    u32x4 qf[12];
-#pragma unroll
-    for (int kk = 0; kk < 12; ++kk) {
-        qf[kk] = u32x4{0, 0, 0, 0};
-        if (row_valid) qf[kk] = *reinterpret_cast<const u32x4 *>(a.q + qrow * kQ + 16 * kk + 8 * hh);
-    }
-
     // ---- DMA ----------------------------------------------------------------------------------
-    // 1-KB block j of a wave: 4 rows of keys or values, 8 rows of the rotated part
-    uint32_t k_dma[kBlk], v_dma[kBlk], r_dma[kRBlk];
-#pragma unroll
-    for (int j = 0; j < kBlk; ++j) {
-        const int r = (wid * kBlk + j) * 4 + (lane >> 4), c = (lane & 15) ^ swz(r);
-        k_dma[j] = (uint32_t)(r * a.k_ts + c * 8) * 2;
-        v_dma[j] = (uint32_t)(r * a.v_ts + c * 8) * 2;
-    }
-#pragma unroll
-    for (int j = 0; j < kRBlk; ++j) {
-        const int r = (wid * kRBlk + j) * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-        r_dma[j] = (uint32_t)(r * a.kr_ts + c * 8) * 2;
-    }
-    auto issue = [&](int t, int slot) {
-        const int64_t at = k0 + (int64_t)t * kTok;
-        const int n = min(kTok, kl - t * kTok);  // rows of the request in this tile
-        const ck_rsrc_t rk = buf_rsrc(a.k + at * a.k_ts + head * a.k_hs, (uint32_t)((n - 1) * a.k_ts + kD) * 2);
-        const ck_rsrc_t rr = buf_rsrc(a.kr + at * a.kr_ts, (uint32_t)((n - 1) * a.kr_ts + kP) * 2);
-        const ck_rsrc_t rv = buf_rsrc(a.v + at * a.v_ts + head * a.v_hs, (uint32_t)((n - 1) * a.v_ts + kD) * 2);
-        CK_LDS char *dst = smem + slot * kStage;
+    // The wave's pieces: rows 4 (kBlk wid + j) .. + 3 of keys and values, 8 (kRBlk wid + j) .. + 7 of
+    // the rotated part.
+    const int p_i = lane >> 4, r_i = lane >> 3;  // the lane's row in a piece
+    const uint32_t k_dma = (uint32_t)((wid * kBlk * 4 + p_i) * a.k_ts + ((lane & 15) ^ p_i) * 8) * 2;
+    const uint32_t v_dma = (uint32_t)((wid * kBlk * 4 + p_i) * a.v_ts + ((lane & 15) ^ (4 * p_i)) * 8) * 2;
+    const uint32_t r_dma = (uint32_t)((wid * kRBlk * 8 + r_i) * a.kr_ts + ((lane & 7) ^ ((r_i >> 1) & 1)) * 8) * 2;
+    // The next tile that is moved: where it begins, and the request's rows from there on. Bytes past
+    // those are not read; past the last tile nothing comes, but as many DMAs are counted.
+    uint64_t k_from = (uint64_t)(uintptr_t)(a.k + k0 * a.k_ts + head * a.k_hs);
+    uint64_t r_from = (uint64_t)(uintptr_t)(a.kr + k0 * a.kr_ts);
+    uint64_t v_from = (uint64_t)(uintptr_t)(a.v + k0 * a.v_ts + head * a.v_hs);
+    const uint32_t k_row = 2 * (uint32_t)a.k_ts, r_row = 2 * (uint32_t)a.kr_ts, v_row = 2 * (uint32_t)a.v_ts;
+    int left = kl;
+    const int lds0 = scalar((int)(uintptr_t)smem);
+    auto issue = [&](int slot) {
+        const int more = min(kTok, left) - 1;
+        auto from = [&](uint64_t at, uint32_t row, int width) {
+            ck_rsrc_t r;
+            r[0] = (int)(uint32_t)at;
+            r[1] = (int)((uint32_t)(at >> 32) & 0xffffu);
+            r[2] = more >= 0 ? (int)(more * row + 2 * width) : 0;
+            r[3] = 0x00020000;
+            return r;
+        };
+        const ck_rsrc_t rk = from(k_from, k_row, kD), rr = from(r_from, r_row, kP), rv = from(v_from, v_row, kD);
+        const int to = lds0 + slot * kStage;
+        static_for<kBlk>([&](auto j) __attribute__((always_inline)) {
+            dma_tile<j * kKPiece>(rk, (int)(k_dma + j * 4 * k_row), 0, to + wid * (kBlk * kKPiece));
+            dma_tile<kVAt + j * kVPiece>(rv, (int)(v_dma + j * 4 * v_row), 0, to + wid * (kBlk * kVPiece));
+        });
+        static_for<kRBlk>([&](auto j) __attribute__((always_inline)) {
+            dma_tile<kRAt + j * kRPiece>(rr, (int)(r_dma + j * 8 * r_row), 0, to + wid * (kRBlk * kRPiece));
+        });
+        k_from += (uint64_t)kTok * k_row;
+        r_from += (uint64_t)kTok * r_row;
+        v_from += (uint64_t)kTok * v_row;
+        left -= kTok;
+    };
+    // What this wave has moved of tile t is in. Where not every query of the workgroup sees all of it,
+    // the values that 0 * V must not make NaN: past the request's end they become zeros; infinite or
+    // NaN ones set the tile's bit in *odd.
+    const int w_first = scalar(seen(row0)), first_odd = w_first / kTok;
+    auto is_odd = [&](int t) { return ((scalar(*odd) >> (t - first_odd)) & 1) != 0; };
+    auto look = [&](int t, int slot) {
+        if (t * kTok + kTok <= w_first) return;
+        int l = tid & 63;
+        asm volatile("" : "+v"(l));
+        uint32_t bad = 0;
 #pragma unroll
         for (int j = 0; j < kBlk; ++j) {
-            dma16_buf(rk, (int)k_dma[j], 0, dst + (wid * kBlk + j) * 1024);
-            dma16_buf(rv, (int)v_dma[j], 0, dst + kKBytes + kRBytes + (wid * kBlk + j) * 1024);
+            const int r = (wid * kBlk + j) * 4 + (l >> 4);
+            CK_LDS u32x4 *at = reinterpret_cast<CK_LDS u32x4 *>(smem + slot * kStage + kVAt + (wid * kBlk + j) * kVPiece + l * 16);
+            if (t * kTok + r < kl) {
+                const u32x4 x = *at;
+                bad |= not_finite<DT>(x[0]) | not_finite<DT>(x[1]) | not_finite<DT>(x[2]) | not_finite<DT>(x[3]);
+            } else {
+                *at = u32x4{0, 0, 0, 0};
+            }
         }
-#pragma unroll
-        for (int j = 0; j < kRBlk; ++j) dma16_buf(rr, (int)r_dma[j], 0, dst + kKBytes + (wid * kRBlk + j) * 1024);
+        if (bad != 0) __hip_atomic_fetch_or(odd, 1 << (t - first_odd), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     };
 
     f32x16 oacc[4];
@@ -219,124 +239,238 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int i = 0; i < 16; ++i) oacc[db][i] = 0.f;
-    float m_run = -INFINITY, l_part = 0.f;
+    float m_run = -INFINITY, sub = -E::kBias, l_part = 0.f;
+    bool fresh = true;  // O is zero
 
-    const int trG = (lane >> 4) & 3, tr_row = (lane & 15) >> 2, tr_e4 = lane & 3;
-    auto vt_off = [&](int s16, int db, int second) {
-        const int t1 = 16 * s16 + 4 * (trG >> 1) + tr_row + 8 * second;
-        const int d = 32 * db + 16 * (trG & 1) + 4 * tr_e4;
-        return kv_off(t1, d >> 3) + (d & 7) * 2;
+    // A lane's place in a tile: of keys n32 (+ 32), chunk hh, and their rotated part; of values by
+    // transpose reads. (That of the rotated part is found again in every step: with it a register
+    // would spill, whose reload waits for the DMAs.)
+    auto rope_at = [&]() {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        return kRAt + ((l >> 3) & 3) * kRPiece + (l & 7) * 128 + ((l >> 5) ^ ((l >> 1) & 1)) * 16;
     };
+    const int trG = (lane >> 4) & 3, tr_row = (lane & 15) >> 2, tr_e4 = lane & 3;
+    const int key_at = (n32 >> 2) * kKPiece + (n32 & 3) * 256 + ((hh ^ n32) & 3) * 16;
+    const int value_at = kVAt + (trG >> 1) * kVPiece + tr_row * 256 + (4 * tr_row + 2 * (trG & 1) + (tr_e4 >> 1)) * 16 + (tr_e4 & 1) * 8;
 
-    wait_vmcnt<0>();
-    for (int t = 0; t < kSlots - 1 && t < ntiles; ++t) issue(t, t);
-    int slot = 0;
-    for (int t = 0; t < ntiles; ++t) {
-        if (t + 1 < ntiles) wait_vmcnt<kDmas>();
-        else wait_vmcnt<0>();
-        const int nv = kl - t * kTok;  // rows of the request from here on
-        CK_LDS char *kb = smem + slot * kStage, *rbuf = kb + kKBytes, *vb = rbuf + kRBytes;
-        if (nv < kTok) {  // values past the request's end, in this wave's blocks: 0 * V must not be NaN
+    u32x4 qf[12];
+    // S^T = K Q^T of the tile in `slot`; between(f) is placed after the f-th product.
+    auto scores = [&](int slot, f32x16 (&x)[2], auto &&between) __attribute__((always_inline)) {
+        const CK_LDS char *tile = smem + slot * kStage;
+        const CK_LDS char *k_even = tile + key_at, *k_odd = tile + (key_at ^ 32), *rope = tile + rope_at();
+        auto kfrag = [&](int f) {
+            const int ks = f >> 1;
+            return *reinterpret_cast<const CK_LDS u32x4 *>(
+                ks < 8 ? (ks & 1 ? k_odd : k_even) + (ks >> 1) * 64 + (f & 1) * 8 * kKPiece
+                       : rope + (ks - 8) * 32 + (f & 1) * 4 * kRPiece);
+        };
+        constexpr int kAhead = 3, kHeld = kAhead + 1;
+        const f32x16 zero16 = {};
+        u32x4 kf[kHeld];
 #pragma unroll
-            for (int j = 0; j < kBlk; ++j)
-                if ((wid * kBlk + j) * 4 + (lane >> 4) >= nv)
-                    *reinterpret_cast<CK_LDS u32x4 *>(vb + (wid * kBlk + j) * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
-        }
-        __syncthreads();  // tile t is in; every wave is done with tile t - 1, whose slot is next
-        if (t + 2 < ntiles) issue(t + 2, slot == 0 ? 2 : slot - 1);
-        slot = slot == 2 ? 0 : slot + 1;
-        if (t * kTok >= w_most) continue;  // the wave's queries see none of it
-
-        f32x16 sb[2];
-        {
-            const f32x16 zero16 = {};
-            auto kfrag = [&](int f) {
-                const int r = 32 * (f & 1) + n32, ks = f >> 1;
-                return *reinterpret_cast<const CK_LDS u32x4 *>(ks < 8 ? kb + kv_off(r, 2 * ks + hh)
-                                                                      : rbuf + rope_off(r, 2 * (ks - 8) + hh));
-            };
-            constexpr int kAhead = 4;
-            u32x4 kfr[kAhead];
-#pragma unroll
-            for (int f = 0; f < kAhead; ++f) kfr[f] = kfrag(f);
+        for (int f = 0; f < kAhead; ++f) kf[f] = kfrag(f);
+        __builtin_amdgcn_sched_barrier(0);
+        static_for<24>([&](auto f) __attribute__((always_inline)) {
+            x[f & 1] = E::mfma32(kf[f % kHeld], qf[f >> 1], f < 2 ? zero16 : x[f & 1]);
+            if (f + kAhead < 24) kf[(f + kAhead) % kHeld] = kfrag(f + kAhead);
+            between(f);
             __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    u32x4 pb[4];
+    // The lane's 32 probabilities in pairs: begun, and a product later, when the exponentials are
+    // there, summed and packed (left for the end, the 32 would need twice the registers).
+    float p0, p1;
+    auto p_begin = [&](const f32x16 (&x)[2], int pair) __attribute__((always_inline)) {
+        const int q2 = pair >> 3, j = pair & 7;
+        p0 = exp2_fast(fmaf(x[q2][2 * j], a.scale_log2, -sub));
+        p1 = exp2_fast(fmaf(x[q2][2 * j + 1], a.scale_log2, -sub));
+    };
+    auto p_end = [&](int pair) __attribute__((always_inline)) {
+        const int q2 = pair >> 3, j = pair & 7;
+        l_part += p0;
+        l_part += p1;
+        uint32_t both = E::pack2(p0, p1);
+        asm volatile("" : "+v"(both));
+        pb[2 * q2 + (j >> 2)][j & 3] = both;
+    };
+    // Values' fragment: keys 16 s .. + 15 of the tile, dims 32 db .. + 31.
+    auto vfrag = [&](int slot, int s, int db) __attribute__((always_inline)) {
+        const CK_LDS char *at = smem + slot * kStage + (value_at ^ (db * 64)) + s * 4 * kVPiece;
+        const uint2 lo = lds_read_tr16(at), hi = lds_read_tr16(at + 2 * kVPiece);
+        return u32x4{lo.x, lo.y, hi.x, hi.y};
+    };
+    // O^T += V^T P^T.
+    auto products = [&](auto ahead, int slot, auto &&clean, auto &&between) __attribute__((always_inline)) {
+        constexpr int kAhead = ahead, kHeld = kAhead + 1;
+        u32x4 vf[kHeld];
 #pragma unroll
-            for (int f = 0; f < 24; ++f) {
-                sb[f & 1] = E::mfma32(kfr[f % kAhead], qf[f >> 1], f < 2 ? zero16 : sb[f & 1]);
-                if (f + kAhead < 24) kfr[f % kAhead] = kfrag(f + kAhead);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        if (t * kTok + kTok > w_least) {
+        for (int i = 0; i < kAhead; ++i) vf[i] = vfrag(slot, i >> 2, i & 3);
+        __builtin_amdgcn_sched_barrier(0);
+        static_for<16>([&](auto i) __attribute__((always_inline)) {
+            clean(vf[i % kHeld]);
+            oacc[i & 3] = E::mfma32(vf[i % kHeld], pb[i >> 2], oacc[i & 3]);
+            if (i + kAhead < 16) vf[(i + kAhead) % kHeld] = vfrag(slot, (i + kAhead) >> 2, (i + kAhead) & 3);
+            between(i);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    auto nothing = [](auto &&...) {};
+    float v = -INFINITY;  // the query's largest score of the lane's keys
+    auto largest = [&](const f32x16 (&x)[2]) {
+        v = max3(x[0][0], x[0][1], x[0][2]);
 #pragma unroll
-            for (int q2 = 0; q2 < 2; ++q2)
+        for (int e = 3; e < 31; e += 2) v = max3(v, x[e >> 4][e & 15], x[(e + 1) >> 4][(e + 1) & 15]);
+        v = max_xor32(fmaxf(v, x[1][15])) * a.scale_log2;
+    };
+    auto next_slot = [](int slot) { return slot == kSlots - 1 ? 0 : slot + 1; };
+
+    issue(0);
+    // Q in pieces of 8 rows x 128 bytes, turned into operands (row n32, chunk 2 kk + hh) through the
+    // wave's 4 KB of the slot that is used last: an operand's own place, 64 lanes in 32 rows, costs a
+    // cycle a lane, 6100 for a workgroup. A row past the last repeats it: it is not stored.
+    if (wrow0 < ql) {
+        const uint16_t *q = a.q + (q0 * a.heads + head) * kQ + 8 * (lane & 7);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int tok = t * kTok + 32 * q2 + (e & 3) + 8 * (e >> 2) + 4 * hh;
-                    if (tok >= limit) sb[q2][e] = -INFINITY;
-                }
-        }
-        float smax = -INFINITY;
+        for (int e = 0; e < 4; ++e) {
+            const uint16_t *row = q + (int64_t)min(wrow0 + 8 * e + (lane >> 3), ql - 1) * a.heads * kQ;
 #pragma unroll
-        for (int q2 = 0; q2 < 2; ++q2)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) smax = fmaxf(smax, sb[q2][e]);
-        smax = max_xor32(smax) * a.scale_log2;
-        const bool moves = smax > m_run + kSlack;
-        if (__builtin_amdgcn_ballot_w64(moves)) {
-            const float dm = moves ? exp2_fast(m_run - smax) : 1.f;
-            if (moves) m_run = smax;
-            l_part *= dm;
-#pragma unroll
-            for (int db = 0; db < 4; ++db)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) oacc[db][e] *= dm;
-        }
-        const float sub = (m_run == -INFINITY ? 0.f : m_run) - E::kBias;
-        float ls = 0.f;
-        u32x4 pb[4];
-#pragma unroll
-        for (int q2 = 0; q2 < 2; ++q2) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float pv = exp2_fast(fmaf(sb[q2][e], a.scale_log2, -sub));
-                sb[q2][e] = pv;
-                ls += pv;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) pb[2 * q2 + (j >> 2)][j & 3] = E::pack2(sb[q2][2 * j], sb[q2][2 * j + 1]);
-        }
-        l_part += ls;
-        // O^T += V^T P^T, V^T fragments read one 16-key group ahead
-        {
-            uint2 vlo[2][4], vhi[2][4];
-#pragma unroll
-            for (int db = 0; db < 4; ++db) {
-                vlo[0][db] = lds_read_tr16(vb + vt_off(0, db, 0));
-                vhi[0][db] = lds_read_tr16(vb + vt_off(0, db, 1));
-            }
-#pragma unroll
-            for (int s16 = 0; s16 < 4; ++s16) {
-                if (s16 + 1 < 4) {
-#pragma unroll
-                    for (int db = 0; db < 4; ++db) {
-                        vlo[(s16 + 1) & 1][db] = lds_read_tr16(vb + vt_off(s16 + 1, db, 0));
-                        vhi[(s16 + 1) & 1][db] = lds_read_tr16(vb + vt_off(s16 + 1, db, 1));
-                    }
-                }
-#pragma unroll
-                for (int db = 0; db < 4; ++db) {
-                    const uint2 lo = vlo[s16 & 1][db], hi = vhi[s16 & 1][db];
-                    oacc[db] = E::mfma32(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[s16], oacc[db]);
-                }
-            }
+            for (int m = 0; m < 3; ++m) qf[4 * m + e] = *reinterpret_cast<const u32x4 *>(row + 64 * m);
         }
     }
+    wait_vmcnt<0>();
+    issue(1);
+    if (wrow0 < ql) {
+        CK_LDS char *at = smem + (kSlots - 1) * kStage + wid * 4096;
+        auto piece = [&](int row, int chunk) {
+            return reinterpret_cast<CK_LDS u32x4 *>(at + row * 128 + ((chunk ^ (row >> 1)) & 7) * 16);
+        };
+#pragma unroll
+        for (int m = 0; m < 3; ++m) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *piece(8 * e + (lane >> 3), lane & 7) = qf[4 * m + e];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qf[4 * m + e] = *piece(n32, 2 * e + hh);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // before tile 2 is moved there
+    }
+    if (tid == 0) *odd = 0;
+    __syncthreads();
+    look(0, 0);
+    __syncthreads();
+    int slot = 0, t = 0;  // tile t's
+    // A step: P of tile t (scores x) beside the scores y of tile t + 1, then the products of tile t
+    // beside the largest of y: the matrix cores wait for neither.
+    auto step = [&](f32x16 (&x)[2], f32x16 (&y)[2]) __attribute__((always_inline)) {
+        const int s1 = next_slot(slot), s2 = next_slot(s1);
+        wait_vmcnt<0>();
+        look(t + 1, s1);
+        __syncthreads();  // tile t + 1 is in; every wave is done with tile t - 1, whose slot is next
+        issue(s2);
+        const int first = t * kTok;
+        if (first < w_most) {
+            const bool hides = first + kTok > w_least;
+            if (hides) {
+                int half = hh;  // again: what it gives is not to be held over the steps
+                asm volatile("" : "+v"(half));
+#pragma unroll
+                for (int q2 = 0; q2 < 2; ++q2)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (first + 32 * q2 + (e & 3) + 8 * (e >> 2) + 4 * half >= limit) x[q2][e] = -INFINITY;
+                largest(x);
+            }
+            if (__builtin_amdgcn_ballot_w64(v > m_run + kSlack)) {
+                const bool mine = v > m_run + kSlack;
+                const float dm = mine ? exp2_fast(m_run - v) : 1.f;
+                if (mine) m_run = v;
+                l_part *= dm;
+                sub = (m_run == -INFINITY ? 0.f : m_run) - E::kBias;
+                if (!fresh) {
+#pragma unroll
+                    for (int db = 0; db < 4; ++db)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) oacc[db][e] *= dm;
+                }
+            }
+            fresh = false;
+            if (first + kTok < w_most) {
+                scores(s1, y, [&](auto f) __attribute__((always_inline)) {
+                    if constexpr (f % 3 != 0) {
+                        constexpr int pair = f - 1 - f / 3;
+                        if constexpr (pair > 0) p_end(pair - 1);
+                        p_begin(x, pair);
+                    }
+                });
+                p_end(15);
+            } else {
+                // unlike the scores above: their exponents are to be made beside the products there, not before
+                asm volatile("" : "+v"(x[0]), "+v"(x[1]));
+                static_for<16>([&](auto i) __attribute__((always_inline)) {
+                    p_begin(x, i);
+                    p_end(i);
+                });
+                asm volatile("" : "=v"(y[0]), "=v"(y[1]));  // not looked at
+            }
+            if (!hides || !is_odd(t)) {
+                products(std::integral_constant<int, 3>{}, slot, nothing, [&](auto i) __attribute__((always_inline)) {
+                    if constexpr (i == 0) v = max3(y[0][0], y[0][1], y[0][2]);
+                    else if constexpr (i < 15) v = max3(v, y[(2 * i + 1) >> 4][(2 * i + 1) & 15], y[(2 * i + 2) >> 4][(2 * i + 2) & 15]);
+                    else v = max_xor32(fmaxf(v, y[1][15])) * a.scale_log2;
+                });
+            } else {
+                // Infinite and NaN values are zeros here, where 0 * inf would reach queries that do not see
+                // them; those that do take them at the end.
+                products(std::integral_constant<int, 1>{}, slot, [](u32x4 &f) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f[i] &= ~((not_finite<DT>(f[i]) >> 15) * 0xffffu);
+                }, nothing);
+                largest(y);
+            }
+        } else {
+            asm volatile("" : "=v"(y[0]), "=v"(y[1]));
+        }
+        slot = s1;
+        ++t;
+    };
+    f32x16 s[2], y[2];
+    asm volatile("" : "=v"(y[0]), "=v"(y[1]));
+    if (w_most > 0) {
+        scores(0, s, nothing);
+        largest(s);
+    } else {
+        asm volatile("" : "=v"(s[0]), "=v"(s[1]));
+    }
+    while (true) {
+        step(s, y);
+        if (t >= ntiles) break;
+        step(y, s);
+        if (t >= ntiles) break;
+    }
+    wait_vmcnt<0>();  // the empty moves too
 
     // ---- normalise, write whole rows through the idle ring ----------------------------------
     const float l_run = l_part + __shfl_xor(l_part, 32);
     __syncthreads();  // every wave is past its last ring read
     if (wrow0 >= ql) return;
+    // Infinite and NaN values of the tiles that had them, for the queries that see them (whose p is
+    // positive): as they are, no finite weight or sum changes what they give.
+    for (int t = w_least / kTok; t * kTok < w_most; ++t) {
+        if (!is_odd(t)) continue;
+        for (int k = 0; k < kTok; ++k) {
+            if (t * kTok + k >= limit) break;
+            const uint16_t *row = a.v + (k0 + t * kTok + k) * a.v_ts + head * a.v_hs + 4 * hh;
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+                const u32x2 w = *reinterpret_cast<const u32x2 *>(row + 8 * c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (not_finite<DT>(w[j >> 1]) & (j & 1 ? 0x80000000u : 0x8000u))
+                        oacc[c >> 2][4 * (c & 3) + j] += j & 1 ? E::hi(w[j >> 1]) : E::lo(w[j >> 1]);
+            }
+        }
+    }
     // l is 0 where nothing was seen (or every score was -inf)
     const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
     if (row_valid && hh == 0)
