@@ -69,6 +69,18 @@ __device__ __forceinline__ int64_t scalar(int64_t x) {
     return ((int64_t)scalar((int)(x >> 32)) << 32) | (uint32_t)scalar((int)x);
 }
 
+// Sums of x over the lanes up to each, none above `most`.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x, uint32_t most) {
+    auto add = [&](uint32_t y) { x = min(x + y, most); };
+    add(__builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, false));  // from 1, 2, 4, 8 lanes below in the row
+    add(__builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, false));  // the row before's last, in rows 1 and 3
+    add(__builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, false));  // lane 31's, in the upper half
+    return x;
+}
+
 // The largest of three; a NaN among them is passed over.
 __device__ __forceinline__ float max3(float x, float y, float z) {
     float r;

@@ -61,7 +61,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kPieces = 9;    // DMAs per wave and tile: 8 rows of the latent, and their rotated dims
 constexpr int kPhase = 256;   // tiles described in LDS at a time
 constexpr int kGroups = 256;  // workgroups: one per CU
-constexpr int kMinPlaces = 4;  // least places of the list per chunk
+constexpr int kMinPlaces = 2;  // least places of the list per chunk
 constexpr int kFoldBlocks = 256;
 constexpr float kSlack = 8.f;
 
@@ -219,11 +219,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
 
     // ---- the list: this thread's requests, their first tile, the total --------------------
     auto first_request = [](KernArgs a, int t) {
-        return (int)min((int64_t)t * ((a->batch + kThreads - 1) / kThreads), (int64_t)a->batch);
+        return min(t * ((a->batch + kThreads - 1) / kThreads), a->batch);  // batch is at most 2^24
     };
     auto len_of = [](KernArgs a, int b) { return (int)clamp_len(a->lens[b], a->bt_cols, a->num_blocks); };
     CK_LDS int *starts = (CK_LDS int *)(smem + kLdsStart), *len0 = (CK_LDS int *)(smem + kLdsLen);
     int total = 0;
+    const int64_t plen = first_args->merge ? *first_args->plen : 0;
     {
         int mine = 0;
         const int b0 = first_request(first_args, first_tid), b1 = first_request(first_args, first_tid + 1);
@@ -232,12 +233,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             if (b == b0) len0[first_tid] = len;
             mine += places_of(len) * first_args->listed;
         }
-        int incl = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int up = __shfl_up(incl, o);
-            if (lane >= o) incl += up;
-        }
+        const int incl = (int)wave_scan((uint32_t)mine, 0x7fffffffu);
         if (lane == 63) scan[wave] = incl;
         if (first_tid == 0) *bad = 0;
         __syncthreads();
@@ -254,9 +250,20 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     // ---- this workgroup's share ------------------------------------------------------------
     int ptiles = 0, unit_tiles = 0, units = 0, splits = 0;
     if (first_args->merge) {
-        ptiles = scalar(tiles_of(clamp_len(*first_args->plen, first_args->pcols, first_args->pblocks)));
+        ptiles = scalar(tiles_of(clamp_len(plen, first_args->pcols, first_args->pblocks)));
         if (ptiles > 0) {
-            splits = scalar(prefix_splits(first_args->pmtiles, ptiles, total, kGroups, min(first_args->most_splits, ptiles)));
+            // a choice per lane
+            const Split mine = split_choice(lane & (kSplitChoices - 1), first_args->pmtiles, ptiles, total, kGroups,
+                                            min(first_args->most_splits, ptiles));
+            auto of = [&](int i) {
+                return Split{__builtin_amdgcn_readlane(mine.splits, i),
+                             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine.end), i))};
+            };
+            Split best = of(0);
+#pragma unroll
+            for (int i = 1; i < kSplitChoices; ++i)
+                if (better(of(i), best)) best = of(i);
+            splits = best.splits;
             unit_tiles = scalar((ptiles + splits - 1) / splits);
             units = first_args->pmtiles * splits;
         }

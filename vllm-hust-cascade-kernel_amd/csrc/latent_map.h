@@ -77,28 +77,24 @@ CK_HD int64_t part_slot(bool began_before, int n, int teams, int team) {
 // How often the prefix's tiles are split, for `row_tiles` row tiles beside a list of w places.
 // A split more shortens the units, but adds a part to fold for each row. Tried are one, what
 // fills the prefix's share of one round of the workgroups (the list takes the others), one round
-// and two, and taken is the one after which the last workgroup ends first.
-CK_HD int prefix_splits(int row_tiles, int tiles, int w, int groups, int most) {
+// and two, and taken is the one after which the last workgroup ends first, the first of equals.
+constexpr int kSplitChoices = 4;
+struct Split {
+    int splits;
+    float end;
+};
+CK_HD Split split_choice(int i, int row_tiles, int tiles, int w, int groups, int most) {
     const float work = (float)row_tiles * (float)tiles;
-    const float share = (float)groups * work / (work + (float)w);
-    int best = 1;
-    float least = 0.f;
-    for (int i = 0; i < 4; ++i) {
-        const float room = i == 0 ? 0.f : i == 1 ? share : (float)((i - 1) * groups);
-        int s = (int)(room / (float)row_tiles);
-        s = s < 1 ? 1 : s > most ? most : s;
-        const int units = row_tiles * s, each = (tiles + s - 1) / s + kItemPlaces;
-        const float rounds = (float)((units + groups - 1) / groups) * (float)each;
-        const float left = rounds * (float)groups - (float)units * (float)each;
-        // a list that the others do not hold is cut over all of them once more
-        const float end = (float)w <= left ? rounds : rounds + ((float)w - left) / (float)groups + (float)kItemPlaces;
-        if (i == 0 || end < least) {
-            best = s;
-            least = end;
-        }
-    }
-    return best;
+    const float room = i == 0 ? 0.f : i == 1 ? (float)groups * work / (work + (float)w) : (float)((i - 1) * groups);
+    int s = (int)(room / (float)row_tiles);
+    s = s < 1 ? 1 : s > most ? most : s;
+    const int units = row_tiles * s, each = (tiles + s - 1) / s + kItemPlaces;
+    const float rounds = (float)((units + groups - 1) / groups) * (float)each;
+    const float left = rounds * (float)groups - (float)units * (float)each;
+    // a list that the others do not hold is cut over all of them once more
+    return Split{s, (float)w <= left ? rounds : rounds + ((float)w - left) / (float)groups + (float)kItemPlaces};
 }
+CK_HD bool better(const Split &x, const Split &than) { return x.end < than.end; }
 
 }  // namespace lat
 }  // namespace ck

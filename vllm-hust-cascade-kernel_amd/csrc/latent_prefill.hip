@@ -72,18 +72,6 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
     return ((w & 0x7fff7fffu) + kGap) & 0x80008000u;
 }
 
-// Sums of x over the lanes up to each, none above `most`.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x, uint32_t most) {
-    auto add = [&](uint32_t y) { x = min(x + y, most); };
-    add(__builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, false));  // from 1, 2, 4, 8 lanes below in the row
-    add(__builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, false));
-    add(__builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, false));
-    add(__builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, false));
-    add(__builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, false));  // the row before's last, in rows 1 and 3
-    add(__builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, false));  // lane 31's, in the upper half
-    return x;
-}
-
 template <int DT, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void latent_prefill_kernel(PrefillArgs a) {
     using E = Elem<DT>;
