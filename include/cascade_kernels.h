@@ -295,7 +295,9 @@ int ck_add_rms_norm_stats(const void *x1, const void *x2, const void *gamma, con
  * [num_blocks, 128, 576] contiguous, token j of request b is row j % 128 of page
  * block_table[b * bt_cols + j / 128]; a page id outside the pool reads as zero rows.
  * kv lengths are clamped to [0, bt_cols * 128]. Rows of a page past a length may hold
- * anything. bt_cols * 128 is at most 2^30 and num_blocks at most 2^31.
+ * anything. bt_cols * 128 is at most 2^30 and num_blocks at most 2^31; a call's tiles
+ * (ceil(bt_cols * 128 / 32) + 3 a request, and per 128 rows where a prefix is shared) stay
+ * below 2^31.
  * ========================================================================== */
 
 /* ----------------------------------------------------------------------------
@@ -344,7 +346,7 @@ int ck_latent_decode(const void *q, const void *cache, const int32_t *block_tabl
 /* ----------------------------------------------------------------------------
  * The same for batch single-token queries that share a prefix: each attends to the
  * prefix (one request: block table [1, prefix_bt_cols], length int64 [1] on the device)
- * and then to its own suffix. The prefix is read once per 64 (sequence, head) rows; the
+ * and then to its own suffix. The prefix is read once per 128 (sequence, head) rows; the
  * parts are folded in fp32. Either may be empty (both: out = 0, lse = -inf); the two
  * pools may be one. Arguments otherwise as above.
  * -------------------------------------------------------------------------- */
@@ -372,7 +374,8 @@ int ck_latent_cascade_decode(const void *q, const void *prefix_cache, const int3
  *            passes num_tokens or num_keys is cut off
  *   out      [num_tokens, num_heads, 128], dtype; lse fp32 [num_tokens * num_heads]
  * A query that sees nothing, and every row behind the last request, gets out = 0,
- * lse = -inf. P is rounded to dtype before the second product, its sum is not.
+ * lse = -inf. P is rounded to dtype before the second product, its sum is not. Keys that a
+ * query does not see may hold anything, infinite and NaN values included.
  * batch is at most 2^16.
  * -------------------------------------------------------------------------- */
 int ck_latent_prefill(const void *q, const void *k, int64_t k_token_stride, int64_t k_head_stride,

@@ -15,6 +15,17 @@ reference's custom ops under ``torch.ops.npu`` (the loader of
   ``torch.ops.npu.cascade_decode(query, prefix_key, prefix_value, prefix_block_table,
   prefix_kv_seqlens, suffix_key, suffix_value, suffix_block_table, suffix_kv_seqlens,
   suffix_kv_layout=0) -> (out bf16 [B,H,D], merged lse fp32 [B*H])``.
+* latent attention (one cached row of 512 + 64 numbers a token serves all heads, as key and as
+  value; bf16 or fp16, scale given by the caller):
+  ``torch.ops.npu.latent_cache_write(kv, gamma, cos_sin, positions, slots, cache, eps=1e-6,
+  interleaved=True)`` norms and rotates tokens into the pages,
+  ``torch.ops.npu.latent_decode(query, cache, block_table, actual_kv_seqlens, scale,
+  q_seqlen_value=1) -> (out [T,H,512], lse fp32 [T*H])`` attends over them,
+  ``torch.ops.npu.latent_cascade_decode(query, prefix_cache, prefix_block_table, prefix_kv_seqlens,
+  suffix_cache, suffix_block_table, suffix_kv_seqlens, scale) -> (out, lse)`` does for a batch that
+  shares a prefix, and ``torch.ops.npu.latent_prefill(query, key, key_rope, value, actual_q_seqlens,
+  actual_kv_seqlens, scale, causal=True) -> (out [T,H,128], lse fp32 [T*H])`` takes prompts with the
+  keys and values of each head laid out.
 
 ``cascade_amd.gate`` holds the cascade-vs-full decision harness.
 

@@ -6,30 +6,35 @@
 //   o = sum_j softmax(s)_j c_j (512 dims),  lse = log sum_j exp(s_j)
 // A row that sees no token gets o = 0, lse = -inf.
 //
-// One cache row serves every head as key and as value, so a tile of it in LDS feeds the
-// query rows of up to 64 (token, head) pairs:
-// * A workgroup (one per CU, 8 waves) streams 32-token tiles through a ring of 4 slots
-//   (36 KB each, buffer -> LDS DMA), two of them in flight while one is computed, for up to
-//   64 query rows. Wave w computes scores of rows 16 (w % 4) .. + 15 against tokens
-//   16 (w / 4) .. + 15 (Q in registers, 72 of them), and owns value dims 64 w .. + 63 of all
-//   64 rows (O in registers, 64 of them): P crosses the waves through LDS, O never does.
-// * S^T = X Q^T and O^T = C^T P^T on 16x16x32 MFMAs: K fragments are 16-byte row reads, C^T
-//   comes from the same tile through ds_read_b64_tr_b16, and a lane holds one query row of
-//   the accumulator.
-// * One barrier per tile. The softmax's reference point m of a row is not its running
-//   maximum but a value that moves only when some score exceeds it by 2^kSlack (any point
-//   gives the same result; p stays at or below 2^kSlack): a wave raises a flag beside its P,
-//   and the raised tile alone exchanges maxima, rescales O and computes P again.
-// * Tiles of all requests form one list, cut into equal chunks, one per workgroup (and per
-//   64-row tile of a request), so ragged lengths balance. A request inside one chunk is
-//   written as it is; parts of a cut one go to the workspace, normalised, with their lse, and
-//   latent_combine_kernel folds them.
-// * Shared prefix: the flattened rows of the batch (sequence, head) form 64-row units over
-//   splits of the prefix, which read each prefix tile once per 64 rows; what a
-//   workgroup has left after its unit it spends on suffix tiles, and the combine
-//   folds prefix and suffix parts in fp32.
+// One cache row serves every head as key and as value: 1152 bytes feed 2176 flops per row of
+// a query. Memory bounds calls of few rows, the matrix cores those of 64 rows and more; the form
+// below reads a tile of 32 tokens once for up to 128 (token, head) rows.
+// * A workgroup per CU, 4 waves, one per SIMD with all its 512 registers: a wave holds 32 rows
+//   (Q in 144 vector registers, O in the 256 accumulation registers) and computes their scores,
+//   softmax and O by itself, so that nothing crosses waves. Against 8 waves of 64 rows that divide
+//   scores and O (P through LDS): 128 heads 640 -> 552 us at 117 sequences on 16001 shared tokens.
+// * Tiles stream through a ring of 4 slots (37 KB, buffer -> LDS DMA), two in flight.
+// * S^T = X Q^T and O^T = C^T P^T on 16x16x32 products: a key fragment is a 16-byte row read, C^T
+//   comes from the same tile through ds_read_b64_tr_b16, P is in the operand's place as it leaves.
+// * A step has one barrier and is one run of code without branches: P of tile t and the DMAs of tile
+//   t + 3 are made in the shadow of tile t + 1's scores, the largest of those in that of tile t's
+//   products. 3450 cycles for 128 rows x 32 tokens, of which the products alone take 2180.
+// * The softmax's reference point m of a row is not its running maximum but a value that moves
+//   only when some score passes it by 2^kSlack (any point gives the same result; p stays at or
+//   below 2^kSlack), so that O is hardly ever rescaled (768 instructions).
+// * Tiles of all requests form one list (each item with some empty places for what opening and
+//   closing it costs), cut into equal chunks, one per workgroup (and per 128-row tile of a request),
+//   so ragged lengths balance. A request inside one chunk is written as it is; parts of a cut one
+//   go to the workspace, normalised, with their lse, and latent_combine_kernel folds them.
+// * Shared prefix: the flattened rows of the batch (sequence, head) form 128-row units over splits
+//   of the prefix, which read each prefix tile once per 128 rows. The number of splits is chosen on
+//   the device, so that the list of suffix tiles fills what the units leave; the combine folds
+//   prefix and suffix parts in fp32.
 // P is rounded to the cache's 16-bit type before the second product (its sum l is not): the
 // relative error of o stays near that of o's own rounding.
+// Measured: 48 x 16 heads over 12000 tokens (fp16, ragged) 92 us, 4.7 TB/s; 64 x 128 heads over 6000
+// 102 us, 670 TFLOP/s (a fifth of it writes and folds the parts); 117 x 128 heads on 16001 shared
+// tokens 440 us, 1.22 PFLOP/s; 1 x 16 heads over 1300 17 us, all latency.
 #include <cmath>
 
 #include "latent_common.h"
@@ -61,7 +66,12 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kPieces = 9;    // DMAs per wave and tile: 8 rows of the latent, and their rotated dims
 constexpr int kPhase = 256;   // tiles described in LDS at a time
 constexpr int kGroups = 256;  // workgroups: one per CU
-constexpr int kMinPlaces = 2;  // least places of the list per chunk
+// Least places of the list per chunk: short requests over more CUs against parts to fold. 2 against
+// 4, us: 1 x 16 heads over 1300 tokens 17.2 / 18.9, 7 x 32 over 900 18.9 / 21.9, 2 x 128 over 3000
+// 30.9 / 30.2.
+constexpr int kMinPlaces = 2;
+// Blocks of 16 rows from which on the fold gives a wave all parts: 512 blocks (64 x 128 heads) in that
+// form / the other 101.8 / 105.3 us a call, 144 blocks (24 x 3 x 32 heads) 49.2 / 45.8.
 constexpr int kFoldBlocks = 256;
 constexpr float kSlack = 8.f;
 

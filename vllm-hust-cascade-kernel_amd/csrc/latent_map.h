@@ -9,7 +9,8 @@ namespace lat {
 
 // An item (a request's row tile) takes its tiles' places on the list and kItemPlaces before
 // them, empty: about what opening and closing it costs, so that chunks of many short items
-// hold fewer tiles. Measured with 128 rows, in cycles: a tile 3450, an item 7000 to 15000.
+// hold fewer tiles. Measured with 128 rows, in cycles: a tile 3450, an item 7000 to 15000. 3 places
+// against none, with what else changed beside them: 19 x 2 x 64 heads over 92 tokens 31 / 58 us.
 constexpr int kItemPlaces = 3;
 
 // n places cut evenly into `chunks` <= n: the first `rem` have q + 1.

@@ -8,15 +8,20 @@
 // Bound by the matrix cores: 640 flops per (query, key) pair of a head, K and V read once
 // per 256 queries. The form is that of the stage-1 kernel with a key of two parts:
 // * A wave owns 32 queries of one head and every key they see, 8 waves a workgroup (256
-//   queries; 4 and 128 for small calls). Q stays in registers (48), so does O (64).
+//   queries). Q stays in registers (48), so does O (64).
 // * 64-key tiles land in a ring of 3 slots by buffer -> LDS DMA: the head's keys (16 KB), the
-//   rotated part all heads share (8 KB) and the values (16 KB), two tiles in flight. The
+//   rotated part all heads share (8 KB) and the values (16 KB), one in flight. The
 //   resources end with the request's last key, so nothing past it is read.
-// * S^T = K Q^T (24 MFMAs a tile of 32x32x16) puts one query on a lane; P^T is in the operand's
-//   place as it leaves; V^T comes through ds_read_b64_tr_b16 (16 MFMAs).
+// * S^T = K Q^T (24 products of 32x32x16 a tile) puts one query on a lane; P^T is in the operand's
+//   place as it leaves; V^T comes through ds_read_b64_tr_b16 (16 products). P of tile t is made in the
+//   shadow of tile t + 1's scores, the largest of those in that of tile t's second product: a step
+//   of the two waves of a SIMD takes 3070 cycles where 80 products take 2560.
 // * A query's reference point of the softmax moves only when a score passes it by 2^kSlack.
 // * Row tiles of a request are dealt last first: under a causal mask those are the longest.
-//   Tiles of one head run on one XCD, whose L2 then holds that head's K and V.
+// P is rounded to the 16-bit type before the second product, its sum is not.
+// Measured: 6000 tokens x 32 heads, causal, 375 us called now and then (983 TFLOP/s), 410 back to
+// back, where the clock falls to 1.6 GHz; 13 ragged prompts of about 900 on 700 x 16 heads 99 us;
+// 147 tokens x 16 heads 12.6 us, most of it the first passage through the code.
 #include <cmath>
 
 #include "latent_common.h"
