@@ -333,7 +333,7 @@ int ck_latent_cache_write(const void *kv, int64_t kv_stride, const void *gamma, 
  *   out      [batch * q_len, num_heads, 512], dtype
  *   lse      fp32 [batch * q_len * num_heads]
  *   workspace  of ck_latent_decode_plan's bytes for kv_cap = bt_cols * 128, 16-byte aligned
- * P is rounded to dtype before the second product, its sum is not. scale finite, > 0.
+ * P is rounded to dtype before the second product, its sum is not. scale > 0, at most 2.3e38.
  * -------------------------------------------------------------------------- */
 int ck_latent_decode_plan(int64_t batch, int64_t q_len, int64_t num_heads, int64_t kv_cap,
                           int64_t *workspace_bytes);

@@ -106,6 +106,7 @@ def test_write_refusals(bad, msg):
     (dict(scale=0.0), "scale must be"),
     (dict(scale=math.nan), "scale must be"),
     (dict(scale=1e300), "scale must be"),
+    (dict(scale=3e38), "scale must be"),
     (dict(lens=torch.empty(3, dtype=torch.int64)), "same HIP device"),
 ])
 def test_decode_refusals(bad, msg):
@@ -186,6 +187,7 @@ def _c_decode(**kw):
     (dict(blocks=2 ** 31 + 1), "CK_E_INVALID_ARG"),
     (dict(scale=0.0), "CK_E_INVALID_ARG"),
     (dict(scale=math.nan), "CK_E_INVALID_ARG"),
+    (dict(scale=3e38), "CK_E_INVALID_ARG"),
     (dict(q=None), "CK_E_NULL_PTR"),
     (dict(cache=None), "CK_E_NULL_PTR"),
     (dict(bt=None), "CK_E_NULL_PTR"),
@@ -249,7 +251,7 @@ def test_c_prefill_refuses():
         return abi.lib().ck_latent_prefill(*a.values())
     c = _codes()
     for bad in (dict(kts=4), dict(khs=-8), dict(vts=2 ** 24 + 8), dict(heads=0), dict(tokens=-1), dict(keys=2 ** 30),
-                dict(batch=2 ** 16 + 1), dict(scale=math.nan), dict(q=ODD), dict(v=ODD), dict(ql=ODD)):
+                dict(batch=2 ** 16 + 1), dict(scale=math.nan), dict(scale=3e38), dict(q=ODD), dict(v=ODD), dict(ql=ODD)):
         assert call(**bad) == c["CK_E_INVALID_ARG"], bad
     for name in ("q", "k", "kr", "v", "ql", "kl", "out", "lse"):
         assert call(**{name: None}) == c["CK_E_NULL_PTR"], name

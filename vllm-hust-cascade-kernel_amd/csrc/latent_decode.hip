@@ -993,7 +993,7 @@ int run(const void *q, const void *cache, const int32_t *block_table, int64_t bt
     if (prefix && (prefix->cols < 0 || prefix->num_blocks < 0 || prefix->num_blocks > ((int64_t)1 << 31) ||
                    prefix_cap != prefix->cols * kPage))
         return CK_E_INVALID_ARG;
-    if (!(scale > 0.f) || !std::isfinite(scale)) return CK_E_INVALID_ARG;
+    if (!(scale > 0.f) || !std::isfinite(scale * kLog2e)) return CK_E_INVALID_ARG;
     if (batch == 0) return CK_OK;
     if (!q || !kv_seqlens || !out || !lse || (bt_cols > 0 && (!block_table || (num_blocks > 0 && !cache))))
         return CK_E_NULL_PTR;

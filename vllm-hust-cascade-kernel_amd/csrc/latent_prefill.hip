@@ -518,7 +518,7 @@ extern "C" int ck_latent_prefill(const void *q, const void *k, int64_t k_token_s
         return CK_E_INVALID_ARG;
     for (int64_t st : {k_token_stride, k_head_stride, kr_stride, v_token_stride, v_head_stride})
         if (st < 0 || st > (1 << 24) || st % 8 != 0) return CK_E_INVALID_ARG;
-    if (!(scale > 0.f) || !std::isfinite(scale)) return CK_E_INVALID_ARG;
+    if (!(scale > 0.f) || !std::isfinite(scale * kLog2e)) return CK_E_INVALID_ARG;
     if (num_tokens == 0) return CK_OK;
     if (!q || !out || !lse || (batch > 0 && (!q_seqlens || !kv_seqlens)) || (num_keys > 0 && (!k || !k_rope || !v)))
         return CK_E_NULL_PTR;

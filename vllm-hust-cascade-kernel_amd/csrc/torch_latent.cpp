@@ -53,7 +53,8 @@ void check_table(const char *op, const char *what, const at::Tensor &table, cons
 
 void check_scale(const char *op, double scale) {
     const float f = static_cast<float>(scale);
-    TORCH_CHECK(std::isfinite(f) && f > 0.f, op, ": scale must be finite and > 0");
+    // the kernels work with scale log2(e)
+    TORCH_CHECK(f > 0.f && std::isfinite(f * 1.44269504f), op, ": scale must be > 0 and at most 2.3e38");
 }
 
 // q rows of `dim` elements; contiguous, its rows 16-byte aligned
