@@ -204,10 +204,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
         left -= kTok;
     };
     // What this wave has moved of tile t is in. Where not every query of the workgroup sees all of it,
-    // the values that 0 * V must not make NaN: past the request's end they become zeros; infinite or
-    // NaN ones set the tile's bit in *odd.
+    // values that 0 * V would turn into NaN become zeros: those past the request's end, and infinite
+    // or NaN ones, which set the tile's bit in *odd and reach the queries that see them at the end.
     const int w_first = scalar(seen(row0)), first_odd = w_first / kTok;
-    auto is_odd = [&](int t) { return ((scalar(*odd) >> (t - first_odd)) & 1) != 0; };
     auto look = [&](int t, int slot) {
         if (t * kTok + kTok <= w_first) return;
         int l = tid & 63;
@@ -217,11 +216,18 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
         for (int j = 0; j < kBlk; ++j) {
             const int r = (wid * kBlk + j) * 4 + (l >> 4);
             CK_LDS u32x4 *at = reinterpret_cast<CK_LDS u32x4 *>(smem + slot * kStage + kVAt + (wid * kBlk + j) * kVPiece + l * 16);
-            if (t * kTok + r < kl) {
-                const u32x4 x = *at;
-                bad |= not_finite<DT>(x[0]) | not_finite<DT>(x[1]) | not_finite<DT>(x[2]) | not_finite<DT>(x[3]);
-            } else {
+            u32x4 x = *at;
+            if (t * kTok + r >= kl) {
                 *at = u32x4{0, 0, 0, 0};
+            } else {
+                const u32x4 odd_ones = {not_finite<DT>(x[0]), not_finite<DT>(x[1]), not_finite<DT>(x[2]), not_finite<DT>(x[3])};
+                const uint32_t any = odd_ones[0] | odd_ones[1] | odd_ones[2] | odd_ones[3];
+                if (any != 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] &= ~((odd_ones[i] >> 15) * 0xffffu);
+                    *at = x;
+                }
+                bad |= any;
             }
         }
         if (bad != 0) __hip_atomic_fetch_or(odd, 1 << (t - first_odd), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
@@ -295,14 +301,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
         return u32x4{lo.x, lo.y, hi.x, hi.y};
     };
     // O^T += V^T P^T.
-    auto products = [&](auto ahead, int slot, auto &&clean, auto &&between) __attribute__((always_inline)) {
-        constexpr int kAhead = ahead, kHeld = kAhead + 1;
+    auto products = [&](int slot, auto &&between) __attribute__((always_inline)) {
+        constexpr int kAhead = 3, kHeld = kAhead + 1;
         u32x4 vf[kHeld];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) vf[i] = vfrag(slot, i >> 2, i & 3);
         __builtin_amdgcn_sched_barrier(0);
         static_for<16>([&](auto i) __attribute__((always_inline)) {
-            clean(vf[i % kHeld]);
             oacc[i & 3] = E::mfma32(vf[i % kHeld], pb[i >> 2], oacc[i & 3]);
             if (i + kAhead < 16) vf[(i + kAhead) % kHeld] = vfrag(slot, (i + kAhead) >> 2, (i + kAhead) & 3);
             between(i);
@@ -389,6 +394,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
             }
             fresh = false;
             if (first + kTok < w_most) {
+                __builtin_amdgcn_s_setprio(1);
                 scores(s1, y, [&](auto f) __attribute__((always_inline)) {
                     if constexpr (f % 3 != 0) {
                         constexpr int pair = f - 1 - f / 3;
@@ -397,6 +403,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
                     }
                 });
                 p_end(15);
+                __builtin_amdgcn_s_setprio(0);
             } else {
                 // unlike the scores above: their exponents are to be made beside the products there, not before
                 asm volatile("" : "+v"(x[0]), "+v"(x[1]));
@@ -406,21 +413,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
                 });
                 asm volatile("" : "=v"(y[0]), "=v"(y[1]));  // not looked at
             }
-            if (!hides || !is_odd(t)) {
-                products(std::integral_constant<int, 3>{}, slot, nothing, [&](auto i) __attribute__((always_inline)) {
-                    if constexpr (i == 0) v = max3(y[0][0], y[0][1], y[0][2]);
-                    else if constexpr (i < 15) v = max3(v, y[(2 * i + 1) >> 4][(2 * i + 1) & 15], y[(2 * i + 2) >> 4][(2 * i + 2) & 15]);
-                    else v = max_xor32(fmaxf(v, y[1][15])) * a.scale_log2;
-                });
-            } else {
-                // Infinite and NaN values are zeros here, where 0 * inf would reach queries that do not see
-                // them; those that do take them at the end.
-                products(std::integral_constant<int, 1>{}, slot, [](u32x4 &f) __attribute__((always_inline)) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) f[i] &= ~((not_finite<DT>(f[i]) >> 15) * 0xffffu);
-                }, nothing);
-                largest(y);
-            }
+            products(slot, [&](auto i) __attribute__((always_inline)) {
+                if constexpr (i == 0) v = max3(y[0][0], y[0][1], y[0][2]);
+                else if constexpr (i < 15) v = max3(v, y[(2 * i + 1) >> 4][(2 * i + 1) & 15], y[(2 * i + 2) >> 4][(2 * i + 2) & 15]);
+                else v = max_xor32(fmaxf(v, y[1][15])) * a.scale_log2;
+            });
         } else {
             asm volatile("" : "=v"(y[0]), "=v"(y[1]));
         }
@@ -447,10 +444,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     const float l_run = l_part + __shfl_xor(l_part, 32);
     __syncthreads();  // every wave is past its last ring read
     if (wrow0 >= ql) return;
-    // Infinite and NaN values of the tiles that had them, for the queries that see them (whose p is
+    // Infinite and NaN values that were left out, for the queries that see them (whose p is
     // positive): as they are, no finite weight or sum changes what they give.
-    for (int t = w_least / kTok; t * kTok < w_most; ++t) {
-        if (!is_odd(t)) continue;
+    const int odd_tiles = scalar(*odd);
+    for (int t = first_odd; odd_tiles >> (t - first_odd) != 0 && t * kTok < w_most; ++t) {
+        if (!((odd_tiles >> (t - first_odd)) & 1)) continue;
         for (int k = 0; k < kTok; ++k) {
             if (t * kTok + k >= limit) break;
             const uint16_t *row = a.v + (k0 + t * kTok + k) * a.v_ts + head * a.v_hs + 4 * hh;
