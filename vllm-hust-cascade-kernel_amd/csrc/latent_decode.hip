@@ -25,7 +25,7 @@
 // * Tiles of all requests form one list (each item with some empty places for what opening and
 //   closing it costs), cut into equal chunks, one per workgroup (and per 128-row tile of a request),
 //   so ragged lengths balance. A request inside one chunk is written as it is; parts of a cut one
-//   go to the workspace, normalised, with their lse, and latent_combine_kernel folds them.
+//   go to the workspace as they are, with m and l, and latent_combine_kernel folds them.
 // * Shared prefix: the flattened rows of the batch (sequence, head) form 128-row units over splits
 //   of the prefix, which read each prefix tile once per 128 rows. The number of splits is chosen on
 //   the device, so that the list of suffix tiles fills what the units leave; the combine folds
@@ -108,11 +108,11 @@ struct DecodeArgs {
     float scale_log2;
     void *out;    // [batch * q_len, heads, 512]
     float *lse;   // [batch * q_len * heads]
-    // Parts are kept by blocks of 16 rows as the lanes hold them, [128 x 4 dims][16 rows][4]:
+    // Parts, not normalised, are kept by blocks of 16 rows as the lanes hold them, [128 x 4 dims][16 rows][4]:
     // neighbouring lanes then store and load neighbouring bytes. Lanes in different rows (2 KB
     // apart) took a cycle each, 16000 of them for a workgroup's 256 KB.
     float *part_o;    // [slots][slot_rows / 16][128][16][4]
-    float *part_lse;  // [slots][slot_rows], log2
+    float2 *part_ml;  // [slots][slot_rows]: reference point (log2) and sum of p
     int32_t *sums;    // [batch + 2]: the list's places before each request and in all; the prefix's splits
     int slot_rows;
     int merge;        // 1: every part goes to the workspace (a prefix is folded in)
@@ -127,7 +127,7 @@ struct DecodeArgs {
     int pmtiles;
     int most_splits;
     float *ppart_o;    // [splits][prows_up / 16][128][16][4]
-    float *ppart_lse;  // [splits][prows_up], log2
+    float2 *ppart_ml;  // [splits][prows_up]
 };
 
 __device__ __forceinline__ int64_t clamp_len(int64_t n, int64_t cols, int64_t num_blocks) {
@@ -176,7 +176,12 @@ __device__ __forceinline__ KernArgs args_again(KernArgs a) {
 constexpr int acc_at(int db, int i) { return 8 * db + 4 * i; }
 
 __device__ __forceinline__ void acc_zero() {
-    static_for<256>([](auto n) __attribute__((always_inline)) { asm volatile("v_accvgpr_write_b32 a%c0, 0" ::"i"(int(n))); });
+    // 16 products of zeros: a register at a time is twice the time and 2 KB of code
+    u32x4 zero = {0, 0, 0, 0};
+    asm volatile("s_nop 7" : "+v"(zero));
+    static_for<16>([zero](auto n) __attribute__((always_inline)) {
+        asm volatile("v_mfma_f32_32x32x16_bf16 a[%c0:%c1], %2, %2, 0" ::"i"(16 * int(n)), "i"(16 * int(n) + 15), "v"(zero));
+    });
     asm volatile("" ::: "a255");  // all of them belong to the kernel
 }
 __device__ __forceinline__ void acc_ready(u32x4 &x, u32x4 &y) { asm volatile("s_nop 7" : "+v"(x), "+v"(y)); }
@@ -199,6 +204,15 @@ template <int DB, int I>
 __device__ __forceinline__ f32x4 acc_read() {
     constexpr int n = acc_at(DB, I);
     return f32x4{acc_read1<n>(), acc_read1<n + 1>(), acc_read1<n + 2>(), acc_read1<n + 3>()};
+}
+// Blocks (DB, I) to 16 bytes a lane at base + at + 1024 * (DB - DB0), for DB0 .. DB0 + 3.
+template <int DB0, int I>
+__device__ __forceinline__ void acc_store4(const float *base, int at) {
+    static_for<4>([base, at](auto k) __attribute__((always_inline)) {
+        constexpr int n = acc_at(DB0 + k, I);
+        asm volatile("global_store_dwordx4 %0, a[%c1:%c2], %3 offset:%c4" ::"v"(at), "i"(n), "i"(n + 3), "s"(base), "i"(1024 * k)
+                     : "memory");
+    });
 }
 // Rows of block i times f_i.
 __device__ __forceinline__ void acc_scale(float f0, float f1) {
@@ -683,36 +697,36 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             // ---- the segment's end ------------------------------------------------------------------
             if (ends) {
                 const KernArgs a = args_again(first_args);
-                float *po = nullptr, *pl = nullptr;  // the wave's first row of its part
+                float *po = nullptr;  // the wave's first row of its part
+                float2 *pl = nullptr;
                 if (in_prefix) {
                     const int64_t row = sp * (int64_t)a->prows_up + seg.row0;
                     po = a->ppart_o + row * kR;
-                    pl = a->ppart_lse + row;
+                    pl = a->ppart_ml + row;
                 } else if (a->merge || seg.began_before || goes_on) {
                     const int64_t slot = seg.began_before || goes_on ? part_slot(seg.began_before, chunk, a->teams, team)
                                                                      : (int64_t)2 * a->chunks * a->teams + seg.item;
                     const int64_t row = slot * a->slot_rows + kWaveRows * wave;
                     po = a->part_o + row * kR;
-                    pl = a->part_lse + row;
+                    pl = a->part_ml + row;
                 }
                 const Lane l(lane);
                 acc_done();
                 static_for<2>([&](auto i) __attribute__((always_inline)) {
                     const float sum = over_groups(l_part[i], [](float x, float y) { return x + y; });
-                    // 0 where no token was seen (or every score was -inf)
-                    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-                    const float lse2 = sum == 0.f ? -INFINITY : m_row[i] - E::kBias + log2f(sum);
                     const int row = 16 * i + l.n16;
                     const bool is_row = row < seg.rows_n;
-                    if (po != nullptr) {
+                    if (po != nullptr) {  // as it is: the fold divides
                         if (is_row) {
-                            float *o = po + 16 * i * kR + 4 * l.id;
-                            static_for<32>([&](auto db) __attribute__((always_inline)) {
-                                *reinterpret_cast<f32x4 *>(o + 256 * db) = acc_read<db, i>() * inv;
+                            static_for<8>([&](auto q) __attribute__((always_inline)) {
+                                acc_store4<4 * q, i>(po + 16 * i * kR + 1024 * q, 16 * l.id);
                             });
-                            if (l.g == 0) pl[row] = lse2;
+                            if (l.g == 0) pl[row] = make_float2(m_row[i], sum);
                         }
                     } else {
+                        // 0 where no token was seen (or every score was -inf)
+                        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+                        const float lse2 = sum == 0.f ? -INFINITY : m_row[i] - E::kBias + log2f(sum);
                         uint16_t *out = static_cast<uint16_t *>(a->out) + (seg.row0 + row) * kR + 16 * (l.g & 1) + 8 * (l.g >> 1);
                         static_for<16>([&](auto p) __attribute__((always_inline)) {
                             const u32x4 o = eight_dims<DT>(acc_read<2 * p, i>() * inv, acc_read<2 * p + 1, i>() * inv);
@@ -721,6 +735,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                         if (is_row && l.g == 0) a->lse[seg.row0 + row] = lse2 * kLn2;
                     }
                 });
+                asm volatile("s_nop 7" ::: "memory");  // the stores have read O
                 stored = seg.rows_n > 0;
                 seg.item = -1;
                 if (opens) {
@@ -830,19 +845,19 @@ __global__ __launch_bounds__(256) void latent_combine_kernel(DecodeArgs a) {
     float mx = -INFINITY, sum = 0.f;
     f32x4 acc[kDb] = {};
     for (int p0 = SHARE ? wave : 0; p0 < total; p0 += kStep * kAhead) {
-        float ls[kAhead];
+        float2 ml[kAhead];
         f32x4 o[kAhead][kDb];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const int p = min(p0 + j * kStep, total - 1);  // past the last part: it again, not added
             const float *po;
             if (p < splits) {
-                ls[j] = a.ppart_lse[(int64_t)p * a.prows_up + prow];
+                ml[j] = a.ppart_ml[(int64_t)p * a.prows_up + prow];
                 po = prefix_o + (int64_t)p * a.prows_up * kR;
             } else {
                 const int c = c0 + p - splits;
                 const int64_t slot = whole ? (int64_t)2 * a.chunks * a.teams + b * a.listed + m : part_slot(c > c0, c, a.teams, team);
-                ls[j] = a.part_lse[slot * a.slot_rows + row];
+                ml[j] = a.part_ml[slot * a.slot_rows + row];
                 po = a.part_o + (slot * a.slot_rows + row - n16) * kR + db0 * 256 + 4 * lane;
             }
 #pragma unroll
@@ -851,8 +866,7 @@ __global__ __launch_bounds__(256) void latent_combine_kernel(DecodeArgs a) {
         float mb = mx;
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            if (p0 + j * kStep >= total) ls[j] = -INFINITY;
-            mb = fmaxf(mb, ls[j]);
+            if (p0 + j * kStep < total) mb = fmaxf(mb, ml[j].x);
         }
         const float mu = mb == -INFINITY ? 0.f : mb;
         const float f = exp2_fast(mx - mu);
@@ -863,8 +877,8 @@ __global__ __launch_bounds__(256) void latent_combine_kernel(DecodeArgs a) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
             if (p0 + j * kStep < total) {
-                const float w = exp2_fast(ls[j] - mu);  // a part that saw nothing holds zeros
-                sum += w;
+                const float w = exp2_fast(ml[j].x - mu);  // 0 of a part that saw nothing, which holds zeros
+                sum = fmaf(ml[j].y, w, sum);
 #pragma unroll
                 for (int d = 0; d < kDb; ++d) acc[d] += o[j][d] * w;
             }
@@ -905,7 +919,7 @@ __global__ __launch_bounds__(256) void latent_combine_kernel(DecodeArgs a) {
         }
     }
     if (db0 == 0 && wave == 0 && g == 0 && head < a.heads)
-        a.lse[r] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+        a.lse[r] = sum == 0.f ? -INFINITY : (mx - Elem<DT>::kBias + log2f(sum)) * kLn2;
 }
 
 int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
@@ -915,7 +929,7 @@ int64_t pad256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 struct LatentPlan {
     int64_t rows, head_groups, mtiles, teams, listed, chunks, slot_rows, slots;
     int64_t prows, prows_up, pmtiles, psplits;
-    int64_t off_lse, off_o, off_plse, off_po, ws_bytes;
+    int64_t off_ml, off_o, off_pml, off_po, ws_bytes;
 };
 
 int make_plan(int64_t batch, int64_t q_len, int64_t heads, int64_t kv_cap, bool merge, int64_t prefix_cap,
@@ -945,10 +959,10 @@ int make_plan(int64_t batch, int64_t q_len, int64_t heads, int64_t kv_cap, bool 
         if (p->psplits > most) p->psplits = most < 1 ? 1 : most;
     }
     int64_t at = pad256((batch + 2) * 4);
-    p->off_lse = at;
-    at += pad256(p->slots * p->slot_rows * 4);
-    p->off_plse = at;
-    at += pad256(p->psplits * p->prows_up * 4);
+    p->off_ml = at;
+    at += pad256(p->slots * p->slot_rows * 8);
+    p->off_pml = at;
+    at += pad256(p->psplits * p->prows_up * 8);
     p->off_o = at;
     at += p->slots * p->slot_rows * kR * 4;
     p->off_po = at;
@@ -1025,7 +1039,7 @@ int run(const void *q, const void *cache, const int32_t *block_table, int64_t bt
     a.out = out;
     a.lse = lse;
     a.sums = reinterpret_cast<int32_t *>(ws);
-    a.part_lse = reinterpret_cast<float *>(ws + p.off_lse);
+    a.part_ml = reinterpret_cast<float2 *>(ws + p.off_ml);
     a.part_o = reinterpret_cast<float *>(ws + p.off_o);
     a.slot_rows = (int)p.slot_rows;
     a.head_groups = (int)p.head_groups;
@@ -1040,7 +1054,7 @@ int run(const void *q, const void *cache, const int32_t *block_table, int64_t bt
         a.prows_up = (int)p.prows_up;
         a.pmtiles = (int)p.pmtiles;
         a.most_splits = (int)p.psplits;
-        a.ppart_lse = reinterpret_cast<float *>(ws + p.off_plse);
+        a.ppart_ml = reinterpret_cast<float2 *>(ws + p.off_pml);
         a.ppart_o = reinterpret_cast<float *>(ws + p.off_po);
     }
     return dtype == CK_DTYPE_BF16 ? launch<CK_DTYPE_BF16>(a, s) : launch<CK_DTYPE_F16>(a, s);
