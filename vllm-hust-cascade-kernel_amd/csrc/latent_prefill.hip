@@ -14,14 +14,14 @@
 //   resources end with the request's last key, so nothing past it is read.
 // * S^T = K Q^T (24 products of 32x32x16 a tile) puts one query on a lane; P^T is in the operand's
 //   place as it leaves; V^T comes through ds_read_b64_tr_b16 (16 products). P of tile t is made in the
-//   shadow of tile t + 1's scores, the largest of those in that of tile t's second product: a step
-//   of the two waves of a SIMD takes 3070 cycles where 80 products take 2560.
+//   shadow of tile t + 1's scores, the largest of those in that of tile t's second product. A step
+//   of the two waves of a SIMD takes about 4200 cycles, its 80 products 2560.
 // * A query's reference point of the softmax moves only when a score passes it by 2^kSlack.
 // * Row tiles of a request are dealt last first: under a causal mask those are the longest.
 // P is rounded to the 16-bit type before the second product, its sum is not.
-// Measured: 6000 tokens x 32 heads, causal, 375 us called now and then (983 TFLOP/s), 410 back to
-// back, where the clock falls to 1.6 GHz; 13 ragged prompts of about 900 on 700 x 16 heads 99 us;
-// 147 tokens x 16 heads 12.6 us, most of it the first passage through the code.
+// Measured: 6000 tokens x 32 heads, causal, 356 us called now and then (1.04 PFLOP/s), 375 back to
+// back; 13 ragged prompts of about 580 on contexts, 16 heads, 89 us; 147 tokens x 16 heads 11.6 us, most
+// of it the first passage through the code.
 #include <cmath>
 
 #include "latent_common.h"
