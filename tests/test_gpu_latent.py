@@ -224,6 +224,62 @@ def test_decode_lengths_are_clamped():
     assert (out == 0).all() and (lse == -math.inf).all()
 
 
+def test_decode_more_row_tiles_than_workgroups():
+    """1100 tokens a request: 275 row tiles, one workgroup each, whose list takes several phases."""
+    lens, q_len = [9000, 0, 700, 1101], 1100
+    g = _gen(13)
+    cache, table = _pool(g, lens, BF)
+    q = _randn(g, len(lens) * q_len, 1, 576)
+    out, lse = OPS.latent_decode(q, cache, table, _i64(lens), SCALE, q_len)
+    for b, n in enumerate(lens):
+        x = _rows(cache, table, b, n)
+        i = torch.arange(q_len, device=DEV)
+        t = slice(b * q_len, (b + 1) * q_len)
+        ol.close(out[t, 0], lse[t], ol.attend(q[t, 0], x, x[:, :512], (n - q_len + 1 + i).clamp(0), SCALE, BF))
+
+
+@pytest.mark.parametrize("batch,q_len,heads,prefix", [(3, 1, 16, None), (40, 2, 33, None), (1, 1, 130, None), (300, 1, 8, None),
+                                                      (5, 1, 16, 700), (33, 1, 40, 0), (150, 1, 128, 130)])
+def test_workspace_is_as_large_as_planned(batch, q_len, heads, prefix):
+    """The C entry points write nothing behind the planned workspace, the output or the lse."""
+    import ctypes
+
+    from cascade_amd import abi
+    g = _gen(batch)
+    lens = torch.randint(0, 400, (batch,), generator=g, device=DEV).tolist()
+    cache, table = _pool(g, lens, BF, cols=4)
+    q = _randn(g, batch * q_len, heads, 576)
+    n, guard = ctypes.c_int64(0), 4096
+    kv = _i64(lens)
+    if prefix is None:
+        assert abi.lib().ck_latent_decode_plan(batch, q_len, heads, 4 * 128, ctypes.byref(n)) == 0
+    else:
+        pcache, ptable = _pool(g, [prefix], BF, cols=6)
+        plen = _i64([prefix])
+        assert abi.lib().ck_latent_cascade_decode_plan(batch, heads, 6 * 128, 4 * 128, ctypes.byref(n)) == 0
+    rows = batch * q_len * heads
+    sizes = {"ws": n.value, "out": rows * 1024, "lse": rows * 4}
+    room = {k: torch.full((v + guard,), 0x5a, dtype=torch.uint8, device=DEV) for k, v in sizes.items()}
+    tail = (room["out"].data_ptr(), room["lse"].data_ptr(), room["ws"].data_ptr(), n.value,
+            torch.cuda.current_stream().cuda_stream)
+    if prefix is None:
+        rc = abi.lib().ck_latent_decode(q.data_ptr(), cache.data_ptr(), table.data_ptr(), 4, kv.data_ptr(), batch, q_len, heads,
+                                        cache.shape[0], 128, 0, SCALE, *tail)
+    else:
+        rc = abi.lib().ck_latent_cascade_decode(q.data_ptr(), pcache.data_ptr(), ptable.data_ptr(), 6, plen.data_ptr(),
+                                                pcache.shape[0], cache.data_ptr(), table.data_ptr(), 4, kv.data_ptr(),
+                                                cache.shape[0], batch, heads, 128, 0, SCALE, *tail)
+    assert rc == 0
+    torch.cuda.synchronize()
+    for k, v in sizes.items():
+        assert (room[k][v:] == 0x5a).all(), k
+    out = room["out"][:sizes["out"]].view(BF).view(batch * q_len, heads, 512)
+    lse = room["lse"][:sizes["lse"]].view(torch.float32)
+    want = OPS.latent_decode(q, cache, table, kv, SCALE, q_len) if prefix is None else \
+        OPS.latent_cascade_decode(q, pcache, ptable, plen, cache, table, kv, SCALE)
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
 def test_decode_long_list():
     """More tiles per workgroup than are described at a time. The pages repeat, so that
     attention over them is that over one copy, with lse + log(copies)."""
@@ -318,6 +374,20 @@ def test_cascade_bad_pages_and_empty_prefix_table():
     out, lse = OPS.latent_cascade_decode(q, cache, none, _i64([300]), cache, table[1:], _i64([70]), SCALE)
     x = cache[table[1, 0]][:70]
     ol.close(out[0], lse, ol.attend(q[0], x, x[:, :512], 70, SCALE, BF))
+
+
+def test_cascade_units_longer_than_described_at_once():
+    """More tiles in a unit of the prefix than are described at a time: its state goes on over phases."""
+    g = _gen(22)
+    suffix = [(37 * b) % 90 for b in range(117)]
+    pcache, ptable = _pool(g, [20000], BF)
+    scache, stable = _pool(g, suffix, BF)
+    q = _randn(g, 117, 128, 576)
+    out, lse = OPS.latent_cascade_decode(q, pcache, ptable, _i64([20000]), scache, stable, _i64(suffix), SCALE)
+    x = _rows(pcache, ptable, 0, 20000)
+    for b in (0, 1, 58, 116):
+        keys = torch.cat([x, _rows(scache, stable, b, suffix[b])])
+        ol.close(out[b], lse.view(117, 128)[b], ol.attend(q[b], keys, keys[:, :512], 20000 + suffix[b], SCALE, BF))
 
 
 # ---- prefill ----------------------------------------------------------------------------------------------
