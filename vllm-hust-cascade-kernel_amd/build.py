@@ -17,6 +17,10 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
+if HERE not in sys.path:
+    sys.path.insert(0, HERE)
+import asm_waits  # noqa: E402
+
 REPO = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(REPO, "include")
@@ -68,15 +72,24 @@ def compile_hip(src):
     return obj
 
 
+def assembly(src):
+    """The device assembly of a source, as it is compiled into the library."""
+    os.makedirs(OBJDIR, exist_ok=True)
+    asm = os.path.join(OBJDIR, os.path.splitext(src)[0] + ".s")
+    run([HIPCC] + HIP_FLAGS + SOURCE_FLAGS.get(src, []) + ["--cuda-device-only", "-S", os.path.join(CSRC, src), "-o", asm])
+    return asm
+
+
 # latent_decode.hip keeps its output accumulators in the accumulation registers, which only
 # its inline assembly names. That is sound as long as the compiler keeps nothing of its own
 # there (it would, were it short of vector registers), so the build looks.
 OWN_ACC_REGISTERS = ["latent_decode.hip"]
+# Sources whose inline assembly reads or writes what matrix products do: the build looks for the
+# waits that the compiler does not insert there (asm_waits.py).
+CHECKED_WAITS = ["latent_decode.hip", "latent_prefill.hip"]
 
 
-def check_acc_registers(src):
-    asm = os.path.join(OBJDIR, os.path.splitext(src)[0] + ".s")
-    run([HIPCC] + HIP_FLAGS + SOURCE_FLAGS.get(src, []) + ["--cuda-device-only", "-S", os.path.join(CSRC, src), "-o", asm])
+def check_acc_registers(asm):
     inline = False
     with open(asm) as f:
         for line in f:
@@ -84,16 +97,23 @@ def check_acc_registers(src):
             if "#ASMSTART" in line or "#ASMEND" in line:
                 inline = "#ASMSTART" in line
             elif not inline and not code.lstrip().startswith(".") and re.search(r"[\s,]a(\d|\[)", code):
-                raise RuntimeError(f"{src}: the compiler uses an accumulation register of its own: {line.strip()}")
+                raise RuntimeError(f"{asm}: the compiler uses an accumulation register of its own: {line.strip()}")
             elif "scratch_" in code:
-                raise RuntimeError(f"{src}: the compiler spills: {line.strip()}")
+                raise RuntimeError(f"{asm}: the compiler spills: {line.strip()}")
+
+
+def check_assembly(src):
+    asm = assembly(src)
+    if src in OWN_ACC_REGISTERS:
+        check_acc_registers(asm)
+    asm_waits.check(asm)
 
 
 def build_kernels(jobs):
     os.makedirs(OBJDIR, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        checks = [ex.submit(check_acc_registers, src) for src in OWN_ACC_REGISTERS]
+        checks = [ex.submit(check_assembly, src) for src in CHECKED_WAITS]
         objs = list(ex.map(compile_hip, KERNEL_SOURCES))
         for c in checks:
             c.result()

@@ -81,12 +81,9 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x, uint32_t most) {
     return x;
 }
 
-// The largest of three; a NaN among them is passed over.
-__device__ __forceinline__ float max3(float x, float y, float z) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
-    return r;
-}
+// The largest of three; a NaN among them is passed over. One instruction, and the compiler's:
+// inside inline assembly it would not keep the distance from the product that made x, y or z.
+__device__ __forceinline__ float max3(float x, float y, float z) { return fmaxf(fmaxf(x, y), z); }
 
 // 16 bytes per lane from r at voff + soff to LDS at base + IMM + 16 * lane, as dma16_buf, with
 // the place in two scalar instructions: they issue in the shadow of a product, where a vector
