@@ -44,8 +44,20 @@ def test_operands_of_hand_written_products_and_loads():
     assert _pairs("v_cvt_pk_bf16_f32 v40, v1, v2\ns_nop 0\n" + product) == [("v_cvt_pk_bf16_f32", "v_mfma_f32_16x16x32_f16", 1, 2)]
     assert _pairs("v_cvt_pk_bf16_f32 v40, v1, v2\ns_nop 1\n" + product) == []
     load = "[[s_add_i32 m0, s4, 16\n\tbuffer_load_dwordx4 v1, s[8:11], s5 offen lds]]\n"
-    assert _pairs("v_readfirstlane_b32 s10, v2\n" + load) == [("v_readfirstlane_b32", "buffer_load_dwordx4", 1, 5)]
-    assert _pairs("v_readfirstlane_b32 s10, v2\ns_nop 3\n" + load) == []
+    assert ("v_readfirstlane_b32", "buffer_load_dwordx4", 1, 5) in _pairs("v_readfirstlane_b32 s10, v2\n" + load)
+    assert _pairs("v_readfirstlane_b32 s10, v2\ns_nop 3\n" + load.replace("\tbuffer", "\ts_nop 0\n\tbuffer")) == []
+
+
+@pytest.mark.parametrize("load", ["buffer_load_dwordx4 v1, s[8:11], s5 offen lds", "global_load_lds_dwordx4 v[2:3], off",
+                                  "global_load_lds_dword v[2:3], off"])
+@pytest.mark.parametrize("m0", ["s_mov_b32 m0, s4", "s_add_i32 m0, s4, 16"])
+def test_loads_to_lds_behind_m0(load, m0):
+    op, m0_op = load.split()[0], m0.split()[0]
+    assert _pairs("[[%s\n\t%s]]\n" % (m0, load)) == [(m0_op, op, 0, 1)]
+    assert _pairs("%s\n[[%s]]\n" % (m0, load)) == [(m0_op, op, 0, 1)]
+    assert _pairs("[[%s\n\ts_nop 0\n\t%s]]\n" % (m0, load)) == []
+    assert _pairs("[[%s\n\ts_nop 0\n\t%s]]\n" % (m0, load) * 2) == []
+    assert _pairs("[[%s\n\t%s]]\n" % (m0, load.replace(" lds", "").replace("_lds", ""))) == []  # not to LDS
 
 
 def test_paths_through_branches():

@@ -10,23 +10,27 @@ the compiler itself keeps between such instructions for gfx950:
 * a matrix product's result, before anything but a product's own sum reads or overwrites it:
   8 (16x16x16, 16x16x32) and 12 (32x32x16),
 * a vector instruction's result, before a matrix product reads it: 2,
-* a scalar register written by a vector instruction, before a memory instruction reads it: 5.
+* a scalar register written by a vector instruction, before a memory instruction reads it: 5,
+* M0, before a load to LDS reads it: 1.
 """
 import collections
 import re
 
 PRODUCT_WAITS = {"16x16x16": 8, "16x16x32": 8, "32x32x16": 12}
-VECTOR_TO_PRODUCT, VECTOR_TO_MEMORY = 2, 5
-FURTHEST = max(*PRODUCT_WAITS.values(), VECTOR_TO_PRODUCT, VECTOR_TO_MEMORY)
+VECTOR_TO_PRODUCT, VECTOR_TO_MEMORY, M0_TO_LDS_LOAD = 2, 5, 1
+FURTHEST = max(*PRODUCT_WAITS.values(), VECTOR_TO_PRODUCT, VECTOR_TO_MEMORY, M0_TO_LDS_LOAD)
 
 Instr = collections.namedtuple("Instr", "line text op inline writes reads product states")
-_REG = re.compile(r"\b([vas])(?:(\d+)\b|\[(\d+):(\d+)\])")
+_REG = re.compile(r"\b([vas])(?:(\d+)\b|\[(\d+):(\d+)\])|\b(m0)\b")
 
 
 def _regs(text):
     out = set()
-    for kind, one, lo, hi in _REG.findall(text):
-        out.update("%s%d" % (kind, i) for i in range(int(one or lo), int(one or hi) + 1))
+    for kind, one, lo, hi, m0 in _REG.findall(text):
+        if m0:
+            out.add("m0")
+        else:
+            out.update("%s%d" % (kind, i) for i in range(int(one or lo), int(one or hi) + 1))
     return out
 
 
@@ -42,6 +46,8 @@ def _decode(line, text, inline):
     count = 0 if stores else 2 if "_swap" in op else 1
     writes = set().union(*(_regs(o) for o in ops[:count])) if ops else set()
     reads = set().union(*(_regs(o) for o in (ops if "_swap" in op else ops[count:]))) if ops else set()
+    if to_lds:
+        reads.add("m0")
     product = None
     if "_mfma_" in op:
         product = next((k for k in PRODUCT_WAITS if k in op), None)
@@ -93,6 +99,8 @@ def _waits(first, then, reg):
         if then.product and reg in then.writes:  # its sum goes on where it is
             return 0 if first.writes == then.writes else PRODUCT_WAITS[first.product]
         return PRODUCT_WAITS[first.product]
+    if reg == "m0":
+        return M0_TO_LDS_LOAD
     if first.op.startswith("v_") and reg in then.reads:
         if reg[0] == "s":
             return VECTOR_TO_MEMORY if _is_memory(then.op) else 0

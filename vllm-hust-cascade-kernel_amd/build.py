@@ -84,9 +84,9 @@ def assembly(src):
 # its inline assembly names. That is sound as long as the compiler keeps nothing of its own
 # there (it would, were it short of vector registers), so the build looks.
 OWN_ACC_REGISTERS = ["latent_decode.hip"]
-# Sources whose inline assembly reads or writes what matrix products do: the build looks for the
-# waits that the compiler does not insert there (asm_waits.py).
-CHECKED_WAITS = ["latent_decode.hip", "latent_prefill.hip"]
+# Sources with instructions in inline assembly: the build looks for the waits that the compiler does
+# not insert there (asm_waits.py).
+CHECKED_WAITS = ["fa_stage1.hip", "suffix_decode.hip", "gateup_swiglu.hip", "latent_decode.hip", "latent_prefill.hip"]
 
 
 def check_acc_registers(asm):

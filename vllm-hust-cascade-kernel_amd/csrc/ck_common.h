@@ -62,10 +62,12 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 // land at lds_base + 16 * l; lds_base must be wave-uniform. Issued as inline asm
 // so the compiler does not guard every later LDS read with a vmcnt(0) wait (it
 // cannot prove transpose reads do not alias the DMA); callers wait explicitly
-// with wait_vmcnt<N>() and a workgroup barrier before reading the data.
+// with wait_vmcnt<N>() and a workgroup barrier before reading the data. M0 is read one wait state
+// after it is written at the earliest: the compiler puts an s_nop there for its own loads, and does
+// not see these.
 __device__ __forceinline__ void dma16(const void *g, CK_LDS void *lds_base) {
     const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds_base);
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                  :
                  : "s"(m0), "v"(g)
                  : "memory", "m0");
@@ -92,7 +94,7 @@ __device__ __forceinline__ ck_rsrc_t buf_rsrc(const void *base, uint32_t bytes) 
 __device__ __forceinline__ void dma16_buf(const ck_rsrc_t &rsrc, int voff, int soff, CK_LDS void *lds_base) {
     const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds_base);
     const int so = __builtin_amdgcn_readfirstlane(soff);
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
                  : "s"(m0), "v"(voff), "s"(rsrc), "s"(so)
                  : "memory", "m0");
@@ -102,7 +104,7 @@ __device__ __forceinline__ void dma16_buf(const ck_rsrc_t &rsrc, int voff, int s
 // lds_base + 4 * l.
 __device__ __forceinline__ void dma4(const void *g, CK_LDS void *lds_base) {
     const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds_base);
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
                  :
                  : "s"(m0), "v"(g)
                  : "memory", "m0");

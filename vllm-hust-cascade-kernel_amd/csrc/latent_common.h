@@ -90,7 +90,7 @@ __device__ __forceinline__ float max3(float x, float y, float z) { return fmaxf(
 // instruction and its trip to the scalar registers would hold the wave up.
 template <int IMM>
 __device__ __forceinline__ void dma_tile(const ck_rsrc_t &r, int voff, int soff, int base) {
-    asm volatile("s_add_i32 m0, %0, %c1\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds"
+    asm volatile("s_add_i32 m0, %0, %c1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds"
                  :
                  : "s"(base), "i"(IMM), "v"(voff), "s"(r), "s"(soff)
                  : "memory", "m0", "scc");
