@@ -294,10 +294,12 @@ int ck_add_rms_norm_stats(const void *x1, const void *x2, const void *gamma, con
  * statistics and norms are fp32. Pages hold 128 tokens: a pool is
  * [num_blocks, 128, 576] contiguous, token j of request b is row j % 128 of page
  * block_table[b * bt_cols + j / 128]; a page id outside the pool reads as zero rows.
- * kv lengths are clamped to [0, bt_cols * 128]. Rows of a page past a length may hold
- * anything. bt_cols * 128 is at most 2^30 and num_blocks at most 2^31; a call's tiles
- * (ceil(bt_cols * 128 / 32) + 3 a request, and per 128 rows where a prefix is shared) stay
- * below 2^31.
+ * kv lengths are clamped to [0, bt_cols * 128], and to 0 where the pool has no pages. Rows
+ * of a page past a length may hold anything. bt_cols * 128 is at most 2^30, num_blocks at most
+ * 2^31, batch and q_len at most 2^24, num_heads at most 2^16; batch * q_len * ceil(num_heads /
+ * 16) stays below 2^24, a call's query rows and its tiles (ceil(bt_cols * 128 / 32) + 3 a
+ * request, and per 128 rows where a prefix is shared) below 2^31. Calls past a limit are
+ * refused (CK_E_INVALID_ARG) before anything is launched.
  * ========================================================================== */
 
 /* ----------------------------------------------------------------------------
@@ -314,7 +316,8 @@ int ck_add_rms_norm_stats(const void *x1, const void *x2, const void *gamma, con
  *              outside [0, max_pos) is not written (-1 pads a batch). Slots that are
  *              written must be distinct: of two tokens with the same slot either may
  *              leave each 16-byte piece.
- * One rounding per value. Other rows of the cache are not touched. eps > 0, finite.
+ * One rounding per value. Other rows of the cache are not touched. eps > 0, finite; tokens at
+ * most 2^26 - 4, kv_stride at most 2^28.
  * -------------------------------------------------------------------------- */
 int ck_latent_cache_write(const void *kv, int64_t kv_stride, const void *gamma, const float *cos_sin,
                           int64_t max_pos, const int64_t *positions, const int64_t *slots, void *cache,
@@ -376,7 +379,8 @@ int ck_latent_cascade_decode(const void *q, const void *prefix_cache, const int3
  * A query that sees nothing, and every row behind the last request, gets out = 0,
  * lse = -inf. P is rounded to dtype before the second product, its sum is not. Keys that a
  * query does not see may hold anything, infinite and NaN values included.
- * batch is at most 2^16.
+ * batch and num_heads are at most 2^16, num_tokens and num_keys below 2^30 and
+ * (floor(num_tokens / 256) + batch + 1) * num_heads below 2^23.
  * -------------------------------------------------------------------------- */
 int ck_latent_prefill(const void *q, const void *k, int64_t k_token_stride, int64_t k_head_stride,
                       const void *k_rope, int64_t kr_stride, const void *v, int64_t v_token_stride,

@@ -215,6 +215,9 @@ __device__ __forceinline__ uint32_t xcd_remap(uint32_t b, uint32_t n) {
     return (b % kNumXcd) * per + b / kNumXcd;
 }
 
+// Host-side check of a launch: a dimension's blocks times threads stay below 2^32 (HIP refuses others).
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks < ((int64_t)1 << 32) / threads; }
+
 // Host-side argument check: p is a multiple of n bytes (null counts as aligned).
 inline bool aligned_to(const void *p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 

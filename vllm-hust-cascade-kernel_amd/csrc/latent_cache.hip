@@ -120,9 +120,10 @@ extern "C" int ck_latent_cache_write(const void *kv, int64_t kv_stride, const vo
     if (tokens < 0 || num_blocks < 0 || max_pos < 0 || kv_stride < lat::kRow || kv_stride % 8 != 0)
         return CK_E_INVALID_ARG;
     if (!(eps > 0.f) || !std::isfinite(eps)) return CK_E_INVALID_ARG;
-    if (num_blocks > ((int64_t)1 << 40) || max_pos > ((int64_t)1 << 40) || tokens > ((int64_t)1 << 32) ||
-        kv_stride > ((int64_t)1 << 28))
+    if (num_blocks > ((int64_t)1 << 40) || max_pos > ((int64_t)1 << 40) || kv_stride > ((int64_t)1 << 28))
         return CK_E_INVALID_ARG;
+    const int64_t groups = tokens / kWavesPerGroup + (tokens % kWavesPerGroup != 0);
+    if (!grid_fits(groups, kWavesPerGroup * 64)) return CK_E_INVALID_ARG;
     if (tokens == 0 || num_blocks == 0) return CK_OK;
     if (!kv || !gamma || !cos_sin || !positions || !slots || !cache) return CK_E_NULL_PTR;
     if (!aligned_to(kv, 16) || !aligned_to(gamma, 16) || !aligned_to(cos_sin, 16) || !aligned_to(cache, 16) ||
@@ -130,7 +131,7 @@ extern "C" int ck_latent_cache_write(const void *kv, int64_t kv_stride, const vo
         return CK_E_INVALID_ARG;
     WriteArgs a{static_cast<const uint16_t *>(kv), static_cast<const uint16_t *>(gamma), cos_sin, positions, slots,
                 static_cast<uint16_t *>(cache), tokens, kv_stride, max_pos, num_blocks * lat::kPage, eps};
-    const dim3 grid((unsigned)((tokens + kWavesPerGroup - 1) / kWavesPerGroup)), block(kWavesPerGroup * 64);
+    const dim3 grid((unsigned)groups), block(kWavesPerGroup * 64);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     if (dtype == CK_DTYPE_BF16) {
         if (interleaved) hipLaunchKernelGGL((latent_cache_write_kernel<CK_DTYPE_BF16, true>), grid, block, 0, s, a);

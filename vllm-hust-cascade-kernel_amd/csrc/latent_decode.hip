@@ -35,6 +35,7 @@
 // Measured: 48 x 16 heads over 12000 tokens (fp16, ragged) 92 us, 4.7 TB/s; 64 x 128 heads over 6000
 // 102 us, 670 TFLOP/s (a fifth of it writes and folds the parts); 117 x 128 heads on 16001 shared
 // tokens 440 us, 1.22 PFLOP/s; 1 x 16 heads over 1300 17 us, all latency.
+#include <algorithm>
 #include <cmath>
 
 #include "latent_common.h"
@@ -73,6 +74,7 @@ constexpr int kMinPlaces = 2;
 // Blocks of 16 rows from which on the fold gives a wave all parts: 512 blocks (64 x 128 heads) in that
 // form / the other 101.8 / 105.3 us a call, 144 blocks (24 x 3 x 32 heads) 49.2 / 45.8.
 constexpr int kFoldBlocks = 256;
+constexpr int kFoldThreads = 256;
 constexpr float kSlack = 8.f;
 
 constexpr int kLdsZero = kSlots * kSlotBytes;  // a row of zeros
@@ -806,7 +808,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
 // the blocks fill the CUs (SHARE false) a wave has 8 x 16 dims of all parts; where they do not, the
 // dims go over 8 workgroups and the parts over 4 waves, which are joined through LDS.
 template <int DT, bool SHARE>
-__global__ __launch_bounds__(256) void latent_combine_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(kFoldThreads) void latent_combine_kernel(DecodeArgs a) {
     constexpr int kDb = SHARE ? 4 : 8, kAhead = SHARE ? 4 : 2, kStep = SHARE ? 4 : 1;
     const int lane = __lane_id(), g = lane >> 4, n16 = lane & 15, wave = scalar((int)threadIdx.x >> 6);
     const int head_blocks = (a.heads + 15) / 16;
@@ -936,7 +938,8 @@ int make_plan(int64_t batch, int64_t q_len, int64_t heads, int64_t kv_cap, bool 
               LatentPlan *p) {
     if (batch < 0 || q_len < 1 || heads < 1 || kv_cap < 0 || prefix_cap < 0) return CK_E_INVALID_ARG;
     if (batch > (1 << 24) || q_len > (1 << 24) || heads > (1 << 16) || kv_cap > ((int64_t)1 << 30) ||
-        prefix_cap > ((int64_t)1 << 30) || batch * q_len >= ((int64_t)1 << 31) / heads)
+        prefix_cap > ((int64_t)1 << 30) || batch * q_len >= ((int64_t)1 << 31) / heads ||
+        !grid_fits(batch * q_len * ceil_div(heads, 16), kFoldThreads))
         return CK_E_INVALID_ARG;
     p->rows = q_len * heads;
     p->head_groups = ceil_div(heads, kWaveRows);
@@ -981,9 +984,9 @@ int launch(const DecodeArgs &a, hipStream_t s) {
     if (e != hipSuccess) return static_cast<int>(e);
     const int64_t blocks = (int64_t)a.batch * a.q_len * ceil_div(a.heads, 16);
     if (blocks >= kFoldBlocks)
-        hipLaunchKernelGGL((latent_combine_kernel<DT, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((latent_combine_kernel<DT, false>), dim3((unsigned)blocks), dim3(kFoldThreads), 0, s, a);
     else
-        hipLaunchKernelGGL((latent_combine_kernel<DT, true>), dim3((unsigned)blocks, 32 / 4), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((latent_combine_kernel<DT, true>), dim3((unsigned)blocks, 32 / 4), dim3(kFoldThreads), 0, s, a);
     CK_RETURN_LAUNCH();
 }
 
@@ -996,17 +999,14 @@ struct PrefixArgs {
 
 int run(const void *q, const void *cache, const int32_t *block_table, int64_t bt_cols, const int64_t *kv_seqlens,
         int64_t batch, int64_t q_len, int64_t heads, int64_t num_blocks, int64_t block_size, int dtype, float scale,
-        int64_t kv_cap, const PrefixArgs *prefix, int64_t prefix_cap, void *out, float *lse, void *workspace,
-        int64_t workspace_bytes, hipStream_t s) {
+        const PrefixArgs *prefix, void *out, float *lse, void *workspace, int64_t workspace_bytes, hipStream_t s) {
+    auto tokens_of = [](int64_t cols) { return cols < 0 ? -1 : std::min(cols, (int64_t)1 << 30) * kPage; };  // no overflow
     LatentPlan p;
-    int rc = make_plan(batch, q_len, heads, kv_cap, prefix != nullptr, prefix_cap, &p);
+    int rc = make_plan(batch, q_len, heads, tokens_of(bt_cols), prefix != nullptr, prefix ? tokens_of(prefix->cols) : 0, &p);
     if (rc != CK_OK) return rc;
     if (block_size != kPage || (dtype != CK_DTYPE_BF16 && dtype != CK_DTYPE_F16)) return CK_E_UNSUPPORTED;
-    if (bt_cols < 0 || num_blocks < 0 || num_blocks > ((int64_t)1 << 31) || kv_cap != bt_cols * kPage)
-        return CK_E_INVALID_ARG;
-    if (prefix && (prefix->cols < 0 || prefix->num_blocks < 0 || prefix->num_blocks > ((int64_t)1 << 31) ||
-                   prefix_cap != prefix->cols * kPage))
-        return CK_E_INVALID_ARG;
+    if (num_blocks < 0 || num_blocks > ((int64_t)1 << 31)) return CK_E_INVALID_ARG;
+    if (prefix && (prefix->num_blocks < 0 || prefix->num_blocks > ((int64_t)1 << 31))) return CK_E_INVALID_ARG;
     if (!(scale > 0.f) || !std::isfinite(scale * kLog2e)) return CK_E_INVALID_ARG;
     if (batch == 0) return CK_OK;
     if (!q || !kv_seqlens || !out || !lse || (bt_cols > 0 && (!block_table || (num_blocks > 0 && !cache))))
@@ -1079,8 +1079,7 @@ extern "C" int ck_latent_decode(const void *q, const void *cache, const int32_t 
                                 int64_t num_blocks, int64_t block_size, int dtype, float scale, void *out, float *lse,
                                 void *workspace, int64_t workspace_bytes, void *stream) {
     return run(q, cache, block_table, bt_cols, kv_seqlens, batch, q_len, num_heads, num_blocks, block_size, dtype,
-               scale, bt_cols * kPage, nullptr, 0, out, lse, workspace, workspace_bytes,
-               reinterpret_cast<hipStream_t>(stream));
+               scale, nullptr, out, lse, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }
 
 extern "C" int ck_latent_cascade_decode_plan(int64_t batch, int64_t num_heads, int64_t prefix_cap, int64_t suffix_cap,
@@ -1101,6 +1100,6 @@ extern "C" int ck_latent_cascade_decode(const void *q, const void *prefix_cache,
                                         float *lse, void *workspace, int64_t workspace_bytes, void *stream) {
     const PrefixArgs prefix{prefix_cache, prefix_block_table, prefix_kv_seqlen, prefix_bt_cols, prefix_num_blocks};
     return run(q, suffix_cache, suffix_block_table, suffix_bt_cols, suffix_kv_seqlens, batch, 1, num_heads,
-               suffix_num_blocks, block_size, dtype, scale, suffix_bt_cols * kPage, &prefix, prefix_bt_cols * kPage, out,
-               lse, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
+               suffix_num_blocks, block_size, dtype, scale, &prefix, out, lse, workspace, workspace_bytes,
+               reinterpret_cast<hipStream_t>(stream));
 }

@@ -491,7 +491,7 @@ int launch(PrefillArgs a, hipStream_t s) {
     // every request's last tile may be a part, and so may that of the rows behind the last
     const int64_t tiles = a.tokens / kRows + a.batch + 1;
     const int64_t grid = tiles * a.heads;
-    if (grid > 0x7FFFFFFF) return CK_E_INVALID_ARG;
+    if (!grid_fits(grid, NW * 64)) return CK_E_INVALID_ARG;
     a.tiles = (int)tiles;
     static std::atomic<uint64_t> lds_set{0};
     int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(&latent_prefill_kernel<DT, NW>), kLds, lds_set);
