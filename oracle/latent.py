@@ -6,6 +6,8 @@ their 16-bit type (half a step: relative ``unit``), and each probability to that
 before the second product (again ``unit``, of the sum of p |value|). Scores, the softmax's
 statistics and sums are fp32.
 """
+import math
+
 import torch
 
 R, P, D, PAGE = 512, 64, 128, 128
@@ -73,3 +75,48 @@ def close(out, lse, ref):
     assert (d_o <= b_o).all(), "out: %.3g over a bound of %.3g" % max(zip(d_o.flatten().tolist(), b_o.flatten().tolist()), key=lambda t: t[0] - t[1])
     assert (d_l <= b_l[~torch.isneginf(l)]).all(), "lse: off by %.3g" % d_l.max()
     return 0.0 if d_o.numel() == 0 else (d_o / b_o.clamp_min(1e-30)).max().item()
+
+
+# ---- exact counts: which tiles of a long call were read, and how often -----------------------------------
+# With q = 0 every score is 0 and every p is one power of two, so that sums of p are whole
+# multiples of it, exact in fp32 below 2^24 tokens, and lse is log(tokens read) but for the last few
+# roundings. Cached tokens hold a 1 in two value dims that name their tile of 32: o is then the
+# share of each dim's tiles.
+TILE = 32
+
+
+def markers(tile):
+    """The two value dims of a tile: its number mod 256, and its number / 256."""
+    return tile % 256, 256 + tile // 256 % 256
+
+
+def mark(rows, first_tile=0):
+    """Cached tokens [n, 576] of a request, from its tile first_tile on, in place."""
+    rows.zero_()
+    tile = torch.arange(rows.shape[0], device=rows.device) // TILE + first_tile
+    for d in markers(tile):
+        rows.scatter_(1, d[:, None], 1)
+
+
+def counted(tokens, dtype):
+    """(o, lse, bounds) of a row that read tokens[t] tokens of tile t (a tensor), as attend() gives them.
+    o rounds to the type behind a division and a product in fp32. lse is ln 2 (log2(sum) - bias), log2 good
+    to a step of its result, the difference to half of one (the bias is below it), then a product by a
+    rounded constant. fp16 sums are 2^7 as large."""
+    tokens = tokens.double()
+    n, tile = tokens.sum(), torch.arange(tokens.numel(), device=tokens.device)
+    o = tokens.new_zeros(R)
+    for d in markers(tile):
+        o.index_add_(0, d, tokens)
+    if n == 0:
+        return o, torch.log(n), o, torch.zeros_like(n)
+    o, lse = o / n, torch.log(n)
+    log2 = torch.log2(n) + (7 if dtype == torch.float16 else 0)
+    step = torch.exp2(torch.floor(torch.log2(log2.clamp_min(1))) - 23)
+    return o, lse, (unit(dtype) + 4 * F32) * o, math.log(2) * 1.5 * step + 2 * F32 * lse
+
+
+def whole(n, device="cpu"):
+    """Tokens of each tile of a request of n tokens."""
+    tile = torch.arange(-(-n // TILE), device=device)
+    return (n - tile * TILE).clamp(max=TILE)
