@@ -1,4 +1,4 @@
-"""Every tile of a long or cut call of the latent decode is read once: exact counts
+"""Every tile of a long or cut call of the latent decode and prefill is read once: exact counts
 (oracle/latent.py), at lengths where a lost tile is far within the bounds of ordinary inputs."""
 import pytest
 import torch
@@ -104,3 +104,36 @@ def test_cascade_counts(dtype, prefix, batch, heads, suffix):
         if n not in of:
             of[n] = ol.counted(torch.cat([ol.whole(prefix, DEV), ol.whole(n, DEV)]), dtype)
         _check(out[b], lse[b], of[n])
+
+
+@pytest.mark.parametrize("dtype,heads,causal,ql,kl", [
+    (HF, 2, True, [6000], [6000]),
+    (HF, 3, True, [32], [8000]),              # a short continuation of a long context
+    (BF, 1, False, [1, 300], [20000, 4097]),
+    (HF, 2, True, [257, 0, 900, 33], [5000, 64, 900, 16]),
+    (HF, 1, False, [70], [131]),
+])
+def test_prefill_counts(dtype, heads, causal, ql, kl):
+    """Every key a query sees is counted once. Value dims: the tile of 64 keys mod 64, and its number / 64."""
+    q = torch.zeros(sum(ql), heads, 192, dtype=dtype, device=DEV)
+    k, kr = torch.ones(sum(kl), heads, 128, dtype=dtype, device=DEV), torch.ones(sum(kl), 64, dtype=dtype, device=DEV)
+    tiles = [torch.arange(n, device=DEV) // 64 for n in kl]
+    marks = torch.cat([torch.nn.functional.one_hot(t % 64, 64) for t in tiles]), \
+        torch.cat([torch.nn.functional.one_hot(t // 64, 64) for t in tiles])
+    v = torch.cat(marks, 1)[:, None].expand(-1, heads, -1).to(dtype)
+    out, lse = OPS.latent_prefill(q, k, kr, v, _i64(ql), _i64(kl), SCALE, causal)
+    lse, qa = lse.view(-1, heads), 0
+    for n, m in zip(ql, kl):
+        if n == 0:
+            continue
+        i = torch.arange(n, device=DEV)
+        sees = (m - n + 1 + i).clamp(0, m) if causal else torch.full((n,), m, device=DEV)
+        tile = torch.arange(-(-m // 64), device=DEV)
+        tokens = (sees[:, None] - 64 * tile).clamp(0, 64).double()
+        names = torch.cat([torch.nn.functional.one_hot(tile % 64, 64), torch.nn.functional.one_hot(tile // 64, 64)], 1)
+        o = tokens @ names.double() / sees.clamp_min(1)[:, None]
+        # the bounds depend on how many tokens were read, not on where
+        b_l = torch.stack([ol.counted(x[None], dtype)[3] for x in sees])
+        for h in range(heads):
+            ol.close(out[qa:qa + n, h], lse[qa:qa + n, h], (o, torch.log(sees.double()), (ol.unit(dtype) + 4 * ol.F32) * o, b_l))
+        qa += n
