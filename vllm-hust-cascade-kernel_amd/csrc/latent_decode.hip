@@ -9,9 +9,10 @@
 // One cache row serves every head as key and as value: 1152 bytes feed 2176 flops per row of
 // a query. Memory bounds calls of few rows, the matrix cores those of 64 rows and more; the form
 // below reads a tile of 32 tokens once for up to 128 (token, head) rows.
-// * A workgroup per CU, 4 waves, one per SIMD with all its 512 registers: a wave holds 32 rows
-//   (Q in 144 vector registers, O in the 256 accumulation registers) and computes their scores,
-//   softmax and O by itself, so that nothing crosses waves. Against 8 waves of 64 rows that divide
+// * A workgroup per CU, 4 waves, one per SIMD with all its 512 registers: a wave holds 32 rows of one
+//   token (fewer heads leave rows empty, and an item of up to 32 rows three waves; a tile takes its
+//   time all the same). Q is in 144 vector registers, O in the 256 accumulation registers; the wave
+//   computes scores, softmax and O by itself, so that nothing crosses waves. Against 8 waves of 64 rows that divide
 //   scores and O (P through LDS): 128 heads 640 -> 552 us at 117 sequences on 16001 shared tokens.
 // * Tiles stream through a ring of 4 slots (37 KB, buffer -> LDS DMA), two in flight.
 // * S^T = X Q^T and O^T = C^T P^T on 16x16x32 products: a key fragment is a 16-byte row read, C^T
@@ -32,9 +33,10 @@
 //   prefix and suffix parts in fp32.
 // P is rounded to the cache's 16-bit type before the second product (its sum l is not): the
 // relative error of o stays near that of o's own rounding.
-// Measured: 48 x 16 heads over 12000 tokens (fp16, ragged) 92 us, 4.7 TB/s; 64 x 128 heads over 6000
-// 102 us, 670 TFLOP/s (a fifth of it writes and folds the parts); 117 x 128 heads on 16001 shared
-// tokens 440 us, 1.22 PFLOP/s; 1 x 16 heads over 1300 17 us, all latency.
+// Measured, inputs changing from call to call: 48 x 16 heads over 12000 tokens (fp16, ragged) 92 us,
+// 4.8 TB/s; 64 x 128 heads over 6000 103 us, 660 TFLOP/s (a fifth of it writes and folds the parts);
+// 117 x 128 heads on 16001 shared tokens 475 us, 1.13 PFLOP/s (454 on the same inputs each time); 1 x 16
+// heads over 1300 17 us, all latency; 24 x 7 x 16 heads over 5000 60 us, as 7 groups of 32 rows in two teams.
 #include <algorithm>
 #include <cmath>
 
@@ -71,8 +73,10 @@ constexpr int kGroups = 256;  // workgroups: one per CU
 // 4, us: 1 x 16 heads over 1300 tokens 17.2 / 18.9, 7 x 32 over 900 18.9 / 21.9, 2 x 128 over 3000
 // 30.9 / 30.2.
 constexpr int kMinPlaces = 2;
-// Blocks of 16 rows from which on the fold gives a wave all parts: 512 blocks (64 x 128 heads) in that
-// form / the other 101.8 / 105.3 us a call, 144 blocks (24 x 3 x 32 heads) 49.2 / 45.8.
+// Blocks of 16 rows from which on the fold gives a wave all parts. In that form / the other, us a call:
+// 64 blocks 24 / 22 (64 x 16 heads over 600) to 66 / 48 (8 x 128 over 12000), 128 blocks 29 / 30 to 65 / 61,
+// 256 blocks 39 / 42 to 48 / 47 (32 x 128 over 3000), 384 blocks 50 / 55 to 136 / 136, 512 blocks 61 / 68 to 157 / 159
+// (shared prefix, 64 x 128: 115 / 111). Where they meet grows with the parts, from 128 blocks to 384.
 constexpr int kFoldBlocks = 256;
 constexpr int kFoldThreads = 256;
 constexpr float kSlack = 8.f;

@@ -19,9 +19,11 @@
 // * A query's reference point of the softmax moves only when a score passes it by 2^kSlack.
 // * Row tiles of a request are dealt last first: under a causal mask those are the longest.
 // P is rounded to the 16-bit type before the second product, its sum is not.
-// Measured: 6000 tokens x 32 heads, causal, 356 us called now and then (1.04 PFLOP/s), 375 back to
-// back; 13 ragged prompts of about 580 on contexts, 16 heads, 89 us; 147 tokens x 16 heads 11.6 us, most
-// of it the first passage through the code.
+// One workgroup walks all keys of its rows: with few queries most CUs have none, and the time is that of
+// the walk. Measured, inputs changing from call to call: 6000 tokens x 32 heads, causal, 370 us (1.00
+// PFLOP/s; 354 on the same inputs each time), every key seen 654 (1.13 PFLOP/s); 13 ragged prompts of
+// about 580 on contexts, 16 heads, 91 us; 147 tokens x 16 heads 11.2 us, most of it the first passage through
+// the code; 32 queries behind 8000 keys 136 us, with 8 heads or 32.
 #include <cmath>
 
 #include "latent_common.h"
@@ -36,6 +38,8 @@ typedef __attribute__((__vector_size__(2 * sizeof(unsigned)))) unsigned u32x2;
 constexpr int kD = 128;            // a head's key part, and its value
 constexpr int kQ = kD + kP;        // query row
 constexpr int kTok = 64;           // keys per tile
+constexpr int kWaves = 8, kThreads = kWaves * 64;
+constexpr int kRows = kWaves * 32;  // queries per workgroup
 // A tile in LDS. Keys: pieces of 4 rows (1 KB, one DMA) 1088 bytes apart, chunk c (16 bytes) of
 // the piece's row i at c ^ i: the 16 rows that a 16-byte read is served for lie in 16 bank groups, and
 // all chunks of a row are two registers and immediates away. Rotated part: pieces of 8 rows 1056
@@ -77,12 +81,11 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
     return ((w & 0x7fff7fffu) + kGap) & 0x80008000u;
 }
 
-template <int DT, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void latent_prefill_kernel(PrefillArgs a) {
+template <int DT>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void latent_prefill_kernel(PrefillArgs a) {
     using E = Elem<DT>;
-    constexpr int kRows = NW * 32;
-    constexpr int kBlk = 16 / NW;   // 1-KB DMAs of the keys (and of the values) per wave and tile
-    constexpr int kRBlk = 8 / NW;   // and of the rotated part
+    constexpr int kBlk = 16 / kWaves;   // 1-KB DMAs of the keys (and of the values) per wave and tile
+    constexpr int kRBlk = 8 / kWaves;   // and of the rotated part
     extern __shared__ __attribute__((aligned(16))) char smem_raw[];
     CK_LDS char *smem = (CK_LDS char *)smem_raw;
     CK_LDS int *odd = (CK_LDS int *)(smem + kSlots * kStage);
@@ -485,18 +488,17 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     }
 }
 
-template <int DT, int NW>
+template <int DT>
 int launch(PrefillArgs a, hipStream_t s) {
-    constexpr int kRows = NW * 32;
     // every request's last tile may be a part, and so may that of the rows behind the last
     const int64_t tiles = a.tokens / kRows + a.batch + 1;
     const int64_t grid = tiles * a.heads;
-    if (!grid_fits(grid, NW * 64)) return CK_E_INVALID_ARG;
+    if (!grid_fits(grid, kThreads)) return CK_E_INVALID_ARG;
     a.tiles = (int)tiles;
     static std::atomic<uint64_t> lds_set{0};
-    int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(&latent_prefill_kernel<DT, NW>), kLds, lds_set);
+    int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(&latent_prefill_kernel<DT>), kLds, lds_set);
     if (rc != CK_OK) return rc;
-    hipLaunchKernelGGL((latent_prefill_kernel<DT, NW>), dim3((unsigned)grid), dim3(NW * 64), kLds, s, a);
+    hipLaunchKernelGGL((latent_prefill_kernel<DT>), dim3((unsigned)grid), dim3(kThreads), kLds, s, a);
     CK_RETURN_LAUNCH();
 }
 
@@ -544,6 +546,6 @@ extern "C" int ck_latent_prefill(const void *q, const void *k, int64_t k_token_s
     a.out = static_cast<uint16_t *>(out);
     a.lse = lse;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if (dtype == CK_DTYPE_BF16) return launch<CK_DTYPE_BF16, 8>(a, s);
-    return launch<CK_DTYPE_F16, 8>(a, s);
+    if (dtype == CK_DTYPE_BF16) return launch<CK_DTYPE_BF16>(a, s);
+    return launch<CK_DTYPE_F16>(a, s);
 }
