@@ -1,4 +1,4 @@
-"""Waits around hand-written instructions (asm_waits.py): the checker on planted listings, and on
+"""Waits around hand-written instructions (asm_waits.py): what it finds in planted listings, and on
 the assembly of the kernels as they are built."""
 import os
 
