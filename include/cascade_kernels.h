@@ -389,6 +389,91 @@ int ck_latent_prefill(const void *q, const void *k, int64_t k_token_stride, int6
                       void *out, float *lse, void *stream);
 
 /* ============================================================================
+ * A K/V cache in 4 bits. No counterpart in the reference (its pools are bf16). A pool is
+ * uint8 [num_blocks, kv_heads, CK_KV4_PAGE_BYTES] contiguous: a page holds 128 tokens of a kv head, slot s is
+ * page s / 128, token s % 128. Keys and values are e2m1 numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+ * negatives); 32 neighbouring dims of a token share a scale 2^(e - 127), e one byte: 136 bytes a token and
+ * kv head against 512 in 16 bits. A page is two units of 64 tokens, 8704 bytes each; the unit holds
+ * for its token t = 32 h + 8 g + 4 j + r (h, j < 2; g, r < 4):
+ *   bytes 0..4095     keys' codes [64 t][64]: byte i has dims 2 i (low half) and 2 i + 1 (high)
+ *   bytes 4096..8191  values' codes [4 q][4 g][16 n][2 h][8: 4 j + r]: dims 8 n + 2 q (low) and the next
+ *   bytes 8192..8447  keys' scales e [4 groups of dims][4 g][4 r][2 h][2 j]
+ *   bytes 8448..8703  values' scales e [4 groups of dims][4 g][2 h][8: 4 j + r]
+ * A code is sign, 2 exponent bits, 1 mantissa bit from the highest bit down; scale byte 255 makes its group
+ * NaN. num_blocks is at most 2^31, kv_heads at most 2^10; head dim 128.
+ * ========================================================================== */
+#define CK_KV4_PAGE_BYTES 17408
+
+/* ----------------------------------------------------------------------------
+ * Quantises tokens into their slots. Per token, kv head and group of 32 dims, max the largest
+ * magnitude: e - 127 = floor(log2 max) - 2, one more where max > 1.75 * 2^floor(log2 max), and e kept within
+ * [8, 252]; a code is x / 2^(e - 127) rounded to the nearest e2m1 number, ties to the even code, at most
+ * 6. A group with an infinite or NaN value gets e = 255 and codes 0.
+ *   k, v     [tokens, kv_heads, 128] of dtype CK_DTYPE_BF16 or CK_DTYPE_F16; element strides per token and
+ *            head, multiples of 8 and at most 2^28
+ *   slots    int64 [tokens] on the device. A token whose slot is outside [0, num_blocks * 128) is not
+ *            written (-1 pads a batch). Slots that are written must be distinct: of two tokens with the
+ *            same slot either may leave each byte.
+ * Other tokens of the pool are not touched. tokens is below 2^28.
+ * -------------------------------------------------------------------------- */
+int ck_kv4_cache_write(const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
+                       int64_t v_token_stride, int64_t v_head_stride, const int64_t *slots, void *cache,
+                       int64_t num_blocks, int64_t tokens, int64_t kv_heads, int dtype, void *stream);
+
+/* ----------------------------------------------------------------------------
+ * Reads tokens back: k, v [tokens, kv_heads, 128] of dtype (16 bits), each value rounded once (bf16 holds
+ * what ck_kv4_cache_write leaves; a value past fp16's range becomes infinite). A slot outside the pool
+ * reads as zeros. With the slots of whole pages the results are [pages, 128, kv_heads, 128]
+ * pools, as ck_fa_fp32_stage1 and ck_suffix_decode take them.
+ * -------------------------------------------------------------------------- */
+int ck_kv4_cache_read(const void *cache, const int64_t *slots, int64_t num_blocks, int64_t tokens, int64_t kv_heads,
+                      int dtype, void *k, void *v, void *stream);
+
+/* ----------------------------------------------------------------------------
+ * Decode attention over the pages, q_len tokens per request (any number >= 1): token i, head h of request b,
+ * k_j and v_j the dequantised tokens of kv head h / (num_heads / kv_heads):
+ *   s_j = scale * q . k_j,  j < kv_seqlens[b] - q_len + 1 + i  (causal among the request's q_len
+ *   newest tokens, which are in the cache already)
+ *   out = sum_j softmax(s)_j * v_j,  lse = log sum_j exp(s_j)
+ * A token that sees nothing gets out = 0, lse = -inf.
+ *   q        [batch * q_len, num_heads, 128], dtype CK_DTYPE_BF16 or CK_DTYPE_F16; num_heads a multiple of kv_heads
+ *   block_table int32 [batch, bt_cols]: token j is row j % 128 of page block_table[b * bt_cols + j / 128]; a
+ *            page id outside the pool reads as zero rows
+ *   kv_seqlens int64 [batch] on the device, the new tokens included; clamped to [0, bt_cols * 128],
+ *            and to 0 where the pool has no pages. Tokens past a length may hold anything.
+ *   out      [batch * q_len, num_heads, 128], dtype
+ *   lse      fp32 [batch * q_len * num_heads]
+ *   workspace  of ck_kv4_decode_plan's bytes for kv_cap = bt_cols * 128, 16-byte aligned
+ * Sums, softmax statistics and P (as two bf16 terms) hold 32 bits or within 2^-17 of them. scale > 0,
+ * at most 2.3e38. bt_cols * 128 is at most 2^30, batch and q_len at most 2^24, num_heads at most 2^16;
+ * batch * q_len * num_heads stays below 2^24, batch * kv_heads * ceil(bt_cols * 128 / 64) below 2^31.
+ * Calls past a limit are refused (CK_E_INVALID_ARG) before anything is launched.
+ * -------------------------------------------------------------------------- */
+int ck_kv4_decode_plan(int64_t batch, int64_t q_len, int64_t num_heads, int64_t kv_heads, int64_t kv_cap,
+                       int64_t *workspace_bytes);
+
+int ck_kv4_decode(const void *q, const void *cache, const int32_t *block_table, int64_t bt_cols,
+                  const int64_t *kv_seqlens, int64_t batch, int64_t q_len, int64_t num_heads, int64_t kv_heads,
+                  int64_t num_blocks, int64_t block_size, int dtype, float scale, void *out, float *lse, void *workspace,
+                  int64_t workspace_bytes, void *stream);
+
+/* ----------------------------------------------------------------------------
+ * The same for batch single-token queries that share a prefix: each attends to the prefix (one request: block
+ * table [1, prefix_bt_cols], length int64 [1] on the device) and then to its own suffix. The prefix is
+ * read for the rows of all sequences together; the parts are folded in fp32. Either may be empty (both:
+ * out = 0, lse = -inf); the two pools may be one. Arguments otherwise as above.
+ * -------------------------------------------------------------------------- */
+int ck_kv4_cascade_decode_plan(int64_t batch, int64_t num_heads, int64_t kv_heads, int64_t prefix_cap,
+                               int64_t suffix_cap, int64_t *workspace_bytes);
+
+int ck_kv4_cascade_decode(const void *q, const void *prefix_cache, const int32_t *prefix_block_table,
+                          int64_t prefix_bt_cols, const int64_t *prefix_kv_seqlen, int64_t prefix_num_blocks,
+                          const void *suffix_cache, const int32_t *suffix_block_table, int64_t suffix_bt_cols,
+                          const int64_t *suffix_kv_seqlens, int64_t suffix_num_blocks, int64_t batch,
+                          int64_t num_heads, int64_t kv_heads, int64_t block_size, int dtype, float scale, void *out,
+                          float *lse, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ============================================================================
  * Health counter of the bounded waits inside the suffix and fused cascade
  * kernels (ck_suffix_decode, ck_cascade_decode, ck_cascade_decode_noalloc, and
  * ck_fa_fp32_stage1_decode).

@@ -50,6 +50,14 @@ SIGNATURES = {
                                         _int, _f32, _vp, _vp, _vp, _i64, _vp]),
     "ck_latent_prefill": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
                                  _int, _f32, _int, _vp, _vp, _vp]),
+    "ck_kv4_cache_write": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
+    "ck_kv4_cache_read": (_int, [_vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _vp]),
+    "ck_kv4_decode_plan": (_int, [_i64, _i64, _i64, _i64, _i64, _p64]),
+    "ck_kv4_decode": (_int, [_vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _int, _f32, _vp, _vp, _vp,
+                             _i64, _vp]),
+    "ck_kv4_cascade_decode_plan": (_int, [_i64, _i64, _i64, _i64, _i64, _p64]),
+    "ck_kv4_cascade_decode": (_int, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64,
+                                     _int, _f32, _vp, _vp, _vp, _i64, _vp]),
     "ck_wait_giveups": (_int, [ctypes.POINTER(ctypes.c_uint64), _int]),
     "ck_bw_probe": (_int, [_vp, _vp, _i64, _int, _vp, _i64, _vp]),
     "ck_mfma_probe": (_int, [_i64, _vp, _i64, ctypes.POINTER(ctypes.c_double), _vp]),
@@ -61,6 +69,7 @@ CK_DTYPE_F32 = 1
 CK_DTYPE_F16 = 2
 CK_E_SCRATCH_LIMIT = -5
 CASCADE_NOALLOC_SCRATCH_BYTES = 32 << 20
+KV4_PAGE_BYTES = 17408
 CK_KV_NHD = 0
 CK_KV_BNSD = 1
 
@@ -143,4 +152,17 @@ def latent_cascade_plan(batch, num_heads, prefix_cap, suffix_cap):
     w = ctypes.c_int64(0)
     check(lib().ck_latent_cascade_decode_plan(batch, num_heads, prefix_cap, suffix_cap, ctypes.byref(w)),
           "ck_latent_cascade_decode_plan")
+    return w.value
+
+
+def kv4_decode_plan(batch, q_len, num_heads, kv_heads, kv_cap):
+    w = ctypes.c_int64(0)
+    check(lib().ck_kv4_decode_plan(batch, q_len, num_heads, kv_heads, kv_cap, ctypes.byref(w)), "ck_kv4_decode_plan")
+    return w.value
+
+
+def kv4_cascade_plan(batch, num_heads, kv_heads, prefix_cap, suffix_cap):
+    w = ctypes.c_int64(0)
+    check(lib().ck_kv4_cascade_decode_plan(batch, num_heads, kv_heads, prefix_cap, suffix_cap, ctypes.byref(w)),
+          "ck_kv4_cascade_decode_plan")
     return w.value

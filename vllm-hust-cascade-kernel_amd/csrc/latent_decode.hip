@@ -144,17 +144,6 @@ __device__ __forceinline__ int64_t clamp_len(int64_t n, int64_t cols, int64_t nu
 __device__ __forceinline__ int tiles_of(int64_t len) { return (int)((len + kTok - 1) / kTok); }
 __device__ __forceinline__ int places_of(int64_t len) { return len > 0 ? tiles_of(len) + kItemPlaces : 0; }
 
-// op over the four lanes n, 16 + n, 32 + n, 48 + n, in each of them: exchanging the odd rows of
-// 16 lanes (then the upper half) of x with the even ones (the lower half) of x leaves one
-// operand in each result.
-template <class Op>
-__device__ __forceinline__ float over_groups(float x, Op &&op) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
 // Of a row's 32 dims, x its dims 4 g .. + 3 and y its dims 16 + 4 g .. + 3 in lane group g:
 // 8 neighbouring ones, from dim 16 (g & 1) + 8 (g >> 1) on, rounded once to 16 bits.
 template <int DT>
