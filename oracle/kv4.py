@@ -103,14 +103,18 @@ def random_pool(gen, blocks, kv_heads, device, spread=3):
     return pool
 
 
-def attend(q, k, v, sees, scale, dtype):
+def attend(q, k, v, sees, scale, dtype, rows):
     """Rows q [n, 128] over keys and values [m, 128]; row i sees the first sees[i] (a list, or one
-    number). Returns (o, lse, bound of |out - o|, bound of |out lse - lse|).
+    number); the call has `rows` of them a kv head. Returns (o, lse, bound of |out - o|, bound of
+    |out lse - lse|).
 
     out rounds by half a step u |o| (fp16 also by half its least step, 2^-25). A score is an fp32 sum of 128
     exact products, (128 + 8) roundings of partial sums below sum |q| |k|, times the scale (2 roundings,
     its conversion to log2 among them); an error e of the scores moves a softmax weight by 2 e of it. P enters
-    as two bf16 terms, off by 2^-18 of it. The sums over m tokens are fp32; exp2 is good to a few steps."""
+    as two bf16 terms, off by 2^-18 of it, or (more than 16 rows a kv head) as an fp16 number, off by 2^-11 of it; 2^7 p
+    then loses bits in steps of 2^-24 where the largest weight is 1 or more: 2^-32 of it for each token, and so
+    does a value below 2^-14, a scale of 2^-23 or more leaving it its bits. The sums over m tokens are fp32;
+    exp2 is good to a few steps."""
     q, k, v = q.double(), k.double(), v.double()
     n, m = q.shape[0], k.shape[0]
     sees = torch.as_tensor(sees, device=q.device).clamp(0, m).expand(n)
@@ -125,7 +129,8 @@ def attend(q, k, v, sees, scale, dtype):
     u = torch.finfo(dtype).eps / 2
     e = (128 + 8 + 2) * F32 * (q.abs() @ k.abs().T).masked_fill(hidden, 0).amax(1) * scale
     sums = (sees + 64) * F32
-    b_o = u * o.abs() + (1 + u) * (2.0 ** -18 + 2 * e + sums)[:, None] * mean
+    p_off, lost = (2.0 ** -18, 0.0) if rows <= 16 else (2.0 ** -11, 2.0 ** -32)
+    b_o = u * o.abs() + (1 + u) * ((p_off + 2 * e + sums)[:, None] * mean + (sees * lost)[:, None] * v.abs().amax())
     if dtype == torch.float16:
         b_o = b_o + 2.0 ** -25
     return o, lse, b_o, e + sums + 8 * F32 * lse.nan_to_num(0, 0, 0).abs()

@@ -123,7 +123,7 @@ def _check_decode(q, pool, table, lens, scale, q_len, got):
         k, v = o4.cached(pool, table[b], n)
         sees = (n - q_len + 1 + torch.arange(q_len, device=DEV)).repeat_interleave(grp)
         for h in range(kv_heads):
-            ref = o4.attend(rows[b, :, h].reshape(-1, 128), k[:, h], v[:, h], sees, scale, q.dtype)
+            ref = o4.attend(rows[b, :, h].reshape(-1, 128), k[:, h], v[:, h], sees, scale, q.dtype, q_len * grp)
             close(out[b, :, h].reshape(-1, 128), lse[b, :, h].reshape(-1), ref)
 
 
@@ -168,5 +168,5 @@ def test_cascade(prefix, suffixes, heads, kv_heads, dtype):
         k, v = torch.cat([pk, k]), torch.cat([pv, v])
         for h in range(kv_heads):
             hs = slice(h * grp, (h + 1) * grp)
-            ref = o4.attend(q[b, hs], k[:, h], v[:, h], prefix + n, SCALE, dtype)
+            ref = o4.attend(q[b, hs], k[:, h], v[:, h], prefix + n, SCALE, dtype, grp * len(suffixes))
             close(out[b, hs], lse.view(-1, heads)[b, hs], ref)

@@ -87,7 +87,8 @@ def assembly(src):
 OWN_ACC_REGISTERS = ["latent_decode.hip"]
 # Sources with instructions in inline assembly: the build looks for the waits that the compiler does
 # not insert there (asm_waits.py).
-CHECKED_WAITS = ["fa_stage1.hip", "suffix_decode.hip", "gateup_swiglu.hip", "latent_decode.hip", "latent_prefill.hip"]
+CHECKED_WAITS = ["fa_stage1.hip", "suffix_decode.hip", "gateup_swiglu.hip", "latent_decode.hip", "latent_prefill.hip",
+                 "kv4_decode.hip"]
 
 
 def check_acc_registers(asm):

@@ -37,10 +37,15 @@ template <int B>
 __device__ __forceinline__ uint32_t pair_bf16(uint32_t w, float scale) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, B));
 }
+template <int B>
+__device__ __forceinline__ uint32_t pair_f16(uint32_t w, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, B));
+}
 // Byte B of four scales, in the exponent field (the other bits hold what was beside it).
 template <int B>
 __device__ __forceinline__ float scale_of(uint32_t w) {
-    return __uint_as_float(B == 3 ? w >> 1 : w << (23 - 8 * B));
+    if constexpr (B == 3) return __uint_as_float(w >> 1);
+    else return __uint_as_float(w << (23 - 8 * B));
 }
 
 }  // namespace kv4

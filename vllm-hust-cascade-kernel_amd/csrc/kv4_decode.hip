@@ -28,15 +28,19 @@
 
 #include "kv4_common.h"
 #include "kv4_map.h"
+#include "latent_common.h"
 
 namespace ck {
 namespace {
 
 using namespace kv4;
 
+typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
+
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kGroups = 512;  // workgroups: two per CU
+constexpr int kGroupsWide = 256;  // of many rows: one per CU
 constexpr int kFoldRows = 4096;  // from which on a row's parts are folded by one group of lanes
 constexpr float kSlack = 8.f;
 constexpr uint32_t kRsrcFlags = 0x00020000;
@@ -52,7 +56,8 @@ struct DecodeArgs {
     int group;   // query heads per kv head
     int rows;    // q_len * group: of an item
     int tiles;   // row tiles of an item
-    int waves;   // that share the list, per row tile
+    int tile_rows;
+    int waves;   // shares of the list (waves', or with many rows workgroups'), per row tile
     int causal;
     int merge;   // every part goes to the workspace
     float scale_log2;
@@ -64,13 +69,101 @@ struct DecodeArgs {
     int32_t *sums;    // [batch + 1]: units before each request (of one kv head)
 };
 
-__device__ __forceinline__ int len_of(const DecodeArgs &a, int b) {
-    const int64_t cap = a.bt_cols * kPage;
-    int64_t n = a.lens[b];
+// The arguments, read where they are used: held in scalar registers throughout they would spill.
+typedef const __attribute__((address_space(4))) DecodeArgs *KernArgs;
+__device__ __forceinline__ KernArgs args_again(KernArgs a) {
+    asm volatile("" : "+s"(a));
+    return a;
+}
+// The lane, so that what depends on it is computed where it is used.
+__device__ __forceinline__ int lane_again(int lane) {
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
+__device__ __forceinline__ int len_of(KernArgs a, int b) {
+    const int64_t cap = a->bt_cols * kPage;
+    int64_t n = a->lens[b];
     if (n > cap) n = cap;
-    return n < 0 || a.num_blocks <= 0 ? 0 : (int)n;
+    return n < 0 || a->num_blocks <= 0 ? 0 : (int)n;
 }
 __device__ __forceinline__ int units_of(int len) { return (len + kUnit - 1) / kUnit; }
+
+// starts[t]: units (of one kv head) before thread t's requests, t's share of the batch, len0[t] the first one's
+// length. Returns the units in all; the first workgroup leaves those before each request for the fold.
+template <int T>
+__device__ __forceinline__ int requests_per_thread(KernArgs a) { return (a->batch + T - 1) / T; }
+template <int T>
+__device__ __forceinline__ int list_starts(KernArgs a, int *starts, int *len0, int *scan, int tid) {
+    const int per = requests_per_thread<T>(a), b0 = min(tid * per, a->batch), b1 = min(b0 + per, a->batch);
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) {
+        const int len = len_of(a, b);
+        if (b == b0) len0[tid] = len;
+        mine += units_of(len);
+    }
+    const int incl = (int)wave_scan((uint32_t)mine, 0x7fffffffu);
+    if ((tid & 63) == 63) scan[tid >> 6] = incl;
+    __syncthreads();
+    int start = incl - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) {
+        if (w < tid >> 6) start += scan[w];
+        total += scan[w];
+    }
+    starts[tid] = start;
+    if (blockIdx.x == 0) {
+        int at = start;
+        for (int b = b0; b < b1; ++b) {
+            a->sums[b] = at;
+            at += units_of(len_of(a, b));
+        }
+        if (tid == 0) a->sums[a->batch] = total;
+    }
+    __syncthreads();
+    return total;
+}
+// The request that holds place u of the list, its first place and its length.
+struct Found {
+    int b, at, len;
+};
+// x: the last thread whose requests begin at or before u.
+template <int T>
+__device__ __forceinline__ Found find_from(KernArgs a, const int *starts, const int *len0, int u, int x) {
+    Found f;
+    f.b = min(x * requests_per_thread<T>(a), a->batch - 1);
+    f.at = starts[x] * a->kv_heads;
+    f.len = len0[x];
+    while (f.b + 1 < a->batch && f.at + units_of(f.len) * a->kv_heads <= u) {  // of the thread's
+        f.at += units_of(f.len) * a->kv_heads;
+        f.len = len_of(a, ++f.b);
+    }
+    return f;
+}
+template <int T>
+__device__ __forceinline__ Found find_request(KernArgs a, const int *starts, const int *len0, int u) {  // u a lane
+    int x = 0;
+#pragma unroll
+    for (int step = T / 2; step > 0; step >>= 1)
+        if (starts[x + step] * a->kv_heads <= u) x += step;
+    return find_from<T>(a, starts, len0, u, x);
+}
+template <int T>
+__device__ __forceinline__ Found find_request_of_wave(KernArgs a, const int *starts, const int *len0, int u, int lane) {
+    constexpr int kEach = T / 64;
+    const int some = __popcll(__builtin_amdgcn_ballot_w64(starts[kEach * lane] * a->kv_heads <= u)) - 1;
+    const int more = __popcll(__builtin_amdgcn_ballot_w64(lane < kEach && starts[kEach * some + lane % kEach] * a->kv_heads <= u)) - 1;
+    return find_from<T>(a, starts, len0, u, scalar(kEach * some + more));
+}
+// A unit's place in memory; bit 0 (addresses are 16-byte aligned) marks a page outside the pool.
+__device__ __forceinline__ uint64_t unit_address(KernArgs a, int b, int h, int i) {
+    const int page = a->bt[(int64_t)b * a->bt_cols + (i >> 1)];
+    const bool ok = page >= 0 && page < a->num_blocks;
+    return (uint64_t)(uintptr_t)a->cache + (ok ? (((uint64_t)(uint32_t)page * a->kv_heads + h) * 2 + (i & 1)) * kUnitBytes : 1);
+}
+__device__ __forceinline__ uint64_t of_lane(uint64_t x, int lane) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+}
 
 // A unit as a wave's lanes hold it: lane (g, n) has group g of keys 8 (n / 4) + n % 4 + {0, 4, 32, 36}
 // and their scales, dims 8 n + 2 q, + 1 of values 8 g .. + 7 and 32 + 8 g .. + 7, and these tokens' scales of dim
@@ -78,9 +171,66 @@ __device__ __forceinline__ int units_of(int len) { return (len + kUnit - 1) / kU
 struct Unit {
     u32x4 k[4], v[4], vs;
     uint32_t ks;
+    __device__ __forceinline__ u32x4 keys(int t) const { return k[t]; }
+    __device__ __forceinline__ u32x4 values(int q) const { return v[q]; }
 };
-__device__ __forceinline__ void load_unit(Unit &u, const char *base, int range, int lane) {
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), (short)0, range, kRsrcFlags);
+// Where a lane's keys lie in a unit in LDS, those of tile t at + 2048 (t / 2) + 256 (t % 2).
+__device__ __forceinline__ int keys_in_lds(int lane) {
+    const int n = lane & 15;
+    return (8 * (n >> 2) + (n & 3)) * 64 + 16 * ((lane >> 4) ^ (n >> 2));
+}
+// A unit in LDS: what is needed is read where it is.
+struct UnitInLds {
+    const CK_LDS char *k_at, *at;  // the lane's
+    u32x4 vs;
+    uint32_t ks;
+    __device__ __forceinline__ u32x4 keys(int t) const {
+        return *reinterpret_cast<const CK_LDS u32x4 *>(k_at + 2048 * (t >> 1) + 256 * (t & 1));
+    }
+    __device__ __forceinline__ u32x4 values(int q) const { return *reinterpret_cast<const CK_LDS u32x4 *>(at + kVAt + 1024 * q); }
+};
+// The same in the compiler's eyes new: what one of two ways through computes from it is not made before them, for
+// both.
+__device__ __forceinline__ u32x4 again(u32x4 x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+// A unit's way to LDS: 10 moves without a register between, 16 bytes a lane of the codes and 4 of the scales. All lie as
+// in memory, but a token's four groups of key codes are exchanged by (token / 8) % 4: the 16 lanes that read one
+// group of 16 tokens, 4 tokens in a row of 8, then touch every bank once.
+constexpr int kPieces = 10;
+template <int IMM>
+__device__ __forceinline__ void dma_words(const ck_rsrc_t &r, int voff, int soff, int base) {
+    asm volatile("s_add_i32 m0, %0, %c1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, %4 offen lds"
+                 :
+                 : "s"(base), "i"(IMM), "v"(voff), "s"(r), "s"(soff)
+                 : "memory", "m0", "scc");
+}
+// The unit at `at` (unit_address) to a slot of kUnitBytes; from a page outside the pool, zeros (a range of nothing).
+__device__ __forceinline__ void move_unit(uint64_t at, const CK_LDS char *slot, int lane) {
+    const ck_rsrc_t r = {(int)(uint32_t)(at & ~1ull), (int)((uint32_t)(at >> 32) & 0xffffu), at & 1 ? 0 : kUnitBytes,
+                         (int)kRsrcFlags};
+    const int base = scalar((int)(uint32_t)(uintptr_t)slot);
+    const int keys = (lane >> 2) * 64 + 16 * ((lane & 3) ^ (lane >> 5));  // tokens 16 P + lane / 4
+    static_for<8>([&](auto p) __attribute__((always_inline)) {
+        constexpr int P = p;
+        lat::dma_tile<1024 * P>(r, P >= 4 ? 16 * lane : P % 2 ? keys ^ 32 : keys, 1024 * P, base);
+    });
+    dma_words<kKsAt>(r, 4 * lane, kKsAt, base);
+    dma_words<kVsAt>(r, 4 * lane, kVsAt, base);
+}
+__device__ __forceinline__ UnitInLds unit_in(const CK_LDS char *slot, int lane) {
+    UnitInLds u;
+    u.k_at = slot + keys_in_lds(lane);
+    u.at = slot + 16 * lane;
+    u.ks = *reinterpret_cast<const CK_LDS uint32_t *>(slot + kKsAt + 4 * lane);
+    u.vs = *reinterpret_cast<const CK_LDS u32x4 *>(slot + kVsAt + ((lane & 15) >> 2) * 64 + 16 * (lane >> 4));
+    return u;
+}
+
+__device__ __forceinline__ void load_unit(Unit &u, uint64_t at, int lane) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char *>((uintptr_t)(at & ~1ull)), (short)0,
+                                                                       at & 1 ? 0 : kUnitBytes, kRsrcFlags);
     const int n = lane & 15, g = lane >> 4;
     const int k_at = (8 * (n >> 2) + (n & 3)) * 64 + 16 * g, v_at = kVAt + 16 * lane;
 #pragma unroll
@@ -93,86 +243,249 @@ __device__ __forceinline__ void load_unit(Unit &u, const char *base, int range, 
         u.v[q] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, v_at + 1024 * q, 0, 0));
 }
 
-__device__ __forceinline__ f32x4 mfma_bf16(u32x4 x, u32x4 y, f32x4 c) { return Elem<CK_DTYPE_BF16>::mfma16(x, y, c); }
+// How a wave of NB row blocks computes. One row block is bound by memory: P enters the second product as two
+// bf16 terms, within 2^-17 of fp32, an fp16 query the first as two bf16 terms, which hold all of it. More row blocks
+// are bound by arithmetic: where a unit's scales lie in [2^-23, 2^8] fp16 holds every value, and P is one fp16
+// number, 2^7 p (fp16's normal range ends at 2^-14; with the largest score at most 2^kSlack past the reference
+// point 2^7 p stays below 65504), half a step off, 2^-11; so does an fp16 query's key. Units of other scales are
+// computed as above. 24 x 3 x 64 heads over 5000 tokens (fp16): 36.7 -> 27.9 us, the units in LDS instead of
+// registers among it.
+template <int DT, int NB>
+struct Form {
+    static constexpr bool kHalf = NB > 1;
+    static constexpr int kTerms = DT == CK_DTYPE_F16 && !kHalf ? 2 : 1;  // of the query, as it is held
+    static constexpr float kBias = kHalf ? 7.f : 0.f;
+};
 
 // The rows of a wave: row 16 i + n in lanes (g, n).
 template <int DT, int NB>
 struct Rows {
-    static constexpr int kTerms = DT == CK_DTYPE_BF16 ? 1 : 2;
-    u32x4 q[NB][kTerms][4];  // dims 32 g + 8 c .. + 7
-    f32x4 o[NB][8];          // O^T: dims 32 g + 8 r + block of the row
-    float m[NB], l[NB];      // reference point (log2; the same for all g), this lane's share of the sum
+    u32x4 q[NB][Form<DT, NB>::kTerms][4];  // dims 32 g + 8 c .. + 7
+    f32x4 o[NB][8];  // O^T: dims 32 g + 8 r + block of the row
+    float m[NB];     // the sum's reference point (log2; the same for all g) is m - kBias
+    float l[NB];     // this lane's share of the sum
+    uint32_t bad;    // bit i: row i sees a value that is not a number in this lane's dims
 };
-
-// Bytes of four scales whose tokens are the first `n` of the four.
-__device__ __forceinline__ uint32_t first_bytes(uint32_t w, int n) {
-    return n >= 4 ? w : n <= 0 ? 0u : w & ((1u << (8 * n)) - 1);
+template <int DT, int NB>
+__device__ __forceinline__ void clear(Rows<DT, NB> &s) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s.o[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        s.m[i] = -INFINITY;
+        s.l[i] = 0.f;
+    }
+    s.bad = 0;
+}
+// Gives O what hide_values() has put off.
+template <int NB>
+__device__ __forceinline__ void add_bad(f32x4 (&o)[NB][8], uint32_t bad) {
+    if (__builtin_expect(!__builtin_amdgcn_ballot_w64(bad != 0), 1)) return;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[i][k][r] = (bad >> i) & 1 ? NAN : o[i][k][r];
 }
 
-// O^T += V^T P^T over a unit, vs the values' scales; P of row block i as operands hi, lo [i][half].
-template <int DT, int NB>
-__device__ __forceinline__ void add_values(Rows<DT, NB> &s, const Unit &u, u32x4 vs, const u32x4 (&hi)[NB][2],
-                                           const u32x4 (&lo)[NB][2]) {
+__device__ __forceinline__ f32x4 mfma_bf16(u32x4 x, u32x4 y, f32x4 c) { return Elem<CK_DTYPE_BF16>::mfma16(x, y, c); }
+__device__ __forceinline__ f32x4 mfma_f16(u32x4 x, u32x4 y, f32x4 c) { return Elem<CK_DTYPE_F16>::mfma16(x, y, c); }
+
+// fp16 numbers as two bf16 terms.
+__device__ __forceinline__ void two_terms(u32x4 x, u32x4 &hi, u32x4 &lo) {
+    using E = Elem<CK_DTYPE_F16>;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        hi[e] = pack_bf16x2(E::lo(x[e]), E::hi(x[e]));
+        lo[e] = pack_bf16x2(E::lo(x[e]) - bf16_lo(hi[e]), E::hi(x[e]) - bf16_hi(hi[e]));
+    }
+}
+
+// Nonzero where a scale byte of w is outside [104, 135] (2^-23 to 2^8).
+constexpr uint32_t kMidScales = 0x68686868;
+__device__ __forceinline__ uint32_t past_half(uint32_t w) { return ((w + 0x18181818) ^ 0x80808080) & 0xe0e0e0e0; }
+
+// Scores of a unit's 16 tokens t, HALF: of fp16 numbers.
+template <bool HALF, int DT, int NB>
+__device__ __forceinline__ void add_scores(const Rows<DT, NB> &s, const u32x4 &codes, float scale, f32x4 (&sc)[NB][4], int t) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const uint32_t w = codes[c];
+        u32x4 a;
+        if constexpr (HALF) a = u32x4{pair_f16<0>(w, scale), pair_f16<1>(w, scale), pair_f16<2>(w, scale), pair_f16<3>(w, scale)};
+        else a = u32x4{pair_bf16<0>(w, scale), pair_bf16<1>(w, scale), pair_bf16<2>(w, scale), pair_bf16<3>(w, scale)};
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            if constexpr (HALF) {
+                sc[i][t] = mfma_f16(a, s.q[i][0][c], sc[i][t]);
+            } else if constexpr (DT == CK_DTYPE_F16 && Form<DT, NB>::kTerms == 1) {
+                u32x4 hi, lo;
+                two_terms(s.q[i][0][c], hi, lo);
+                sc[i][t] = mfma_bf16(a, hi, sc[i][t]);
+                sc[i][t] = mfma_bf16(a, lo, sc[i][t]);
+            } else {
+#pragma unroll
+                for (int x = 0; x < Form<DT, NB>::kTerms; ++x) sc[i][t] = mfma_bf16(a, s.q[i][x][c], sc[i][t]);
+            }
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+template <bool HALF, int DT, int NB>
+__device__ __forceinline__ void add_scores(const Rows<DT, NB> &s, const u32x4 (&k)[4], uint32_t ks, f32x4 (&sc)[NB][4]) {
+    add_scores<HALF>(s, k[0], scale_of<0>(ks), sc, 0);
+    add_scores<HALF>(s, k[1], scale_of<1>(ks), sc, 1);
+    add_scores<HALF>(s, k[2], scale_of<2>(ks), sc, 2);
+    add_scores<HALF>(s, k[3], scale_of<3>(ks), sc, 3);
+}
+
+// P of row blocks I0 .. I0 + N - 1 over a unit, its sums, and O^T += V^T P^T; vs: the values' scales.
+template <bool HALF, int I0, int N, int DT, int NB>
+__device__ __forceinline__ void add_values(Rows<DT, NB> &s, const u32x4 (&v)[4], u32x4 vs, const f32x4 (&sc)[NB][4], float scale_log2) {
+    constexpr int kParts = HALF ? 1 : 2;
+    u32x4 p[N][kParts][2];  // [term][half of the tokens]
+    asm volatile("" : "+s"(scale_log2));  // not the other form's exponentials
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int i = I0 + k;
+        const float sub = s.m[i] == -INFINITY ? 0.f : s.m[i] - Form<DT, NB>::kBias;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x = exp2_fast(fmaf(sc[i][e >> 1][2 * (e & 1)], scale_log2, -sub));
+            const float y = exp2_fast(fmaf(sc[i][e >> 1][2 * (e & 1) + 1], scale_log2, -sub));
+            sum += x;
+            sum += y;
+            if constexpr (HALF) {
+                p[k][0][e >> 2][e & 3] = Elem<CK_DTYPE_F16>::pack2(x, y);
+            } else {
+                const uint32_t h = pack_bf16x2(x, y);
+                p[k][0][e >> 2][e & 3] = h;
+                p[k][kParts - 1][e >> 2][e & 3] = pack_bf16x2(x - bf16_lo(h), y - bf16_hi(h));
+            }
+        }
+        s.l[i] += sum;
+        __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        float sc[8];
+        float f[8];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-            sc[4 * w] = scale_of<0>(vs[2 * h + w]);
-            sc[4 * w + 1] = scale_of<1>(vs[2 * h + w]);
-            sc[4 * w + 2] = scale_of<2>(vs[2 * h + w]);
-            sc[4 * w + 3] = scale_of<3>(vs[2 * h + w]);
+            f[4 * w] = scale_of<0>(vs[2 * h + w]);
+            f[4 * w + 1] = scale_of<1>(vs[2 * h + w]);
+            f[4 * w + 2] = scale_of<2>(vs[2 * h + w]);
+            f[4 * w + 3] = scale_of<3>(vs[2 * h + w]);
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             u32x4 even, odd;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-                const uint32_t c = u.v[q][2 * h + w];
-                const uint32_t t0 = pair_bf16<0>(c, sc[4 * w]), t1 = pair_bf16<1>(c, sc[4 * w + 1]);
-                const uint32_t t2 = pair_bf16<2>(c, sc[4 * w + 2]), t3 = pair_bf16<3>(c, sc[4 * w + 3]);
-                even[2 * w] = __builtin_amdgcn_perm(t1, t0, 0x05040100);
-                odd[2 * w] = __builtin_amdgcn_perm(t1, t0, 0x07060302);
-                even[2 * w + 1] = __builtin_amdgcn_perm(t3, t2, 0x05040100);
-                odd[2 * w + 1] = __builtin_amdgcn_perm(t3, t2, 0x07060302);
+                const uint32_t c = v[q][2 * h + w];
+                uint32_t t[4];
+                if constexpr (HALF) {
+                    t[0] = pair_f16<0>(c, f[4 * w]), t[1] = pair_f16<1>(c, f[4 * w + 1]);
+                    t[2] = pair_f16<2>(c, f[4 * w + 2]), t[3] = pair_f16<3>(c, f[4 * w + 3]);
+                } else {
+                    t[0] = pair_bf16<0>(c, f[4 * w]), t[1] = pair_bf16<1>(c, f[4 * w + 1]);
+                    t[2] = pair_bf16<2>(c, f[4 * w + 2]), t[3] = pair_bf16<3>(c, f[4 * w + 3]);
+                }
+                even[2 * w] = __builtin_amdgcn_perm(t[1], t[0], 0x05040100);
+                odd[2 * w] = __builtin_amdgcn_perm(t[1], t[0], 0x07060302);
+                even[2 * w + 1] = __builtin_amdgcn_perm(t[3], t[2], 0x05040100);
+                odd[2 * w + 1] = __builtin_amdgcn_perm(t[3], t[2], 0x07060302);
             }
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                s.o[i][2 * q] = mfma_bf16(even, hi[i][h], s.o[i][2 * q]);
-                s.o[i][2 * q + 1] = mfma_bf16(odd, hi[i][h], s.o[i][2 * q + 1]);
-                s.o[i][2 * q] = mfma_bf16(even, lo[i][h], s.o[i][2 * q]);
-                s.o[i][2 * q + 1] = mfma_bf16(odd, lo[i][h], s.o[i][2 * q + 1]);
-            }
+            for (int x = 0; x < kParts; ++x)
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    f32x4 &lo = s.o[I0 + k][2 * q], &hi = s.o[I0 + k][2 * q + 1];
+                    if constexpr (HALF) {
+                        lo = mfma_f16(even, p[k][x][h], lo);
+                        hi = mfma_f16(odd, p[k][x][h], hi);
+                    } else {
+                        lo = mfma_bf16(even, p[k][x][h], lo);
+                        hi = mfma_bf16(odd, p[k][x][h], hi);
+                    }
+                }
             __builtin_amdgcn_sched_barrier(0);
         }
     }
 }
 
+// Moves the reference points of rows whose scores pass them by 2^kSlack (most: the lane's largest) to the
+// largest; no score passes them by as much again.
+template <int NB>
+__device__ __forceinline__ void move_points(f32x4 (&o)[NB][8], float (&m)[NB], float (&l)[NB], const float (&most)[NB]) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const float all = over_groups(most[i], [](float x, float y) { return fmaxf(x, y); });
+        const float to = all > m[i] + kSlack ? all : m[i];
+        const float by = to == m[i] ? 1.f : exp2_fast(m[i] - to);
+        l[i] *= by;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[i][k][r] *= by;
+        m[i] = to;
+    }
+}
+
+// The first n bytes of w, the others `rest`.
+__device__ __forceinline__ uint32_t first_bytes(uint32_t w, int n, uint32_t rest) {
+    const uint32_t mask = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
+    return (w & mask) | (rest & ~mask);
+}
+
+// The values' scales of a half unit that not every row sees whole (sees and left counted from its first token; x, y those
+// of tokens 8 g .. + 7). Those of tokens from `left` on go, and values that are not numbers would reach rows that
+// do not see them (0 times them is none): their scales become ordinary ones, and rows that do see one are marked.
+// A lane (g, n) has the dims of group g of its rows' O.
+template <int NB>
+__device__ __forceinline__ void hide_values(uint32_t &bad, uint32_t &x, uint32_t &y, const int (&sees)[NB], int left, int g) {
+    int first_bad = kUnit;
+#pragma unroll
+    for (int w = 1; w >= 0; --w) {
+        uint32_t &s = w ? y : x;
+        const int t0 = 8 * g + 4 * w;
+        s = first_bytes(s, left - t0, kMidScales);
+#pragma unroll
+        for (int b = 3; b >= 0; --b) {
+            if (((s >> (8 * b)) & 0xff) != kBad) continue;
+            first_bad = t0 + b;
+            s ^= (kBad ^ (kMidScales & 0xff)) << (8 * b);
+        }
+    }
+    if (__builtin_expect(!__builtin_amdgcn_ballot_w64(first_bad < kUnit), 1)) return;
+    first_bad = (int)over_groups((float)first_bad, [](float x, float y) { return fminf(x, y); });
+    first_bad = __shfl(first_bad, 4 * g);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) bad |= first_bad < sees[i] ? 1u << i : 0;
+}
+
 // One unit. Where tail: tokens from sees[i] on are hidden from row block i's row, those from `left` on
 // (counted from the unit's first) hold anything.
-template <int DT, int NB>
-__device__ __forceinline__ void compute(Rows<DT, NB> &s, const Unit &u, float scale_log2, int lane, bool tail,
+template <int DT, int NB, class U>
+__device__ __forceinline__ void compute(Rows<DT, NB> &s, const U &u, float scale_log2, int lane, bool tail,
                                         const int (&sees)[NB], int left) {
-    const int g = lane >> 4;
+    constexpr bool kHalf = Form<DT, NB>::kHalf, kHalfKeys = kHalf && DT == CK_DTYPE_F16;
+    u32x4 k[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) k[t] = u.keys(t);
     f32x4 sc[NB][4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const float ks = t == 0 ? scale_of<0>(u.ks) : t == 1 ? scale_of<1>(u.ks) : t == 2 ? scale_of<2>(u.ks) : scale_of<3>(u.ks);
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int i = 0; i < NB; ++i) sc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 4; ++t) sc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (kHalfKeys && __builtin_expect(!__builtin_amdgcn_ballot_w64(past_half(u.ks) != 0), 1)) add_scores<true>(s, k, u.ks, sc);
+    else add_scores<false>(s, k, u.ks, sc);
+    u32x4 vs = u.vs, v[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const uint32_t w = u.k[t][c];
-            const u32x4 a = {pair_bf16<0>(w, ks), pair_bf16<1>(w, ks), pair_bf16<2>(w, ks), pair_bf16<3>(w, ks)};
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int x = 0; x < Rows<DT, NB>::kTerms; ++x) sc[i][t] = mfma_bf16(a, s.q[i][x][c], sc[i][t]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    }
-    u32x4 vs = u.vs;
-    if (tail) {
+    for (int q = 0; q < 4; ++q) v[q] = u.values(q);
+    if (__builtin_expect(tail, 0)) {
+        const int g = lane_again(lane) >> 4;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             const int n = sees[i] - 8 * g;  // token of sc[i][t][r]: 32 (t / 2) + 8 g + 4 (t % 2) + r
@@ -180,41 +493,21 @@ __device__ __forceinline__ void compute(Rows<DT, NB> &s, const Unit &u, float sc
             for (int e = 0; e < 16; ++e)
                 if (32 * (e >> 3) + (e & 7) >= n) sc[i][e >> 2][e & 3] = -INFINITY;
         }
-        // Values that are not numbers would reach rows that do not see them (0 times them is none): their scales
-        // become the least one, and rows that do see one get it added. A lane (g, n) has the dims of group g.
-        int first_bad = kUnit;
+        int sees2[NB];
 #pragma unroll
-        for (int w = 3; w >= 0; --w) {
-            const int t0 = 32 * (w >> 1) + 8 * g + 4 * (w & 1);
-            vs[w] = first_bytes(vs[w], left - t0);
-#pragma unroll
-            for (int b = 3; b >= 0; --b) {
-                if (((vs[w] >> (8 * b)) & 0xff) != kBad) continue;
-                first_bad = t0 + b;
-                vs[w] &= ~(0xffu << (8 * b));
-            }
-        }
-        if (__builtin_amdgcn_ballot_w64(first_bad < kUnit)) {
-            first_bad = (int)over_groups((float)first_bad, [](float x, float y) { return fminf(x, y); });
-            first_bad = __shfl(first_bad, 4 * g);
-#pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                if (first_bad >= sees[i]) continue;
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s.o[i][k][r] = NAN;
-            }
-        }
+        for (int i = 0; i < NB; ++i) sees2[i] = sees[i] - 32;
+        uint32_t x[4] = {vs[0], vs[1], vs[2], vs[3]};
+        hide_values<NB>(s.bad, x[0], x[1], sees, left, g);
+        hide_values<NB>(s.bad, x[2], x[3], sees2, left - 32, g);
+        vs = u32x4{x[0], x[1], x[2], x[3]};
     }
-    u32x4 hi[NB][2], lo[NB][2];
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
         float most = max3(sc[i][0][0], sc[i][0][1], sc[i][0][2]);
 #pragma unroll
         for (int e = 3; e < 15; e += 2) most = max3(most, sc[i][e >> 2][e & 3], sc[i][(e + 1) >> 2][(e + 1) & 3]);
         most = fmaxf(most, sc[i][3][3]) * scale_log2;
-        if (__builtin_amdgcn_ballot_w64(most > s.m[i] + kSlack)) {
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > s.m[i] + kSlack) != 0, 0)) {
             const float all = over_groups(most, [](float x, float y) { return fmaxf(x, y); });
             const float m = all > s.m[i] + kSlack ? all : s.m[i];
             const float f = m == s.m[i] ? 1.f : exp2_fast(s.m[i] - m);
@@ -225,146 +518,94 @@ __device__ __forceinline__ void compute(Rows<DT, NB> &s, const Unit &u, float sc
                 for (int r = 0; r < 4; ++r) s.o[i][k][r] *= f;
             s.m[i] = m;
         }
-        const float sub = s.m[i] == -INFINITY ? 0.f : s.m[i];
-        float p[16], sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            p[e] = exp2_fast(fmaf(sc[i][e >> 2][e & 3], scale_log2, -sub));
-            sum += p[e];
-        }
-        s.l[i] += sum;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t h = pack_bf16x2(p[2 * e], p[2 * e + 1]);
-            hi[i][e >> 2][e & 3] = h;
-            lo[i][e >> 2][e & 3] = pack_bf16x2(p[2 * e] - bf16_lo(h), p[2 * e + 1] - bf16_hi(h));
-        }
-        __builtin_amdgcn_sched_barrier(0);
     }
-    add_values(s, u, vs, hi, lo);
+    if (kHalf && __builtin_expect(!__builtin_amdgcn_ballot_w64((past_half(vs[0]) | past_half(vs[1]) | past_half(vs[2]) | past_half(vs[3])) != 0), 1))
+        add_values<true, 0, NB>(s, v, vs, sc, scale_log2);
+    else
+        add_values<false, 0, NB>(s, v, again(vs), sc, scale_log2);
 }
 
 template <int DT, int NB>
-__global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(DecodeArgs a) {
-    __shared__ int starts[kThreads], scan[kWaves];
+__global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(DecodeArgs) {
+    const KernArgs args = (KernArgs)__builtin_amdgcn_kernarg_segment_ptr();
+    KernArgs a = args_again(args);
+    __shared__ int starts[kThreads], len0[kThreads], scan[kWaves];
+    __shared__ __attribute__((aligned(16))) char ring[NB > 1 ? kWaves * 2 * kUnitBytes : 16];
     const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
     constexpr int kRows = 16 * NB;
-    constexpr bool kAhead = NB == 1;  // the next item's queries are loaded ahead
+    constexpr bool kQAhead = NB == 1;  // the next item's queries are loaded ahead
 
-    // ---- units before each thread's requests, and in all (of one kv head) --------------------------
-    const int per = (a.batch + kThreads - 1) / kThreads;
-    const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
-    int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += units_of(len_of(a, b));
-    const int incl = (int)wave_scan((uint32_t)mine, 0x7fffffffu);
-    if (lane == 63) scan[wave] = incl;
-    __syncthreads();
-    int start = incl - mine, total = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) start += scan[w];
-        total += scan[w];
-    }
-    total = scalar(total);
-    starts[tid] = start;
-    if (blockIdx.x == 0) {
-        int at = start;
-        for (int b = b0; b < b1; ++b) {
-            a.sums[b] = at;
-            at += units_of(len_of(a, b));
-        }
-        if (tid == 0) a.sums[a.batch] = total;
-    }
-    __syncthreads();
+    const int total = scalar(list_starts<kThreads>(a, starts, len0, scan, tid));
 
     // ---- this wave's share ---------------------------------------------------------------------------
-    // One row tile: neighbouring shares on different CUs, so that few units spread over all of
-    // them; several: a unit's row tiles side by side.
-    const int nw = (int)gridDim.x * kWaves;
-    const int id = a.tiles == 1 ? wave * (int)gridDim.x + (int)blockIdx.x : (int)blockIdx.x * kWaves + wave;
-    if (id >= a.waves * a.tiles) return;
-    const int w = scalar(id / a.tiles), tile = scalar(id - w * a.tiles);
-    const Cut cut = list_cut(total * a.kv_heads, a.waves);
+    // neighbouring shares on different CUs, so that few units spread over all of them
+    const int w = scalar(wave * (int)gridDim.x + (int)blockIdx.x);
+    const Cut cut = list_cut(total * a->kv_heads, a->waves);
     if (w >= cut.chunks) return;
     const int lo = scalar(cut_lo(cut, w)), hi = scalar(cut_lo(cut, w + 1));
-    const int tile_rows = min(kRows, a.rows - kRows * tile), slot_rows = min(kRows, a.rows);
+    const int slot_rows = min(kRows, a->rows);
 
     Rows<DT, NB> s;
     u32x4 next_q[NB][4];
     int tok[NB];  // of row block i's row, among the request's
 #pragma unroll
-    for (int i = 0; i < NB; ++i) tok[i] = (kRows * tile + 16 * i + (lane & 15)) / a.group;
+    for (int i = 0; i < NB; ++i) tok[i] = (16 * i + (lane & 15)) / a->group;
 
-    // The lane again, so that addresses of rows and parts are not held over the units.
-    auto lane_again = [&]() {
-        int x = lane;
-        asm volatile("" : "+v"(x));
-        return x;
-    };
     auto load_q = [&](int item) {
-        const int b = scalar(item / a.kv_heads), h = item - b * a.kv_heads;
-        const int x = lane_again(), n16 = x & 15, g4 = x >> 4;
+        const KernArgs a = args_again(args);
+        const int b = scalar(item / a->kv_heads), h = item - b * a->kv_heads;
+        const int x = lane_again(lane), n16 = x & 15, g4 = x >> 4;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const int r = kRows * tile + 16 * i + n16;
-            const uint16_t *p = a.q + (((int64_t)b * a.q_len + tok[i]) * a.heads + h * a.group + (r - tok[i] * a.group)) * kD + 32 * g4;
+            const int r = 16 * i + n16;
+            const uint16_t *p = a->q + (((int64_t)b * a->q_len + tok[i]) * a->heads + h * a->group + (r - tok[i] * a->group)) * kD + 32 * g4;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 next_q[i][c] = u32x4{0, 0, 0, 0};
-                if (r < a.rows) next_q[i][c] = *reinterpret_cast<const u32x4 *>(p + 8 * c);
+                if (r < a->rows) next_q[i][c] = *reinterpret_cast<const u32x4 *>(p + 8 * c);
             }
         }
     };
     auto open_item = [&](int item) {
-        if constexpr (!kAhead) load_q(item);
+        if constexpr (!kQAhead) load_q(item);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                if constexpr (DT == CK_DTYPE_BF16) {
-                    s.q[i][0][c] = next_q[i][c];
-                } else {
-                    using E = Elem<DT>;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float x = E::lo(next_q[i][c][e]), y = E::hi(next_q[i][c][e]);
-                        const uint32_t top = pack_bf16x2(x, y);
-                        s.q[i][0][c][e] = top;
-                        s.q[i][Rows<DT, NB>::kTerms - 1][c][e] = pack_bf16x2(x - bf16_lo(top), y - bf16_hi(top));
-                    }
-                }
+                constexpr int kTerms = Form<DT, NB>::kTerms;
+                if constexpr (kTerms == 1) s.q[i][0][c] = next_q[i][c];
+                else two_terms(next_q[i][c], s.q[i][0][c], s.q[i][kTerms - 1][c]);
             }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) s.o[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
-            s.m[i] = -INFINITY;
-            s.l[i] = 0.f;
         }
+        clear(s);
     };
     auto close_item = [&](int item, bool before, bool after) {
-        const int b = scalar(item / a.kv_heads), h = item - b * a.kv_heads;
-        const int x = lane_again(), n16 = x & 15, g4 = x >> 4;
-        const bool whole = !before && !after && !a.merge;
-        const int64_t slot = part_slot(before, after, w, a.waves, item) * a.tiles + tile;
+        const KernArgs a = args_again(args);
+        const int b = scalar(item / a->kv_heads), h = item - b * a->kv_heads;
+        const int x = lane_again(lane), n16 = x & 15, g4 = x >> 4;
+        add_bad<NB>(s.o, s.bad);
+        const bool whole = !before && !after && !a->merge;
+        const int64_t slot = part_slot(before, after, w, a->waves, item);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const int r = kRows * tile + 16 * i + n16;
-            const float l = over_groups(s.l[i], [](float x, float y) { return x + y; });
-            if (r >= a.rows) continue;
+            const int r = 16 * i + n16;
+            const float l = over_groups(s.l[i], [](float x, float y) { return x + y; }), m = s.m[i] - Form<DT, NB>::kBias;
+            if (r >= a->rows) continue;
             if (whole) {
                 using E = Elem<DT>;
-                const int64_t row = ((int64_t)b * a.q_len + tok[i]) * a.heads + h * a.group + (r - tok[i] * a.group);
+                const int64_t row = ((int64_t)b * a->q_len + tok[i]) * a->heads + h * a->group + (r - tok[i] * a->group);
                 const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
                     u32x4 x;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[e] = E::pack2(s.o[i][2 * e][d] * inv, s.o[i][2 * e + 1][d] * inv);
-                    *reinterpret_cast<u32x4 *>(a.out + row * kD + 32 * g4 + 8 * d) = x;
+                    *reinterpret_cast<u32x4 *>(a->out + row * kD + 32 * g4 + 8 * d) = x;
                 }
-                if (g4 == 0) a.lse[row] = l == 0.f ? -INFINITY : (s.m[i] + __log2f(l)) * kLn2;
+                if (g4 == 0) a->lse[row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
             } else {
                 const int at = 16 * i + n16;
-                float *p = a.part_o + slot * slot_rows * kD;
+                float *p = a->part_o + slot * slot_rows * kD;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     // dims 32 g + 4 j + e: 8 (j / 2) + block 4 (j % 2) + e
@@ -372,7 +613,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(DecodeArgs a) {
                                      s.o[i][4 * (j & 1) + 2][j >> 1], s.o[i][4 * (j & 1) + 3][j >> 1]};
                     *reinterpret_cast<f32x4 *>(p + ((j * slot_rows + at) * 4 + g4) * 4) = x;
                 }
-                if (g4 == 0) a.part_ml[slot * slot_rows + at] = make_float2(s.m[i], l);
+                if (g4 == 0) a->part_ml[slot * slot_rows + at] = make_float2(m, l);
             }
         }
     };
@@ -381,42 +622,32 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(DecodeArgs a) {
     int item = -1;
     bool before = false, goes_on = false;  // the open item: begun in an earlier share; its last unit not seen yet
     for (int base = lo; base < hi; base += 64) {
+        a = args_again(args);
         const int n = min(64, hi - base);
         int d_item = 0, d_first = 0, d_len = 0;
         uint64_t d_at = 0;
         if (lane < n) {
             const int u = base + lane;
-            int x = 0;  // the last thread whose requests begin at or before u and that has some
-#pragma unroll
-            for (int step = kThreads / 2; step > 0; step >>= 1)
-                if (starts[x + step] * a.kv_heads <= u) x += step;
-            int b = min(x * per, a.batch - 1), at = starts[x] * a.kv_heads;
-            int len = len_of(a, b);
-            while (b + 1 < a.batch && at + units_of(len) * a.kv_heads <= u) {  // the thread's request that holds u
-                at += units_of(len) * a.kv_heads;
-                len = len_of(a, ++b);
-            }
-            const int each = units_of(len), h = (u - at) / each, i = u - at - h * each;
-            const int page = a.bt[(int64_t)b * a.bt_cols + (i >> 1)];
-            const bool ok = page >= 0 && page < a.num_blocks;
-            d_item = b * a.kv_heads + h;
+            const Found f = find_request<kThreads>(a, starts, len0, u);
+            const int each = units_of(f.len), h = (u - f.at) / each, i = u - f.at - h * each;
+            d_item = f.b * a->kv_heads + h;
             d_first = i * kUnit;
-            d_len = len;
-            d_at = (uint64_t)(uintptr_t)a.cache;  // 16-byte aligned: bit 0 marks an invalid page
-            d_at += ok ? (((uint64_t)(uint32_t)page * a.kv_heads + h) * 2 + (i & 1)) * kUnitBytes : 1;
+            d_len = f.len;
+            d_at = unit_address(a, f.b, h, i);
         }
-        auto unit_at = [&](Unit &u, int j) {
-            const uint64_t at = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(d_at >> 32), j) << 32) |
-                                (uint32_t)__builtin_amdgcn_readlane((int)d_at, j);
-            // a range of nothing reads zeros
-            load_unit(u, reinterpret_cast<const char *>((uintptr_t)(at & ~1ull)), at & 1 ? 0 : kUnitBytes, lane);
-        };
+        // One row block: the next unit in registers; more: in the wave's other half of its ring.
         Unit next;
-        unit_at(next, 0);
-        if (const int first = __builtin_amdgcn_readlane(d_item, 0); kAhead && first != item) load_q(first);
+        CK_LDS char *slots = (CK_LDS char *)ring + (NB > 1 ? wave * 2 * kUnitBytes : 0);
+        auto fetch = [&](int j) {
+            const uint64_t at = of_lane(d_at, j);
+            if constexpr (NB > 1) move_unit(at, slots + (j & 1) * kUnitBytes, lane_again(lane));
+            else load_unit(next, at, lane);
+        };
+        fetch(0);
+        if (const int first = __builtin_amdgcn_readlane(d_item, 0); kQAhead && first != item) load_q(first);
 #pragma unroll 1
         for (int j = 0; j < n; ++j) {
-            const Unit u = next;
+            const Unit in_registers = next;
             const int it = __builtin_amdgcn_readlane(d_item, j), first = __builtin_amdgcn_readlane(d_first, j);
             const int len = __builtin_amdgcn_readlane(d_len, j);
             if (it != item) {
@@ -427,17 +658,390 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(DecodeArgs a) {
             }
             goes_on = first + kUnit < len;
             if (j + 1 < n) {
-                unit_at(next, j + 1);
-                if (const int then = __builtin_amdgcn_readlane(d_item, j + 1); kAhead && then != it) load_q(then);
+                fetch(j + 1);
+                if (const int then = __builtin_amdgcn_readlane(d_item, j + 1); kQAhead && then != it) load_q(then);
             }
-            const int left = len - first, first_sees = a.causal ? left - a.q_len + 1 : left;
+            const int left = len - first, first_sees = a->causal ? left - a->q_len + 1 : left;
             int sees[NB];
 #pragma unroll
-            for (int i = 0; i < NB; ++i) sees[i] = a.causal ? first_sees + tok[i] : left;
-            compute<DT, NB>(s, u, a.scale_log2, lane, first_sees < kUnit, sees, left);
+            for (int i = 0; i < NB; ++i) sees[i] = a->causal ? first_sees + tok[i] : left;
+            if constexpr (NB > 1) {
+                if (j + 1 < n) wait_vmcnt<kPieces>();
+                else wait_vmcnt<0>();
+                asm volatile("" ::: "memory");
+                compute<DT, NB>(s, unit_in(slots + (j & 1) * kUnitBytes, lane), a->scale_log2, lane, first_sees < kUnit, sees, left);
+            } else {
+                compute<DT, NB>(s, in_registers, a->scale_log2, lane, first_sees < kUnit, sees, left);
+            }
         }
     }
     close_item(item, before, goes_on);
+}
+
+// ---- many rows ---------------------------------------------------------------------------------------------
+// The same for items of more than 32 rows, on workgroups of 8 waves with a CU to themselves, two per SIMD, which fill
+// each other's waits. A workgroup takes a row tile of 64 rows, whose query is in LDS (O alone takes half of a wave's
+// registers); its waves take an item's units in turn, each through a double buffer of its own in LDS, so that
+// nothing holds them together: with a ring that all read, and a barrier for every 4 units, 117 x 64 heads on 16001 tokens
+// took 108 to 118 us. Their parts are joined through LDS, so that few go to memory. A wave works in halves of 32 tokens.
+// The shares of the list are workgroups', neighbours on one XCD, so that the row tiles of a share meet in its L2.
+constexpr int kWideThreads = 512, kWideWaves = kWideThreads / 64;
+constexpr int kWideQ = kWideWaves * 2 * kUnitBytes;  // [NB][4] operands of 1 KB, behind the waves' buffers
+constexpr int kWideStarts = kWideQ + 4 * 4 * 1024;
+constexpr int kWideLds = kWideStarts + (2 * kWideThreads + kWideWaves) * 4;
+constexpr int kWidePart = (4 * 8 + 2) * 1024;  // a wave's O, m and l as its lanes hold them, in the buffers' and the query's place
+static_assert(kWideWaves / 2 * kWidePart <= kWideStarts && kWideLds <= 160 * 1024, "LDS");
+
+// A half unit (tokens 32 h .. + 31) as a wave's lanes hold it.
+struct Half {
+    u32x4 k[2];
+    uint32_t ks, v[4][2], vs[2];
+};
+typedef __attribute__((__vector_size__(2 * sizeof(unsigned)))) unsigned u32x2;
+__device__ __forceinline__ void read_half(Half &x, const CK_LDS char *slot, int h, int lane) {
+    const CK_LDS char *at = slot + 16 * lane;
+    const CK_LDS char *k_at = slot + keys_in_lds(lane) + 2048 * h;
+    x.k[0] = *reinterpret_cast<const CK_LDS u32x4 *>(k_at);
+    x.k[1] = *reinterpret_cast<const CK_LDS u32x4 *>(k_at + 256);
+    x.ks = *reinterpret_cast<const CK_LDS uint16_t *>(slot + kKsAt + 4 * lane + 2 * h);
+    const u32x2 s = *reinterpret_cast<const CK_LDS u32x2 *>(slot + kVsAt + ((lane & 15) >> 2) * 64 + 16 * (lane >> 4) + 8 * h);
+    x.vs[0] = s[0], x.vs[1] = s[1];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const u32x2 y = *reinterpret_cast<const CK_LDS u32x2 *>(at + kVAt + 1024 * d + 8 * h);
+        x.v[d][0] = y[0], x.v[d][1] = y[1];
+    }
+}
+
+// Scores of a half; q: the lane's place in the query's operands.
+template <bool HALF, int DT, int NB>
+__device__ __forceinline__ void half_scores(f32x4 (&sc)[NB][2], const Half &x, const CK_LDS char *q) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) sc[i][0] = sc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float f[2] = {scale_of<0>(x.ks), scale_of<1>(x.ks)};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        u32x4 a[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint32_t w = x.k[t][c];
+            if constexpr (HALF) a[t] = u32x4{pair_f16<0>(w, f[t]), pair_f16<1>(w, f[t]), pair_f16<2>(w, f[t]), pair_f16<3>(w, f[t])};
+            else a[t] = u32x4{pair_bf16<0>(w, f[t]), pair_bf16<1>(w, f[t]), pair_bf16<2>(w, f[t]), pair_bf16<3>(w, f[t])};
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const u32x4 y = *reinterpret_cast<const CK_LDS u32x4 *>(q + (4 * i + c) * 1024);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if constexpr (HALF) {
+                    sc[i][t] = mfma_f16(a[t], y, sc[i][t]);
+                } else if constexpr (DT == CK_DTYPE_F16) {
+                    u32x4 hi, lo;
+                    two_terms(y, hi, lo);
+                    sc[i][t] = mfma_bf16(a[t], hi, sc[i][t]);
+                    sc[i][t] = mfma_bf16(a[t], lo, sc[i][t]);
+                } else {
+                    sc[i][t] = mfma_bf16(a[t], y, sc[i][t]);
+                }
+            }
+        }
+        if (NB > 2 || !HALF) __builtin_amdgcn_sched_barrier(0);
+    }
+}
+// The largest score of a row block's lane.
+__device__ __forceinline__ float largest(const f32x4 (&s)[2]) {
+    float x = max3(s[0][0], s[0][1], s[0][2]);
+    x = max3(x, s[0][3], s[1][0]);
+    x = max3(x, s[1][1], s[1][2]);
+    return fmaxf(x, s[1][3]);
+}
+
+// P of row blocks I0 .. I0 + N - 1 over a half, its sums, and O^T += V^T P^T.
+template <bool HALF, int I0, int N, int NB>
+__device__ __forceinline__ void half_values(f32x4 (&o)[NB][8], float (&l)[NB], const float (&m)[NB], const Half &x,
+                                            const f32x4 (&sc)[NB][2], float scale_log2) {
+    constexpr int kParts = HALF ? 1 : 2;
+    u32x4 p[N][kParts];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int i = I0 + k;
+        const float sub = m[i] == -INFINITY ? 0.f : m[i] - Form<CK_DTYPE_BF16, NB>::kBias;
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float a = exp2_fast(fmaf(sc[i][e >> 1][2 * (e & 1)], scale_log2, -sub));
+            const float b = exp2_fast(fmaf(sc[i][e >> 1][2 * (e & 1) + 1], scale_log2, -sub));
+            sum[0] += a;
+            sum[1] += b;
+            if constexpr (HALF) {
+                p[k][0][e] = Elem<CK_DTYPE_F16>::pack2(a, b);
+            } else {
+                p[k][0][e] = pack_bf16x2(a, b);
+                p[k][kParts - 1][e] = pack_bf16x2(a - bf16_lo(p[k][0][e]), b - bf16_hi(p[k][0][e]));
+            }
+        }
+        l[i] += sum[0] + sum[1];
+        if (NB > 2) __builtin_amdgcn_sched_barrier(0);
+    }
+    float f[8];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        f[4 * w] = scale_of<0>(x.vs[w]);
+        f[4 * w + 1] = scale_of<1>(x.vs[w]);
+        f[4 * w + 2] = scale_of<2>(x.vs[w]);
+        f[4 * w + 3] = scale_of<3>(x.vs[w]);
+    }
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        u32x4 even, odd;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const uint32_t c = x.v[d][w];
+            uint32_t t[4];
+            if constexpr (HALF) {
+                t[0] = pair_f16<0>(c, f[4 * w]), t[1] = pair_f16<1>(c, f[4 * w + 1]);
+                t[2] = pair_f16<2>(c, f[4 * w + 2]), t[3] = pair_f16<3>(c, f[4 * w + 3]);
+            } else {
+                t[0] = pair_bf16<0>(c, f[4 * w]), t[1] = pair_bf16<1>(c, f[4 * w + 1]);
+                t[2] = pair_bf16<2>(c, f[4 * w + 2]), t[3] = pair_bf16<3>(c, f[4 * w + 3]);
+            }
+            even[2 * w] = __builtin_amdgcn_perm(t[1], t[0], 0x05040100);
+            odd[2 * w] = __builtin_amdgcn_perm(t[1], t[0], 0x07060302);
+            even[2 * w + 1] = __builtin_amdgcn_perm(t[3], t[2], 0x05040100);
+            odd[2 * w + 1] = __builtin_amdgcn_perm(t[3], t[2], 0x07060302);
+        }
+#pragma unroll
+        for (int e = 0; e < kParts; ++e)
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                f32x4 &lo = o[I0 + k][2 * d], &hi = o[I0 + k][2 * d + 1];
+                lo = HALF ? mfma_f16(even, p[k][e], lo) : mfma_bf16(even, p[k][e], lo);
+                hi = HALF ? mfma_f16(odd, p[k][e], hi) : mfma_bf16(odd, p[k][e], hi);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Any half: of any scales, with tokens that some row does not see (row0, group: of the wave's rows, where several
+// tokens of a request are causal among themselves, first_sees < left), or with scores past a reference point.
+template <int DT, int NB>
+__device__ __forceinline__ void any_half(f32x4 (&o)[NB][8], float (&m)[NB], float (&l)[NB], uint32_t &bad, const CK_LDS char *q,
+                                         const CK_LDS char *slot, int h, float scale_log2, int lane, int left, int first_sees,
+                                         int row0, int group) {
+    Half x;
+    read_half(x, slot, h, lane);
+    f32x4 sc[NB][2];
+    half_scores<false, DT, NB>(sc, x, q);
+    if (first_sees < 32) {
+        const int y = lane_again(lane), g = y >> 4;
+        int sees[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            sees[i] = first_sees < left ? min(first_sees + (row0 + 16 * i + (y & 15)) / group, left) : left;
+            const int n = sees[i] - 8 * g;  // token of sc[i][t][r]: 8 g + 4 t + r
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e >= n) sc[i][e >> 2][e & 3] = -INFINITY;
+        }
+        hide_values<NB>(bad, x.vs[0], x.vs[1], sees, left, g);
+    }
+    float most[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) most[i] = largest(sc[i]) * scale_log2;
+    move_points<NB>(o, m, l, most);
+    static_for<NB>([&](auto i) __attribute__((always_inline)) {
+        // a row block at a time, and nothing kept from one for the next: there are no registers for more
+        asm volatile("" : "+v"(x.vs[0]), "+v"(x.vs[1]));
+#pragma unroll
+        for (int d = 0; d < 4; ++d) asm volatile("" : "+v"(x.v[d][0]), "+v"(x.v[d][1]));
+        half_values<false, int(i), 1, NB>(o, l, m, x, sc, scale_log2);
+    });
+}
+
+template <int DT, int NB>
+__global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(DecodeArgs) {
+    using E = Elem<DT>;
+    constexpr int kTileRows = 16 * NB;
+    const KernArgs args = (KernArgs)__builtin_amdgcn_kernarg_segment_ptr();
+    KernArgs a = args_again(args);
+    extern __shared__ __attribute__((aligned(16))) char wide_raw[];
+    CK_LDS char *smem = (CK_LDS char *)wide_raw;
+    int *starts = reinterpret_cast<int *>(wide_raw + kWideStarts), *len0 = starts + kWideThreads;
+    const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
+    const int total = scalar(list_starts<kWideThreads>(a, starts, len0, len0 + kWideThreads, tid));
+    const int block = scalar((int)xcd_remap(blockIdx.x, gridDim.x));
+    const int share = scalar(block / a->tiles), tile = block - share * a->tiles;
+    const Cut cut = list_cut(total * a->kv_heads, a->waves);
+    if (share >= cut.chunks) return;
+    int cur = scalar(cut_lo(cut, share));
+    const int hi = scalar(cut_lo(cut, share + 1));
+    const int row0 = kTileRows * tile;
+    CK_LDS char *buffer = smem + wave * 2 * kUnitBytes;
+
+    f32x4 o[NB][8];
+    float m[NB], l[NB];
+    uint32_t bad;
+    while (cur < hi) {
+        a = args_again(args);
+        const Found f = find_request_of_wave<kWideThreads>(a, starts, len0, cur, lane);
+        const int b = scalar(f.b), len = scalar(f.len), each = units_of(len), in = cur - scalar(f.at);
+        const int h = scalar(in / each), i0 = in - h * each, i1 = min(each, i0 + hi - cur);
+        const int item = b * a->kv_heads + h;
+        const bool before = i0 > 0, after = i1 < each, causal = a->causal;
+        const int q_len = a->q_len, group = a->group;
+        const float scale_log2 = a->scale_log2;
+        cur += i1 - i0;
+        // the query's operands, some of each wave
+        {
+            const int x = lane_again(lane), n16 = x & 15, g = x >> 4;
+#pragma unroll
+            for (int e = 0; e < NB * 4 / kWideWaves; ++e) {
+                const int piece = e * kWideWaves + wave, c = piece & 3;  // (i, c)
+                const int r = kTileRows * tile + 16 * (piece >> 2) + n16, t = r / a->group;
+                u32x4 y = {0, 0, 0, 0};
+                if (r < a->rows)
+                    y = *reinterpret_cast<const u32x4 *>(
+                        a->q + (((int64_t)b * q_len + t) * a->heads + h * a->group + (r - t * a->group)) * kD + 32 * g + 8 * c);
+                *reinterpret_cast<CK_LDS u32x4 *>(smem + kWideQ + piece * 1024 + 16 * x) = y;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+        }
+        bad = 0;
+        bool fresh = true;  // nothing has been added to O
+        const CK_LDS char *q = smem + kWideQ + 16 * lane;
+        __syncthreads();
+        for (int c0 = i0 + wave; c0 < i1; c0 += 64 * kWideWaves) {
+            // this wave's units: c0 + 8 k, lane k has the address
+            const int n = min(64, (i1 - c0 + kWideWaves - 1) / kWideWaves);
+            const uint64_t d_at = unit_address(a, b, h, c0 + kWideWaves * min(lane, n - 1));
+            auto slot_of = [&](int k) { return buffer + (k & 1) * kUnitBytes; };
+            move_unit(of_lane(d_at, 0), slot_of(0), lane_again(lane));
+            int k = 0, half = 0;
+            // The first loop takes what it can, halves seen whole by all rows, of fp16's scales and with no score past a
+            // reference point; nothing else changes O in it, or the compiler would hold O twice and copy it.
+            for (;;) {
+                int left, first_sees;
+                const CK_LDS char *slot;
+#pragma unroll 1
+                for (;;) {
+                    if (half == 0) {
+                        if (k + 1 < n) {
+                            move_unit(of_lane(d_at, k + 1), slot_of(k + 1), lane_again(lane));
+                            wait_vmcnt<kPieces>();
+                        } else {
+                            wait_vmcnt<0>();
+                        }
+                        asm volatile("" ::: "memory");
+                    }
+                    slot = slot_of(k);
+                    left = len - (c0 + kWideWaves * k) * kUnit - 32 * half;
+                    first_sees = causal ? left - q_len + 1 : left;
+                    if (__builtin_expect(first_sees < 32, 0)) break;
+                    Half x;
+                    read_half(x, slot, half, lane);
+                    uint32_t past = past_half(x.vs[0]) | past_half(x.vs[1]);
+                    if constexpr (DT == CK_DTYPE_F16) past |= past_half(x.ks | (kMidScales & 0xffff0000));
+                    f32x4 sc[NB][2];
+                    half_scores<DT == CK_DTYPE_F16, DT, NB>(sc, x, q);
+                    if (__builtin_expect(__builtin_amdgcn_ballot_w64(past != 0) != 0, 0)) break;
+                    bool moves = false;
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) moves |= largest(sc[i]) * scale_log2 > m[i] + kSlack;
+                    if (__builtin_expect(__builtin_amdgcn_ballot_w64(moves) != 0, 0)) {
+                        if (!fresh) break;
+#pragma unroll
+                        for (int i = 0; i < NB; ++i)  // nothing to scale yet
+                            m[i] = over_groups(largest(sc[i]), [](float x, float y) { return fmaxf(x, y); }) * scale_log2;
+                    }
+                    fresh = false;
+                    half_values<true, 0, NB, NB>(o, l, m, x, sc, scale_log2);
+                    half ^= 1;
+                    if (half == 0 && ++k == n) break;
+                }
+                if (k == n) break;
+                fresh = false;
+                any_half<DT, NB>(o, m, l, bad, q, slot, half, scale_log2, lane, left, first_sees, row0, group);
+                half ^= 1;
+                if (half == 0 && ++k == n) break;
+            }
+        }
+
+        add_bad<NB>(o, bad);
+
+        // ---- the waves' parts, joined: of each pair the second's, through LDS, into the first's ----------------
+        __syncthreads();
+#pragma unroll 1
+        for (int step = kWideWaves / 2; step > 0; step >>= 1) {
+            CK_LDS char *p = smem + (wave & (step - 1)) * kWidePart + 16 * lane_again(lane);
+            if (wave >= step && wave < 2 * step) {
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) *reinterpret_cast<CK_LDS f32x4 *>(p + (8 * i + k) * 1024) = o[i][k];
+                    *reinterpret_cast<CK_LDS f32x2 *>(p + 32 * 1024 + 8 * (i & 1) + 1024 * (i >> 1)) = f32x2{m[i], l[i]};
+                }
+            }
+            __syncthreads();
+            if (wave < step) {
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    const f32x2 ml = *reinterpret_cast<const CK_LDS f32x2 *>(p + 32 * 1024 + 8 * (i & 1) + 1024 * (i >> 1));
+                    const float top = fmaxf(m[i], ml[0]);
+                    const float f0 = m[i] == -INFINITY ? 0.f : exp2_fast(m[i] - top);
+                    const float f1 = ml[0] == -INFINITY ? 0.f : exp2_fast(ml[0] - top);
+                    l[i] = l[i] * f0 + ml[1] * f1;
+                    m[i] = top;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const f32x4 y = *reinterpret_cast<const CK_LDS f32x4 *>(p + (8 * i + k) * 1024);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[i][k][r] = fmaf(o[i][k][r], f0, y[r] * f1);
+                        if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (wave > 0) continue;
+        a = args_again(args);
+        const bool whole = !before && !after && !a->merge;
+        const int slot_rows = min(kTileRows, a->rows);
+        const int64_t slot = part_slot(before, after, share, a->waves, item) * a->tiles + tile;
+        const int x = lane_again(lane), n16 = x & 15, g = x >> 4;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int at = 16 * i + n16, r = kTileRows * tile + at;
+            const float sum = over_groups(l[i], [](float x, float y) { return x + y; }), ref = m[i] - Form<DT, NB>::kBias;
+            if (r >= a->rows) continue;
+            if (whole) {
+                const int t = r / a->group;
+                const int64_t row = ((int64_t)b * q_len + t) * a->heads + h * a->group + (r - t * a->group);
+                const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    u32x4 y;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = E::pack2(o[i][2 * e][d] * inv, o[i][2 * e + 1][d] * inv);
+                    *reinterpret_cast<u32x4 *>(a->out + row * kD + 32 * g + 8 * d) = y;
+                }
+                if (g == 0) a->lse[row] = sum == 0.f ? -INFINITY : (ref + __log2f(sum)) * kLn2;
+            } else {
+                float *to = a->part_o + slot * slot_rows * kD + (at * 4 + g) * 4;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    *reinterpret_cast<f32x4 *>(to + j * slot_rows * 16) =
+                        f32x4{o[i][4 * (j & 1)][j >> 1], o[i][4 * (j & 1) + 1][j >> 1], o[i][4 * (j & 1) + 2][j >> 1],
+                              o[i][4 * (j & 1) + 3][j >> 1]};
+                if (g == 0) a->part_ml[slot * slot_rows + at] = make_float2(ref, sum);
+            }
+        }
+    }
 }
 
 // ---- the fold of cut items, and of a prefix with its suffixes ---------------------------------------------
@@ -568,22 +1172,29 @@ int64_t pad256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 // One list over the waves (a call's requests, or its prefix) and its part of the workspace.
 struct Side {
-    int64_t rows, blocks, tiles, groups, waves, slot_rows, slots;
+    int64_t rows, blocks, tile_rows, tiles, groups, waves, slot_rows, slots;
+    bool wide;  // the form for many rows
     int64_t off_sums, off_ml, off_o, end;
 };
 
 int plan_side(int64_t batch, int64_t rows, int64_t kv_heads, int64_t kv_cap, bool merge, int64_t at, Side *p) {
     p->rows = rows;
-    p->blocks = rows <= 16 ? 1 : 2;
-    p->tiles = ceil_div(rows, 16 * p->blocks);
-    p->groups = kGroups;
-    if (p->groups * kWaves < p->tiles) p->groups = ceil_div(p->tiles, kWaves);
+    p->wide = rows > 32;
+    p->blocks = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    p->tile_rows = 16 * p->blocks;
+    p->tiles = ceil_div(rows, p->tile_rows);
+    if (p->wide) {  // shares of workgroups
+        p->waves = p->tiles < kGroupsWide ? kGroupsWide / p->tiles : 1;
+        p->groups = p->waves * p->tiles;
+    } else {
+        p->groups = kGroups;
+        p->waves = p->groups * kWaves;
+    }
     if (!grid_fits(p->groups, kThreads)) return CK_E_INVALID_ARG;
-    p->waves = p->groups * kWaves / p->tiles;
     // the list's places are 32-bit, and its shares' numbers
     if (batch * kv_heads >= (int64_t)1 << 31 || batch * kv_heads * ceil_div(kv_cap, kUnit) >= (int64_t)1 << 31)
         return CK_E_INVALID_ARG;
-    p->slot_rows = rows < 16 * p->blocks ? rows : 16 * p->blocks;
+    p->slot_rows = rows < p->tile_rows ? rows : p->tile_rows;
     p->slots = (2 * p->waves + (merge ? batch * kv_heads : 0)) * p->tiles;
     p->off_sums = at;
     p->off_ml = p->off_sums + pad256((batch + 1) * 4);
@@ -616,9 +1227,19 @@ int make_plan(int64_t batch, int64_t q_len, int64_t heads, int64_t kv_heads, int
     return CK_OK;
 }
 
+template <int DT, int NB>
+int launch_wide(const DecodeArgs &a, dim3 grid, hipStream_t s) {
+    static std::atomic<uint64_t> lds_set{0};
+    const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(&kv4_wide_kernel<DT, NB>), kWideLds, lds_set);
+    if (rc != CK_OK) return rc;
+    hipLaunchKernelGGL((kv4_wide_kernel<DT, NB>), grid, dim3(kWideThreads), kWideLds, s, a);
+    CK_RETURN_LAUNCH();
+}
+
 template <int DT>
 int launch_side(const DecodeArgs &a, const Side &p, hipStream_t s) {
     const dim3 grid((unsigned)p.groups), block(kThreads);
+    if (p.wide) return launch_wide<DT, 4>(a, grid, s);
     if (p.blocks == 1) hipLaunchKernelGGL((kv4_decode_kernel<DT, 1>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((kv4_decode_kernel<DT, 2>), grid, block, 0, s, a);
     CK_RETURN_LAUNCH();
@@ -660,11 +1281,12 @@ void fill(DecodeArgs *a, FoldSide *f, const Pool &pool, const Side &p, int64_t b
     a->batch = (int)batch;
     a->rows = (int)p.rows;
     a->tiles = (int)p.tiles;
+    a->tile_rows = (int)p.tile_rows;
     a->waves = (int)p.waves;
     a->part_o = reinterpret_cast<float *>(ws + p.off_o);
     a->part_ml = reinterpret_cast<float2 *>(ws + p.off_ml);
     a->sums = reinterpret_cast<int32_t *>(ws + p.off_sums);
-    *f = FoldSide{a->part_o, a->part_ml, a->sums, a->batch, a->waves, a->tiles, (int)(16 * p.blocks), (int)p.slot_rows};
+    *f = FoldSide{a->part_o, a->part_ml, a->sums, a->batch, a->waves, a->tiles, a->tile_rows, (int)p.slot_rows};
 }
 
 int run(const void *q, const Pool &pool, const Pool *prefix, int64_t batch, int64_t q_len, int64_t heads,
