@@ -861,7 +861,8 @@ __device__ __forceinline__ void any_half(f32x4 (&o)[NB][8], float (&m)[NB], floa
 template <int DT, int NB>
 __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(DecodeArgs) {
     using E = Elem<DT>;
-    constexpr int kTileRows = 16 * NB;
+    constexpr int kTileRows = 16 * NB, kParts = kWideWaves / 2;
+    static_assert(NB == 4, "a wave joins half of a row block's dims");
     const KernArgs args = (KernArgs)__builtin_amdgcn_kernarg_segment_ptr();
     KernArgs a = args_again(args);
     extern __shared__ __attribute__((aligned(16))) char wide_raw[];
@@ -891,20 +892,6 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(DecodeArgs) {
         const int q_len = a->q_len, group = a->group;
         const float scale_log2 = a->scale_log2;
         cur += i1 - i0;
-        // the query's operands, some of each wave
-        {
-            const int x = lane_again(lane), n16 = x & 15, g = x >> 4;
-#pragma unroll
-            for (int e = 0; e < NB * 4 / kWideWaves; ++e) {
-                const int piece = e * kWideWaves + wave, c = piece & 3;  // (i, c)
-                const int r = kTileRows * tile + 16 * (piece >> 2) + n16, t = r / a->group;
-                u32x4 y = {0, 0, 0, 0};
-                if (r < a->rows)
-                    y = *reinterpret_cast<const u32x4 *>(
-                        a->q + (((int64_t)b * q_len + t) * a->heads + h * a->group + (r - t * a->group)) * kD + 32 * g + 8 * c);
-                *reinterpret_cast<CK_LDS u32x4 *>(smem + kWideQ + piece * 1024 + 16 * x) = y;
-            }
-        }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
 #pragma unroll
@@ -914,14 +901,37 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(DecodeArgs) {
         }
         bad = 0;
         bool fresh = true;  // nothing has been added to O
+        // The first unit, and the query's operands, some of each wave. Units of this wave: c0 + 8 k, lane k has the
+        // address.
+        const int w0 = i0 + wave;
+        uint64_t d_at = 0;
+        if (w0 < i1) d_at = unit_address(a, b, h, min(w0 + kWideWaves * lane, i1 - 1));
+        {
+            const int x = lane_again(lane), n16 = x & 15, g = x >> 4;
+            u32x4 y[NB * 4 / kWideWaves];
+#pragma unroll
+            for (int e = 0; e < NB * 4 / kWideWaves; ++e) {
+                const int piece = e * kWideWaves + wave, c = piece & 3;  // (i, c)
+                const int r = kTileRows * tile + 16 * (piece >> 2) + n16, t = r / a->group;
+                y[e] = u32x4{0, 0, 0, 0};
+                if (r < a->rows)
+                    y[e] = *reinterpret_cast<const u32x4 *>(
+                        a->q + (((int64_t)b * q_len + t) * a->heads + h * a->group + (r - t * a->group)) * kD + 32 * g + 8 * c);
+            }
+            if (w0 < i1) move_unit(of_lane(d_at, 0), buffer, lane_again(lane));
+#pragma unroll
+            for (int e = 0; e < NB * 4 / kWideWaves; ++e)
+                *reinterpret_cast<CK_LDS u32x4 *>(smem + kWideQ + (e * kWideWaves + wave) * 1024 + 16 * x) = y[e];
+        }
         const CK_LDS char *q = smem + kWideQ + 16 * lane;
         __syncthreads();
-        for (int c0 = i0 + wave; c0 < i1; c0 += 64 * kWideWaves) {
-            // this wave's units: c0 + 8 k, lane k has the address
+        for (int c0 = w0; c0 < i1; c0 += 64 * kWideWaves) {
             const int n = min(64, (i1 - c0 + kWideWaves - 1) / kWideWaves);
-            const uint64_t d_at = unit_address(a, b, h, c0 + kWideWaves * min(lane, n - 1));
             auto slot_of = [&](int k) { return buffer + (k & 1) * kUnitBytes; };
-            move_unit(of_lane(d_at, 0), slot_of(0), lane_again(lane));
+            if (c0 != w0) {
+                d_at = unit_address(a, b, h, min(c0 + kWideWaves * lane, i1 - 1));
+                move_unit(of_lane(d_at, 0), slot_of(0), lane_again(lane));
+            }
             int k = 0, half = 0;
             // The first loop takes what it can, halves seen whole by all rows, of fp16's scales and with no score past a
             // reference point; nothing else changes O in it, or the compiler would hold O twice and copy it.
@@ -974,73 +984,90 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(DecodeArgs) {
 
         add_bad<NB>(o, bad);
 
-        // ---- the waves' parts, joined: of each pair the second's, through LDS, into the first's ----------------
+        // ---- the waves' parts, joined: waves 4 to 7's into those of 0 to 3; then a wave takes half the dims of a row block
         __syncthreads();
-#pragma unroll 1
-        for (int step = kWideWaves / 2; step > 0; step >>= 1) {
-            CK_LDS char *p = smem + (wave & (step - 1)) * kWidePart + 16 * lane_again(lane);
-            if (wave >= step && wave < 2 * step) {
+        CK_LDS char *part = smem + (wave & (kParts - 1)) * kWidePart + 16 * lane_again(lane);
+        auto ml_at = [](int i) { return 4 * 8 * 1024 + 1024 * (i >> 1) + 8 * (i & 1); };
+        auto leave = [&]() __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i < NB; ++i) {
+            for (int i = 0; i < NB; ++i) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) *reinterpret_cast<CK_LDS f32x4 *>(p + (8 * i + k) * 1024) = o[i][k];
-                    *reinterpret_cast<CK_LDS f32x2 *>(p + 32 * 1024 + 8 * (i & 1) + 1024 * (i >> 1)) = f32x2{m[i], l[i]};
+                for (int k = 0; k < 8; ++k) *reinterpret_cast<CK_LDS f32x4 *>(part + (8 * i + k) * 1024) = o[i][k];
+                *reinterpret_cast<CK_LDS f32x2 *>(part + ml_at(i)) = f32x2{m[i], l[i]};
+            }
+        };
+        if (wave >= kParts) leave();
+        __syncthreads();
+        if (wave < kParts) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const f32x2 ml = *reinterpret_cast<const CK_LDS f32x2 *>(part + ml_at(i));
+                const float top = fmaxf(m[i], ml[0]);
+                const float f0 = m[i] == -INFINITY ? 0.f : exp2_fast(m[i] - top);
+                const float f1 = ml[0] == -INFINITY ? 0.f : exp2_fast(ml[0] - top);
+                l[i] = l[i] * f0 + ml[1] * f1;
+                m[i] = top;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const f32x4 y = *reinterpret_cast<const CK_LDS f32x4 *>(part + (8 * i + k) * 1024);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[i][k][r] = fmaf(o[i][k][r], f0, y[r] * f1);
+                    if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            __syncthreads();
-            if (wave < step) {
-#pragma unroll
-                for (int i = 0; i < NB; ++i) {
-                    const f32x2 ml = *reinterpret_cast<const CK_LDS f32x2 *>(p + 32 * 1024 + 8 * (i & 1) + 1024 * (i >> 1));
-                    const float top = fmaxf(m[i], ml[0]);
-                    const float f0 = m[i] == -INFINITY ? 0.f : exp2_fast(m[i] - top);
-                    const float f1 = ml[0] == -INFINITY ? 0.f : exp2_fast(ml[0] - top);
-                    l[i] = l[i] * f0 + ml[1] * f1;
-                    m[i] = top;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const f32x4 y = *reinterpret_cast<const CK_LDS f32x4 *>(p + (8 * i + k) * 1024);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) o[i][k][r] = fmaf(o[i][k][r], f0, y[r] * f1);
-                        if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
-            }
-            __syncthreads();
+            leave();
         }
-        if (wave > 0) continue;
-        a = args_again(args);
-        const bool whole = !before && !after && !a->merge;
-        const int slot_rows = min(kTileRows, a->rows);
-        const int64_t slot = part_slot(before, after, share, a->waves, item) * a->tiles + tile;
-        const int x = lane_again(lane), n16 = x & 15, g = x >> 4;
+        __syncthreads();
+        {
+            a = args_again(args);
+            const int x = lane_again(lane), n16 = x & 15, g = x >> 4, i = wave >> 1, k0 = 4 * (wave & 1);
+            const CK_LDS char *p = smem + 16 * x;
+            float top = -INFINITY, sum = 0.f;
+            f32x2 ml[kParts];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
+            for (int w = 0; w < kParts; ++w) {
+                ml[w] = *reinterpret_cast<const CK_LDS f32x2 *>(p + w * kWidePart + ml_at(i));
+                top = fmaxf(top, ml[w][0]);
+            }
+            f32x4 y[4];
+#pragma unroll
+            for (int w = 0; w < kParts; ++w) {
+                const float f = ml[w][0] == -INFINITY ? 0.f : exp2_fast(ml[w][0] - top);
+                sum = fmaf(ml[w][1], f, sum);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const f32x4 z = *reinterpret_cast<const CK_LDS f32x4 *>(p + w * kWidePart + (8 * i + k0 + k) * 1024);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[k][r] = w ? fmaf(z[r], f, y[k][r]) : z[r] * f;
+                }
+            }
+            sum = over_groups(sum, [](float x, float y) { return x + y; });
+            const float ref = top - Form<DT, NB>::kBias;
+            const bool whole = !before && !after && !a->merge;
             const int at = 16 * i + n16, r = kTileRows * tile + at;
-            const float sum = over_groups(l[i], [](float x, float y) { return x + y; }), ref = m[i] - Form<DT, NB>::kBias;
-            if (r >= a->rows) continue;
-            if (whole) {
-                const int t = r / a->group;
-                const int64_t row = ((int64_t)b * q_len + t) * a->heads + h * a->group + (r - t * a->group);
-                const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+            if (r < a->rows) {
+                // dims 32 g + 8 d + k0 .. + 3
+                if (whole) {
+                    const int t = r / a->group;
+                    const int64_t row = ((int64_t)b * q_len + t) * a->heads + h * a->group + (r - t * a->group);
+                    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    u32x4 y;
+                    for (int d = 0; d < 4; ++d)
+                        *reinterpret_cast<uint2 *>(a->out + row * kD + 32 * g + 8 * d + k0) =
+                            make_uint2(E::pack2(y[0][d] * inv, y[1][d] * inv), E::pack2(y[2][d] * inv, y[3][d] * inv));
+                    if (g == 0 && k0 == 0) a->lse[row] = sum == 0.f ? -INFINITY : (ref + __log2f(sum)) * kLn2;
+                } else {
+                    const int slot_rows = min(kTileRows, a->rows);
+                    const int64_t slot = part_slot(before, after, share, a->waves, item) * a->tiles + tile;
+                    float *to = a->part_o + slot * slot_rows * kD + (at * 4 + g) * 4;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] = E::pack2(o[i][2 * e][d] * inv, o[i][2 * e + 1][d] * inv);
-                    *reinterpret_cast<u32x4 *>(a->out + row * kD + 32 * g + 8 * d) = y;
+                    for (int d = 0; d < 4; ++d)
+                        *reinterpret_cast<f32x4 *>(to + (2 * d + (wave & 1)) * slot_rows * 16) = f32x4{y[0][d], y[1][d], y[2][d], y[3][d]};
+                    if (g == 0 && k0 == 0) a->part_ml[slot * slot_rows + at] = make_float2(ref, sum);
                 }
-                if (g == 0) a->lse[row] = sum == 0.f ? -INFINITY : (ref + __log2f(sum)) * kLn2;
-            } else {
-                float *to = a->part_o + slot * slot_rows * kD + (at * 4 + g) * 4;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    *reinterpret_cast<f32x4 *>(to + j * slot_rows * 16) =
-                        f32x4{o[i][4 * (j & 1)][j >> 1], o[i][4 * (j & 1) + 1][j >> 1], o[i][4 * (j & 1) + 2][j >> 1],
-                              o[i][4 * (j & 1) + 3][j >> 1]};
-                if (g == 0) a->part_ml[slot * slot_rows + at] = make_float2(ref, sum);
             }
         }
+        if (cur < hi) __syncthreads();
     }
 }
 
