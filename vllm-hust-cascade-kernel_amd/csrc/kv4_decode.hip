@@ -25,6 +25,7 @@
 // * Rows past 16 NB are row tiles of their own, given to neighbouring waves, which read the same units.
 // * Shared prefix: the batch is one request's rows over the prefix; then the suffixes; one fold for both.
 #include <cmath>
+#include <type_traits>
 
 #include "kv4_common.h"
 #include "kv4_map.h"
@@ -155,6 +156,33 @@ __device__ __forceinline__ Found find_request_of_wave(KernArgs a, const int *sta
     const int more = __popcll(__builtin_amdgcn_ballot_w64(lane < kEach && starts[kEach * some + lane % kEach] * a->kv_heads <= u)) - 1;
     return find_from<T>(a, starts, len0, u, scalar(kEach * some + more));
 }
+// The list of a call's units for a workgroup of T threads; SINGLE: of one request (a prefix), which needs no table.
+template <int T, bool SINGLE>
+struct List {
+    const int *starts, *len0;
+    int total;  // units of one kv head
+    int len;    // of the one request
+    // All threads come here (a barrier).
+    __device__ __forceinline__ List(KernArgs a, int *starts_at, int *len0_at, int *scan, int tid) : starts(starts_at), len0(len0_at) {
+        if constexpr (SINGLE) {
+            len = scalar(len_of(a, 0));
+            total = units_of(len);
+            if (blockIdx.x == 0 && tid < 2) a->sums[tid] = tid * total;
+        } else {
+            len = 0;
+            total = scalar(list_starts<T>(a, starts_at, len0_at, scan, tid));
+        }
+    }
+    __device__ __forceinline__ List(const int *starts_at, const int *len0_at, int units) : starts(starts_at), len0(len0_at), total(units), len(0) {}
+    __device__ __forceinline__ Found find(KernArgs a, int u) const {  // u a lane
+        if constexpr (SINGLE) return Found{0, 0, len};
+        else return find_request<T>(a, starts, len0, u);
+    }
+    __device__ __forceinline__ Found find_of_wave(KernArgs a, int u, int lane) const {
+        if constexpr (SINGLE) return Found{0, 0, len};
+        else return find_request_of_wave<T>(a, starts, len0, u, lane);
+    }
+};
 // A unit's place in memory; bit 0 (addresses are 16-byte aligned) marks a page outside the pool.
 __device__ __forceinline__ uint64_t unit_address(KernArgs a, int b, int h, int i) {
     const int page = a->bt[(int64_t)b * a->bt_cols + (i >> 1)];
@@ -525,21 +553,13 @@ __device__ __forceinline__ void compute(Rows<DT, NB> &s, const U &u, float scale
         add_values<false, 0, NB>(s, v, again(vs), sc, scale_log2);
 }
 
-template <int DT, int NB>
-__global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(DecodeArgs) {
-    const KernArgs args = (KernArgs)__builtin_amdgcn_kernarg_segment_ptr();
+// What a wave makes of its share w of the list; more than one row block: through its ring of two units in LDS.
+template <int DT, int NB, class L>
+__device__ __forceinline__ void decode_share(const KernArgs args, const L &list, CK_LDS char *ring, int w, int lane) {
     KernArgs a = args_again(args);
-    __shared__ int starts[kThreads], len0[kThreads], scan[kWaves];
-    __shared__ __attribute__((aligned(16))) char ring[NB > 1 ? kWaves * 2 * kUnitBytes : 16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
     constexpr int kRows = 16 * NB;
     constexpr bool kQAhead = NB == 1;  // the next item's queries are loaded ahead
-
-    const int total = scalar(list_starts<kThreads>(a, starts, len0, scan, tid));
-
-    // ---- this wave's share ---------------------------------------------------------------------------
-    // neighbouring shares on different CUs, so that few units spread over all of them
-    const int w = scalar(wave * (int)gridDim.x + (int)blockIdx.x);
+    const int total = list.total;
     const Cut cut = list_cut(total * a->kv_heads, a->waves);
     if (w >= cut.chunks) return;
     const int lo = scalar(cut_lo(cut, w)), hi = scalar(cut_lo(cut, w + 1));
@@ -628,7 +648,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(DecodeArgs) {
         uint64_t d_at = 0;
         if (lane < n) {
             const int u = base + lane;
-            const Found f = find_request<kThreads>(a, starts, len0, u);
+            const Found f = list.find(a, u);
             const int each = units_of(f.len), h = (u - f.at) / each, i = u - f.at - h * each;
             d_item = f.b * a->kv_heads + h;
             d_first = i * kUnit;
@@ -637,10 +657,9 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(DecodeArgs) {
         }
         // One row block: the next unit in registers; more: in the wave's other half of its ring.
         Unit next;
-        CK_LDS char *slots = (CK_LDS char *)ring + (NB > 1 ? wave * 2 * kUnitBytes : 0);
         auto fetch = [&](int j) {
             const uint64_t at = of_lane(d_at, j);
-            if constexpr (NB > 1) move_unit(at, slots + (j & 1) * kUnitBytes, lane_again(lane));
+            if constexpr (NB > 1) move_unit(at, ring + (j & 1) * kUnitBytes, lane_again(lane));
             else load_unit(next, at, lane);
         };
         fetch(0);
@@ -669,13 +688,37 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(DecodeArgs) {
                 if (j + 1 < n) wait_vmcnt<kPieces>();
                 else wait_vmcnt<0>();
                 asm volatile("" ::: "memory");
-                compute<DT, NB>(s, unit_in(slots + (j & 1) * kUnitBytes, lane), a->scale_log2, lane, first_sees < kUnit, sees, left);
+                compute<DT, NB>(s, unit_in(ring + (j & 1) * kUnitBytes, lane), a->scale_log2, lane, first_sees < kUnit, sees, left);
             } else {
                 compute<DT, NB>(s, in_registers, a->scale_log2, lane, first_sees < kUnit, sees, left);
             }
         }
     }
     close_item(item, before, goes_on);
+}
+
+// The arguments of a call's lists lie one behind the other: the suffixes', or a prefix's (a request of NB row
+// blocks) and then the suffixes' (of one), whose shares a wave takes one after the other.
+struct PairArgs {
+    DecodeArgs prefix, own;
+};
+template <int DT, int NB, bool PAIR>
+__global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(std::conditional_t<PAIR, PairArgs, DecodeArgs>) {
+    const KernArgs args = (KernArgs)__builtin_amdgcn_kernarg_segment_ptr();
+    __shared__ int starts[kThreads], len0[kThreads], scan[kWaves];
+    __shared__ __attribute__((aligned(16))) char ring[NB > 1 ? kWaves * 2 * kUnitBytes : 16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
+    // neighbouring shares on different CUs, so that few units spread over all of them
+    const int w = scalar(wave * (int)gridDim.x + (int)blockIdx.x);
+    CK_LDS char *mine = (CK_LDS char *)ring + (NB > 1 ? wave * 2 * kUnitBytes : 0);
+    const List<kThreads, PAIR> list(args, starts, len0, scan, tid);
+    if constexpr (PAIR) {
+        const List<kThreads, false> own(args + 1, starts, len0, scan, tid);
+        decode_share<DT, NB>(args, list, mine, w, lane);
+        decode_share<DT, 1>(args + 1, own, mine, w, lane);
+    } else {
+        decode_share<DT, NB>(args, list, mine, w, lane);
+    }
 }
 
 // ---- many rows ---------------------------------------------------------------------------------------------
@@ -858,24 +901,24 @@ __device__ __forceinline__ void any_half(f32x4 (&o)[NB][8], float (&m)[NB], floa
     });
 }
 
-template <int DT, int NB>
-__global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(DecodeArgs) {
+template <int DT, bool PAIR>
+__global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditional_t<PAIR, PairArgs, DecodeArgs>) {
     using E = Elem<DT>;
-    constexpr int kTileRows = 16 * NB, kParts = kWideWaves / 2;
-    static_assert(NB == 4, "a wave joins half of a row block's dims");
+    constexpr int NB = 4, kTileRows = 16 * NB, kParts = kWideWaves / 2;
     const KernArgs args = (KernArgs)__builtin_amdgcn_kernarg_segment_ptr();
     KernArgs a = args_again(args);
     extern __shared__ __attribute__((aligned(16))) char wide_raw[];
     CK_LDS char *smem = (CK_LDS char *)wide_raw;
-    int *starts = reinterpret_cast<int *>(wide_raw + kWideStarts), *len0 = starts + kWideThreads;
+    int *starts = reinterpret_cast<int *>(wide_raw + kWideStarts), *len0 = starts + kWideThreads, *scan = len0 + kWideThreads;
     const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
-    const int total = scalar(list_starts<kWideThreads>(a, starts, len0, len0 + kWideThreads, tid));
+    const List<kWideThreads, PAIR> list(a, starts, len0, scan, tid);
+    int own_total = 0;
+    if constexpr (PAIR) own_total = List<kWideThreads, false>(args + 1, starts, len0, scan, tid).total;
     const int block = scalar((int)xcd_remap(blockIdx.x, gridDim.x));
     const int share = scalar(block / a->tiles), tile = block - share * a->tiles;
-    const Cut cut = list_cut(total * a->kv_heads, a->waves);
-    if (share >= cut.chunks) return;
-    int cur = scalar(cut_lo(cut, share));
-    const int hi = scalar(cut_lo(cut, share + 1));
+    const Cut cut = list_cut(list.total * a->kv_heads, a->waves);
+    int cur = share < cut.chunks ? scalar(cut_lo(cut, share)) : 0;
+    const int hi = share < cut.chunks ? scalar(cut_lo(cut, share + 1)) : 0;
     const int row0 = kTileRows * tile;
     CK_LDS char *buffer = smem + wave * 2 * kUnitBytes;
 
@@ -884,7 +927,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(DecodeArgs) {
     uint32_t bad;
     while (cur < hi) {
         a = args_again(args);
-        const Found f = find_request_of_wave<kWideThreads>(a, starts, len0, cur, lane);
+        const Found f = list.find_of_wave(a, cur, lane);
         const int b = scalar(f.b), len = scalar(f.len), each = units_of(len), in = cur - scalar(f.at);
         const int h = scalar(in / each), i0 = in - h * each, i1 = min(each, i0 + hi - cur);
         const int item = b * a->kv_heads + h;
@@ -1069,6 +1112,10 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(DecodeArgs) {
         }
         if (cur < hi) __syncthreads();
     }
+    if constexpr (PAIR) {
+        const List<kWideThreads, false> own(starts, len0, own_total);
+        decode_share<DT, 1>(args + 1, own, nullptr, scalar(wave * (int)gridDim.x + (int)blockIdx.x), lane);
+    }
 }
 
 // ---- the fold of cut items, and of a prefix with its suffixes ---------------------------------------------
@@ -1204,7 +1251,8 @@ struct Side {
     int64_t off_sums, off_ml, off_o, end;
 };
 
-int plan_side(int64_t batch, int64_t rows, int64_t kv_heads, int64_t kv_cap, bool merge, int64_t at, Side *p) {
+// waves: the shares of a list whose launch another one sizes, or 0
+int plan_side(int64_t batch, int64_t rows, int64_t kv_heads, int64_t kv_cap, bool merge, int64_t at, int64_t waves, Side *p) {
     p->rows = rows;
     p->wide = rows > 32;
     p->blocks = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
@@ -1215,7 +1263,7 @@ int plan_side(int64_t batch, int64_t rows, int64_t kv_heads, int64_t kv_cap, boo
         p->groups = p->waves * p->tiles;
     } else {
         p->groups = kGroups;
-        p->waves = p->groups * kWaves;
+        p->waves = waves ? waves : p->groups * kWaves;
     }
     if (!grid_fits(p->groups, kThreads)) return CK_E_INVALID_ARG;
     // the list's places are 32-bit, and its shares' numbers
@@ -1232,6 +1280,7 @@ int plan_side(int64_t batch, int64_t rows, int64_t kv_heads, int64_t kv_cap, boo
 
 struct Plan {
     Side own, prefix;
+    bool paired;  // prefix and suffixes in one launch, of as many waves for both
     int64_t ws_bytes;
 };
 
@@ -1243,42 +1292,49 @@ int make_plan(int64_t batch, int64_t q_len, int64_t heads, int64_t kv_heads, int
         !grid_fits(batch * q_len * heads, 256))
         return CK_E_INVALID_ARG;
     const int64_t group = heads / kv_heads;
-    int rc = plan_side(batch, q_len * group, kv_heads, kv_cap, merge, 0, &p->own);
+    int rc;
+    int64_t at = 0, waves = 0;
+    p->paired = false;
+    if (merge && batch > 0) {
+        rc = plan_side(1, batch * group, kv_heads, prefix_cap, true, at, 0, &p->prefix);
+        if (rc != CK_OK) return rc;
+        at = p->prefix.end;
+        p->paired = group <= 16;
+        if (p->paired) waves = p->prefix.groups * (p->prefix.wide ? kWideWaves : kWaves);
+    }
+    rc = plan_side(batch, q_len * group, kv_heads, kv_cap, merge, at, waves, &p->own);
     if (rc != CK_OK) return rc;
     p->ws_bytes = p->own.end;
-    if (merge && batch > 0) {
-        rc = plan_side(1, batch * group, kv_heads, prefix_cap, true, p->own.end, &p->prefix);
-        if (rc != CK_OK) return rc;
-        p->ws_bytes = p->prefix.end;
-    }
     return CK_OK;
 }
 
-template <int DT, int NB>
-int launch_wide(const DecodeArgs &a, dim3 grid, hipStream_t s) {
+template <int DT, bool PAIR, class A>
+int launch_wide(const A &a, dim3 grid, hipStream_t s) {
     static std::atomic<uint64_t> lds_set{0};
-    const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(&kv4_wide_kernel<DT, NB>), kWideLds, lds_set);
+    const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(&kv4_wide_kernel<DT, PAIR>), kWideLds, lds_set);
     if (rc != CK_OK) return rc;
-    hipLaunchKernelGGL((kv4_wide_kernel<DT, NB>), grid, dim3(kWideThreads), kWideLds, s, a);
+    hipLaunchKernelGGL((kv4_wide_kernel<DT, PAIR>), grid, dim3(kWideThreads), kWideLds, s, a);
     CK_RETURN_LAUNCH();
 }
 
-template <int DT>
-int launch_side(const DecodeArgs &a, const Side &p, hipStream_t s) {
+template <int DT, bool PAIR, class A>
+int launch_side(const A &a, const Side &p, hipStream_t s) {
     const dim3 grid((unsigned)p.groups), block(kThreads);
-    if (p.wide) return launch_wide<DT, 4>(a, grid, s);
-    if (p.blocks == 1) hipLaunchKernelGGL((kv4_decode_kernel<DT, 1>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((kv4_decode_kernel<DT, 2>), grid, block, 0, s, a);
+    if (p.wide) return launch_wide<DT, PAIR>(a, grid, s);
+    if (p.blocks == 1) hipLaunchKernelGGL((kv4_decode_kernel<DT, 1, PAIR>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((kv4_decode_kernel<DT, 2, PAIR>), grid, block, 0, s, a);
     CK_RETURN_LAUNCH();
 }
 
 template <int DT>
 int launch(const DecodeArgs &own, const DecodeArgs *prefix, const Plan &p, const FoldArgs &f, hipStream_t s) {
-    if (prefix) {
-        const int rc = launch_side<DT>(*prefix, p.prefix, s);
-        if (rc != CK_OK) return rc;
+    int rc = CK_OK;
+    if (prefix && p.paired) {
+        rc = launch_side<DT, true>(PairArgs{*prefix, own}, p.prefix, s);
+    } else {
+        if (prefix) rc = launch_side<DT, false>(*prefix, p.prefix, s);
+        if (rc == CK_OK) rc = launch_side<DT, false>(own, p.own, s);
     }
-    const int rc = launch_side<DT>(own, p.own, s);
     if (rc != CK_OK) return rc;
     if (f.rows >= kFoldRows)
         hipLaunchKernelGGL((kv4_combine_kernel<DT, 1>), dim3((unsigned)ceil_div(f.rows, 8)), dim3(256), 0, s, f);
