@@ -58,6 +58,45 @@ def test_write_of_neighbouring_slots():
     assert torch.equal(pool, want)
 
 
+def _slots(gen, how, tokens, blocks):
+    """Slots of many tokens: anywhere; a prompt from inside a page on, over scattered pages; prompts of other
+    alignments one after another, padded with -1 and slots past the pool, the last pages among them."""
+    perm = torch.randperm(blocks, generator=gen, device=DEV)
+    j = torch.arange(tokens, device=DEV)
+    if how == "anywhere":
+        return torch.randperm(blocks * 128, generator=gen, device=DEV)[:tokens]
+    if how == "prompt":
+        return perm[(j + 37) // 128] * 128 + (j + 37) % 128
+    parts, at, page = [], 0, 0
+    for n, first in ((517, 0), (3, 127), (1, 5), (700, 8), (64, 64), (9, 3), (tokens, 121)):
+        n = min(n, tokens - at)
+        i = torch.arange(n, device=DEV) + first
+        parts.append(perm[page + i // 128] * 128 + i % 128)
+        at, page = at + n, page + -(-(n + first) // 128)
+    slots = torch.cat(parts)
+    slots[100:103], slots[600], slots[-1] = -1, blocks * 128, -9
+    return slots
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("how", ["anywhere", "prompt", "mixed"])
+@pytest.mark.parametrize("tokens,kv_heads", [(1024, 8), (2049, 4), (2740, 3)])
+def test_write_and_read_of_many_tokens(tokens, kv_heads, how, dtype):
+    """From 8192 rows on, eight neighbouring tokens are moved together."""
+    g = _gen(tokens)
+    blocks = tokens // 128 + 12
+    slots = _slots(g, how, tokens, blocks)
+    pool = torch.randint(0, 256, (blocks, kv_heads, o4.PAGE_BYTES), generator=g, device=DEV, dtype=torch.uint8)
+    kv = _normal(g, tokens, 2 * kv_heads, 136, dtype=dtype)[..., :128]
+    k, v = kv[:, :kv_heads], kv[:, kv_heads:]
+    want = o4.write(pool, k, v, slots)
+    OPS.kv4_cache_write(k, v, slots, pool)
+    assert torch.equal(pool, want)
+    for order in (slots, slots.flip(0).contiguous()):
+        for got, ref in zip(OPS.kv4_cache_read(pool, order, dtype), o4.read(pool, order)):
+            assert torch.equal(got.double().nan_to_num(7), ref.to(torch.float32).to(dtype).double().nan_to_num(7))
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_write_of_special_values(dtype):
     """Each group of one kind: ties, borders of the scale, the type's largest and least numbers, zeros, values

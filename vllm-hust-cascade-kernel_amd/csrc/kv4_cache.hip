@@ -74,6 +74,19 @@ __device__ __forceinline__ uint32_t quantise(u32x4 w, int &e) {
     return c;
 }
 
+// Writes one token's row: kc, vc the lane's codes, ke, ve its group's scales.
+__device__ __forceinline__ void put_token(const WriteArgs &a, int64_t slot, int head, int l16, uint32_t kc, uint32_t vc, int ke, int ve) {
+    const Place p = place_of(slot, head, a.kv_heads, l16);
+    uint8_t *unit = a.cache + p.unit;
+    *reinterpret_cast<uint32_t *>(unit + p.k) = kc;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) unit[p.v + 1024 * q] = (uint8_t)(vc >> (8 * q));
+    if ((l16 & 3) == 0) {
+        unit[p.ks] = (uint8_t)ke;
+        unit[p.vs] = (uint8_t)ve;
+    }
+}
+
 template <int DT>
 __global__ __launch_bounds__(kThreads) void kv4_write_kernel(WriteArgs a) {
     const int l16 = threadIdx.x & 15, head = blockIdx.y;
@@ -85,14 +98,76 @@ __global__ __launch_bounds__(kThreads) void kv4_write_kernel(WriteArgs a) {
     if (slot < 0 || slot >= a.num_slots) return;  // the same for the 16 lanes of a row
     int ke, ve;
     const uint32_t kc = quantise<DT>(kw, ke), vc = quantise<DT>(vw, ve);
-    const Place p = place_of(slot, head, a.kv_heads, l16);
-    uint8_t *unit = a.cache + p.unit;
-    *reinterpret_cast<uint32_t *>(unit + p.k) = kc;
+    put_token(a, slot, head, l16, kc, vc, ke, ve);
+}
+
+// ---- many tokens: 16 lanes take 8, whose bytes lie together where their slots are eight in a row ---------------
+// The eight slots of a group of lanes' tokens, tokens t0 .. + 7 (some may lie outside the call): base is the first
+// token's slot if they are neighbours from a multiple of 8 on, all in the call and in the pool; else -1, and
+// each lane holds the slot of token t0 + its place in 8.
+struct Eight {
+    int64_t t0, base, slot;
+};
+__device__ __forceinline__ Eight eight_slots(const int64_t *slots, int64_t tokens, int64_t num_slots, int64_t group, int l16) {
+    Eight e;
+    // groups begin where the first token's neighbours do: a prompt's tokens then meet the multiples of 8
+    e.t0 = group * 8 - (slots[0] & 7);
+    const int64_t t = e.t0 + (l16 & 7);
+    e.slot = t >= 0 && t < tokens ? slots[t] : -1;
+    const int64_t first = __shfl(e.slot, 0, 8);
+    const bool ok = e.slot >= 0 && e.slot < num_slots && e.slot == first + (l16 & 7) && (first & 7) == 0;
+    const uint64_t all = __builtin_amdgcn_ballot_w64(ok);
+    const int at = threadIdx.x & 48;
+    e.base = ((all >> at) & 0xffff) == 0xffff ? first : -1;
+    return e;
+}
+// Byte q of each of four words.
+template <int Q>
+__device__ __forceinline__ uint32_t bytes_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    const uint32_t x = __builtin_amdgcn_perm(b, a, 0x0c0c0400 + 0x0101 * Q), y = __builtin_amdgcn_perm(d, c, 0x0c0c0400 + 0x0101 * Q);
+    return x | y << 16;
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void kv4_write8_kernel(WriteArgs a) {
+    const int l16 = threadIdx.x & 15, head = blockIdx.y;
+    const Eight e = eight_slots(a.slots, a.tokens, a.num_slots, (int64_t)blockIdx.x * kRowsPerBlock + (threadIdx.x >> 4), l16);
+    if (e.t0 >= a.tokens) return;
+    u32x4 kw[8], vw[8];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) unit[p.v + 1024 * q] = (uint8_t)(vc >> (8 * q));
-    if ((l16 & 3) == 0) {
-        unit[p.ks] = (uint8_t)ke;
-        unit[p.vs] = (uint8_t)ve;
+    for (int i = 0; i < 8; ++i) {
+        const int64_t t = min(max(e.t0 + i, (int64_t)0), a.tokens - 1);
+        kw[i] = *reinterpret_cast<const u32x4 *>(a.k + t * a.k_token + head * a.k_head + 8 * l16);
+        vw[i] = *reinterpret_cast<const u32x4 *>(a.v + t * a.v_token + head * a.v_head + 8 * l16);
+    }
+    uint32_t kc[8], vc[8];
+    int ke[8], ve[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        kc[i] = quantise<DT>(kw[i], ke[i]);
+        vc[i] = quantise<DT>(vw[i], ve[i]);
+    }
+    if (e.base >= 0) {
+        const Place p = place_of(e.base, head, a.kv_heads, l16);
+        uint8_t *unit = a.cache + p.unit;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t *>(unit + p.k + 64 * i) = kc[i];
+        static_for<4>([&](auto q) __attribute__((always_inline)) {
+            *reinterpret_cast<uint2 *>(unit + p.v + 1024 * q) =
+                make_uint2(bytes_of<q>(vc[0], vc[1], vc[2], vc[3]), bytes_of<q>(vc[4], vc[5], vc[6], vc[7]));
+        });
+        if ((l16 & 3) == 0) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) *reinterpret_cast<uint16_t *>(unit + p.ks + 4 * r) = (uint16_t)(ke[r] | ke[4 + r] << 8);
+            *reinterpret_cast<uint2 *>(unit + p.vs) =
+                make_uint2(ve[0] | ve[1] << 8 | ve[2] << 16 | ve[3] << 24, ve[4] | ve[5] << 8 | ve[6] << 16 | ve[7] << 24);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int64_t slot = __shfl(e.slot, i, 8);
+            if (slot >= 0 && slot < a.num_slots) put_token(a, slot, head, l16, kc[i], vc[i], ke[i], ve[i]);
+        }
     }
 }
 
@@ -118,12 +193,9 @@ __device__ __forceinline__ u32x4 dequantise(uint32_t w, float scale) {
     }
 }
 
+// Reads one token's row and writes it out.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void kv4_read_kernel(ReadArgs a) {
-    const int l16 = threadIdx.x & 15, head = blockIdx.y;
-    const int64_t t = (int64_t)blockIdx.x * kRowsPerBlock + (threadIdx.x >> 4);
-    if (t >= a.tokens) return;
-    const int64_t slot = a.slots[t];
+__device__ __forceinline__ void get_token(const ReadArgs &a, int64_t t, int64_t slot, int head, int l16) {
     u32x4 kw = {0, 0, 0, 0}, vw = {0, 0, 0, 0};
     if (slot >= 0 && slot < a.num_slots) {
         const Place p = place_of(slot, head, a.kv_heads, l16);
@@ -140,7 +212,59 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(ReadArgs a) {
     *reinterpret_cast<u32x4 *>(a.v + at) = vw;
 }
 
+template <int DT>
+__global__ __launch_bounds__(kThreads) void kv4_read_kernel(ReadArgs a) {
+    const int64_t t = (int64_t)blockIdx.x * kRowsPerBlock + (threadIdx.x >> 4);
+    if (t < a.tokens) get_token<DT>(a, t, a.slots[t], blockIdx.y, threadIdx.x & 15);
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void kv4_read8_kernel(ReadArgs a) {
+    const int l16 = threadIdx.x & 15, head = blockIdx.y;
+    const Eight e = eight_slots(a.slots, a.tokens, a.num_slots, (int64_t)blockIdx.x * kRowsPerBlock + (threadIdx.x >> 4), l16);
+    if (e.t0 >= a.tokens) return;
+    if (e.base >= 0) {
+        const Place p = place_of(e.base, head, a.kv_heads, l16);
+        const uint8_t *unit = a.cache + p.unit;
+        uint32_t kc[8];
+        uint2 vq[4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) kc[i] = *reinterpret_cast<const uint32_t *>(unit + p.k + 64 * i);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) vq[q] = *reinterpret_cast<const uint2 *>(unit + p.v + 1024 * q);
+        const u32x4 ks = *reinterpret_cast<const u32x4 *>(unit + (p.ks & ~15));  // [r][h][j]
+        const uint2 vs = *reinterpret_cast<const uint2 *>(unit + p.vs);
+        const int h = (p.ks >> 1) & 1;
+        const int64_t at = (e.t0 * a.kv_heads + head) * kD + 8 * l16, step = a.kv_heads * kD;
+        static_for<8>([&](auto i) __attribute__((always_inline)) {
+            constexpr int I = i, J = I >> 2, R = I & 3;
+            const uint32_t k2 = ks[R] >> (16 * h);  // bytes j = 0, 1
+            const uint32_t v4 = J ? vs.y : vs.x;
+            *reinterpret_cast<u32x4 *>(a.k + at + I * step) = dequantise<DT>(kc[I], scale_of<J>(k2));
+            const uint32_t vc = bytes_of<R>(J ? vq[0].y : vq[0].x, J ? vq[1].y : vq[1].x, J ? vq[2].y : vq[2].x, J ? vq[3].y : vq[3].x);
+            *reinterpret_cast<u32x4 *>(a.v + at + I * step) = dequantise<DT>(vc, scale_of<R>(v4));
+        });
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int64_t t = e.t0 + i, slot = __shfl(e.slot, i, 8);
+            if (t >= 0 && t < a.tokens) get_token<DT>(a, t, slot, head, l16);
+        }
+    }
+}
+
+constexpr int64_t kManyRows = 8192;
 constexpr int64_t kMostHeads = 1 << 10, kMostStride = 1 << 28;
+
+// The kernel of a token for 16 lanes, or that of eight.
+template <class K, class A>
+void launch(K one, K eight, const A &a, hipStream_t s) {
+    const bool many = a.tokens * a.kv_heads >= kManyRows;
+    // eight: one group more, as they need not begin with the first token
+    const int64_t groups = many ? (a.tokens + 6) / 8 + 1 : a.tokens;
+    const dim3 grid((unsigned)((groups - 1) / kRowsPerBlock + 1), (unsigned)a.kv_heads);
+    hipLaunchKernelGGL(many ? eight : one, grid, dim3(kThreads), 0, s, a);
+}
 
 int check_pool(int64_t num_blocks, int64_t kv_heads, int64_t tokens) {
     if (num_blocks < 0 || num_blocks > ((int64_t)1 << 31) || kv_heads < 1 || kv_heads > kMostHeads || tokens < 0)
@@ -169,10 +293,9 @@ extern "C" int ck_kv4_cache_write(const void *k, int64_t k_token_stride, int64_t
     WriteArgs a{static_cast<const uint16_t *>(k), static_cast<const uint16_t *>(v), k_token_stride, k_head_stride,
                 v_token_stride, v_head_stride, slots, static_cast<uint8_t *>(cache), tokens, kv_heads,
                 num_blocks * kv4::kPage};
-    const dim3 grid((unsigned)((tokens - 1) / kRowsPerBlock + 1), (unsigned)kv_heads), block(kThreads);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if (dtype == CK_DTYPE_BF16) hipLaunchKernelGGL((kv4_write_kernel<CK_DTYPE_BF16>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((kv4_write_kernel<CK_DTYPE_F16>), grid, block, 0, s, a);
+    if (dtype == CK_DTYPE_BF16) launch(kv4_write_kernel<CK_DTYPE_BF16>, kv4_write8_kernel<CK_DTYPE_BF16>, a, s);
+    else launch(kv4_write_kernel<CK_DTYPE_F16>, kv4_write8_kernel<CK_DTYPE_F16>, a, s);
     CK_RETURN_LAUNCH();
 }
 
@@ -187,9 +310,8 @@ extern "C" int ck_kv4_cache_read(const void *cache, const int64_t *slots, int64_
         return CK_E_INVALID_ARG;
     ReadArgs a{static_cast<const uint8_t *>(cache), slots, static_cast<uint16_t *>(k), static_cast<uint16_t *>(v),
                tokens, kv_heads, num_blocks * kv4::kPage};
-    const dim3 grid((unsigned)((tokens - 1) / kRowsPerBlock + 1), (unsigned)kv_heads), block(kThreads);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if (dtype == CK_DTYPE_BF16) hipLaunchKernelGGL((kv4_read_kernel<CK_DTYPE_BF16>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((kv4_read_kernel<CK_DTYPE_F16>), grid, block, 0, s, a);
+    if (dtype == CK_DTYPE_BF16) launch(kv4_read_kernel<CK_DTYPE_BF16>, kv4_read8_kernel<CK_DTYPE_BF16>, a, s);
+    else launch(kv4_read_kernel<CK_DTYPE_F16>, kv4_read8_kernel<CK_DTYPE_F16>, a, s);
     CK_RETURN_LAUNCH();
 }

@@ -42,7 +42,10 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kGroups = 512;  // workgroups: two per CU
 constexpr int kGroupsWide = 256;  // of many rows: one per CU
-constexpr int kFoldRows = 4096;  // from which on a row's parts are folded by one group of lanes
+// Up to how many rows a row's parts are folded by 8, 4 and 2 groups of lanes. us with 8 / 4 / 2 / 1: 32 rows of 21 parts
+// 4.1 / 4.7 / 5.4 / 6.7, 256 of 36 5.0 / 5.2 / 6.9 / 12, 1024 of 17 7.3 / 6.7 / 7.0 / 9.4, 2048 of 10 10.0 / 7.5 / 7.8 / 10.0
+// (of 5: 8.3 / 6.0 / 5.4 / 5.5), 4608 of 11 13.4 / 8.3 / 7.8 / 8.6, 7488 of 6 23 / 16.6 / 11.6 / 9.3.
+constexpr int kFoldRows[3] = {512, 2048, 6144};
 constexpr float kSlack = 8.f;
 constexpr uint32_t kRsrcFlags = 0x00020000;
 
@@ -1128,8 +1131,8 @@ struct FoldSide {
 struct FoldArgs {
     FoldSide own, prefix;
     int q_len, heads, kv_heads, group;
-    int64_t rows;  // batch * q_len * heads
-    int merge;     // with a prefix, and every part there
+    int rows;   // batch * q_len * heads
+    int merge;  // with a prefix, and every part there
     uint16_t *out;
     float *lse;
 };
@@ -1167,13 +1170,12 @@ template <int DT, int PG>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(FoldArgs a) {
     constexpr int kBlockRows = 8 / PG;
     const int group = threadIdx.x >> 5, lane = threadIdx.x & 31, pg = group % PG, g4 = lane & 3, j = lane >> 2;
-    const int64_t row = (int64_t)blockIdx.x * kBlockRows + group / PG;
+    const int row = (int)blockIdx.x * kBlockRows + group / PG;  // below 2^24
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     bool done = row >= a.rows;  // or written by the wave that had all of it
     if (!done) {
-        const int64_t t = row / a.heads;
-        const int head = (int)(row - t * a.heads), b = (int)(t / a.q_len), tok = (int)(t - (int64_t)b * a.q_len);
+        const int t = row / a.heads, head = row - t * a.heads, b = t / a.q_len, tok = t - b * a.q_len;
         const int h = head / a.group, hg = head - h * a.group;
         auto fold = [&](const Parts &p, int slot_rows) {
             constexpr int kBatch = 4;
@@ -1211,23 +1213,23 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(FoldArgs a) {
         if (a.merge) fold(parts_of(a.prefix, a.kv_heads, 0, h, b * a.group + hg), a.prefix.slot_rows);
     }
     if constexpr (PG > 1) {
-        __shared__ f32x4 part[PG][32];
-        __shared__ float2 part_ml[PG];
-        part[pg][lane] = o;
-        if (lane == 0) part_ml[pg] = make_float2(m, l);
+        __shared__ f32x4 part[8][32];
+        __shared__ float2 part_ml[8];
+        part[group][lane] = o;
+        if (lane == 0) part_ml[group] = make_float2(m, l);
         __syncthreads();
-        if (pg > 0) return;
+        if (pg > 0) return;  // the others of the row: group + 1 .. + PG - 1
         float top = m;
 #pragma unroll
-        for (int i = 1; i < PG; ++i) top = fmaxf(top, part_ml[i].x);
+        for (int i = 1; i < PG; ++i) top = fmaxf(top, part_ml[group + i].x);
         l = 0.f;
         o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < PG; ++i) {
-            const float2 ml = part_ml[i];
+            const float2 ml = part_ml[group + i];
             const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - top);
             l = fmaf(ml.y, f, l);
-            const f32x4 x = part[i][lane];
+            const f32x4 x = part[group + i][lane];
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
         }
@@ -1237,7 +1239,7 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(FoldArgs a) {
     using E = Elem<DT>;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     const uint2 x = make_uint2(E::pack2(o[0] * inv, o[1] * inv), E::pack2(o[2] * inv, o[3] * inv));
-    *reinterpret_cast<uint2 *>(a.out + row * kD + 32 * g4 + 4 * j) = x;
+    *reinterpret_cast<uint2 *>(a.out + (int64_t)row * kD + 32 * g4 + 4 * j) = x;
     if (lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
@@ -1336,10 +1338,14 @@ int launch(const DecodeArgs &own, const DecodeArgs *prefix, const Plan &p, const
         if (rc == CK_OK) rc = launch_side<DT, false>(own, p.own, s);
     }
     if (rc != CK_OK) return rc;
-    if (f.rows >= kFoldRows)
-        hipLaunchKernelGGL((kv4_combine_kernel<DT, 1>), dim3((unsigned)ceil_div(f.rows, 8)), dim3(256), 0, s, f);
-    else
-        hipLaunchKernelGGL((kv4_combine_kernel<DT, 8>), dim3((unsigned)f.rows), dim3(256), 0, s, f);
+    auto fold = [&](auto groups) {
+        constexpr int PG = groups;
+        hipLaunchKernelGGL((kv4_combine_kernel<DT, PG>), dim3((unsigned)ceil_div(f.rows, 8 / PG)), dim3(256), 0, s, f);
+    };
+    if (f.rows <= kFoldRows[0]) fold(std::integral_constant<int, 8>{});
+    else if (f.rows <= kFoldRows[1]) fold(std::integral_constant<int, 4>{});
+    else if (f.rows <= kFoldRows[2]) fold(std::integral_constant<int, 2>{});
+    else fold(std::integral_constant<int, 1>{});
     CK_RETURN_LAUNCH();
 }
 
@@ -1413,7 +1419,7 @@ int run(const void *q, const Pool &pool, const Pool *prefix, int64_t batch, int6
     f.heads = a.heads;
     f.kv_heads = a.kv_heads;
     f.group = a.group;
-    f.rows = batch * q_len * heads;
+    f.rows = (int)(batch * q_len * heads);
     f.merge = a.merge;
     f.out = a.out;
     f.lse = lse;
