@@ -108,7 +108,8 @@ def attend(q, k, v, sees, scale, dtype, rows):
     number); the call has `rows` of them a kv head. Returns (o, lse, bound of |out - o|, bound of
     |out lse - lse|).
 
-    out rounds by half a step u |o| (fp16 also by half its least step, 2^-25). A score is an fp32 sum of 128
+    out rounds by half a step u |o|, below the least normal number by half the least step: 2^-25 in fp16 (steps of
+    2^-14-10), 2^-134 in bf16 (of 2^-126-7). A score is an fp32 sum of 128
     exact products, (128 + 8) roundings of partial sums below sum |q| |k|, times the scale (2 roundings,
     its conversion to log2 among them); an error e of the scores moves a softmax weight by 2 e of it. P enters
     as two bf16 terms, off by 2^-18 of it, or (more than 16 rows a kv head) as an fp16 number, off by 2^-11 of it; 2^7 p
@@ -131,6 +132,5 @@ def attend(q, k, v, sees, scale, dtype, rows):
     sums = (sees + 64) * F32
     p_off, lost = (2.0 ** -18, 0.0) if rows <= 16 else (2.0 ** -11, 2.0 ** -32)
     b_o = u * o.abs() + (1 + u) * ((p_off + 2 * e + sums)[:, None] * mean + (sees * lost)[:, None] * v.abs().amax())
-    if dtype == torch.float16:
-        b_o = b_o + 2.0 ** -25
+    b_o = b_o + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134)
     return o, lse, b_o, e + sums + 8 * F32 * lse.nan_to_num(0, 0, 0).abs()
