@@ -80,9 +80,9 @@ def _slots(gen, how, tokens, blocks):
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("how", ["anywhere", "prompt", "mixed"])
-@pytest.mark.parametrize("tokens,kv_heads", [(1024, 8), (2049, 4), (2740, 3)])
+@pytest.mark.parametrize("tokens,kv_heads", [(2049, 4), (6144, 8), (16385, 3)])
 def test_write_and_read_of_many_tokens(tokens, kv_heads, how, dtype):
-    """From 8192 rows on, eight neighbouring tokens are moved together."""
+    """From 49152 rows on, eight neighbouring tokens are moved together."""
     g = _gen(tokens)
     blocks = tokens // 128 + 12
     slots = _slots(g, how, tokens, blocks)

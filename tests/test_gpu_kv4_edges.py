@@ -299,9 +299,9 @@ def test_offsets_past_32_bits(kv_heads):
         want = [o4.values(*o4.quantise(x)) for x in (k, v)]
         for got, ref in zip(OPS.kv4_cache_read(pool, slots), want):
             assert torch.equal(got.double(), ref)
-    big = slots.repeat(30)  # from 8192 rows on
+    big = slots.repeat(130)  # eight tokens at a time
     for got, ref in zip(OPS.kv4_cache_read(pool, big), want):
-        assert torch.equal(got.double(), ref.repeat(30, 1, 1))
+        assert torch.equal(got.double(), ref.repeat(130, 1, 1))
     table = torch.tensor([ids], dtype=torch.int32, device=DEV)
     for group in (2, 20, 40):
         q = _normal(g, 1, group * kv_heads, 128)
@@ -382,15 +382,15 @@ def test_streams_and_repeats():
 def test_graphs_of_a_step():
     """Write, read, decode and shared-prefix decode captured, two graphs of other shapes replayed in turn on other contents,
     lengths and tables, with eager calls between the replays."""
-    def inputs(seed, heads, tokens):
+    def inputs(seed, heads, tokens, pages):
         g = _gen(seed)
-        table = torch.randperm(24, generator=g, device=DEV)[:12].view(3, 4).to(torch.int32)
+        table = torch.randperm(pages, generator=g, device=DEV)[:12].view(3, 4).to(torch.int32)
         lens = [[130, 5, 400], [0, 512, 33], [1, 1, 256], [512, 300, 0]][seed % 4]
-        slots = torch.randperm(24 * 128, generator=g, device=DEV)[:tokens]
+        slots = torch.randperm(pages * 128, generator=g, device=DEV)[:tokens]
         slots[0] = -1
         if seed % 2:
             slots = slots.sort().values
-        return dict(k=_normal(g, tokens, 2, 128), v=_normal(g, tokens, 2, 128), slots=slots, pool=o4.random_pool(g, 24, 2, DEV),
+        return dict(k=_normal(g, tokens, 2, 128), v=_normal(g, tokens, 2, 128), slots=slots, pool=o4.random_pool(g, pages, 2, DEV),
                     table=table, lens=_i64(lens), plen=_i64([[512, 100, 0, 33][seed % 4]]), q=_normal(g, 3, heads, 128),
                     q2=_normal(g, 6, heads, 128))
 
@@ -402,10 +402,10 @@ def test_graphs_of_a_step():
         c = OPS.kv4_cascade_decode(t["q"], t["pool"], t["table"][:1], t["plen"], t["pool"], t["table"], t["lens"], SCALE)
         return r + a + b + c + (t["pool"],)
 
-    shapes = [(16, 3), (48, 3000)]
+    shapes = [(16, 3, 24), (48, 24600, 200)]
     statics, graphs, outs = [], [], []
-    for heads, tokens in shapes:
-        static = inputs(0, heads, tokens)
+    for shape in shapes:
+        static = inputs(0, *shape)
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
