@@ -6,24 +6,31 @@
 //   o = sum_j softmax(s)_j v_j,  lse = log sum_j exp(s_j)
 // A row that sees no token gets o = 0, lse = -inf.
 //
-// A token and kv head are 136 bytes and 512 flops a row: up to some 32 rows a kv head memory
-// bounds the call. A wave computes alone, for 16 NB rows of a kv head (tokens of a request times query
-// heads of the kv head):
-// * A unit of 64 tokens (8704 bytes that lie together) is 10 loads of a wave, straight into registers in
-//   the operands' order; the next unit's are under way while one is computed.
-// * S^T = K Q^T on 16x16x32 products: lane (g, n) holds group g of a token's key, four codes-to-bf16
-//   conversions (two values each, the scale in the instruction) make an operand. O^T = V^T P^T: lane (g, n)
-//   holds dims 8 n .. + 7 of tokens 8 g .. + 7; two conversions give (token, dim pair) words, two byte
-//   permutations turn them to (dim, token pair). P is in its operand's place as it leaves the scores.
-// * bf16 holds every dequantised value; P enters as two bf16 terms, within 2^-17 of fp32; an fp16 query as
-//   two bf16 terms, which hold all of it.
+// A token and kv head are 136 bytes and 512 flops a row: memory bounds a call up to some 16 rows a kv head
+// (tokens of a request times query heads of the kv head), arithmetic beyond.
+// * S^T = K Q^T on 16x16x32 products: lane (g, n) holds group g of a token's key, four code conversions (two
+//   values each, the scale in the instruction) make an operand. O^T = V^T P^T: lane (g, n) holds dims 8 n .. + 7 of
+//   tokens 8 g .. + 7; two conversions give (token, dim pair) words, two byte permutations turn them to (dim, token
+//   pair). P is in its operand's place as it leaves the scores. The pool's order is that of these operands, so that a
+//   lane loads 16 bytes at a time and nothing is exchanged.
 // * The softmax's reference point m of a row moves only when a score passes it by 2^kSlack (any point gives the
 //   same result), so that O is hardly ever rescaled.
-// * The units of all requests and kv heads form one list, cut evenly over the waves of a grid that fills the
-//   chip once, so ragged lengths balance. An item (request and kv head) inside one share is written as it is;
-//   parts of a cut one go to the workspace, and kv4_combine_kernel folds them.
-// * Rows past 16 NB are row tiles of their own, given to neighbouring waves, which read the same units.
-// * Shared prefix: the batch is one request's rows over the prefix; then the suffixes; one fold for both.
+// * The units (64 tokens, 8704 bytes that lie together) of all requests and kv heads form one list, cut evenly
+//   over a grid that fills the chip once, so ragged lengths balance. An item (request and kv head) inside one share is
+//   written as it is; parts of a cut one go to the workspace, not normalised, and kv4_combine_kernel folds them.
+// * Up to 32 rows a wave computes alone (kv4_decode_kernel): up to 16 with units in registers, the next one's loads
+//   under way while one is computed; up to 32 with a ring of two units in LDS. More rows take kv4_wide_kernel.
+// * Shared prefix: the batch is one request's rows over the prefix. Where the suffixes have up to 16 rows each, one
+//   launch takes both lists, a wave its share of the prefix and then of the suffixes; one fold for all parts.
+//   us a call, one launch / two: 8 x 32 heads on 2000 + 200 tokens 16.0 / 18.4, 64 x 32 on 8000 + 200 40 / 47,
+//   on 500 + 2000 46 / 51, 256 x 32 on 8000 + 300 78 / 85.
+//
+// Measured (kernel + fold in us; query / kv heads): 64 requests of 2048 to 8192 tokens, 32 / 8, 73 + 5, 4.8 TB/s; 16 of 16384
+// to 65536, 64 / 8, 160 + 7, 5.3 TB/s; 5 of 5000 to 20011, 20 / 20 in fp16, 31 + 5; one of 1300, 32 / 8, 6 + 4, chains of
+// round trips (lengths, table, unit, fold) and two launches. 24 requests of 1250 to 5000, 3 tokens, 64 / 8 in fp16 (24
+// rows): 28 + 8, 12 of them vector instructions, 25 MB of parts written and read. 17 / 24 / 32 rows in the form for
+// 32 against the one for 64, us a call: 24 requests of 1000 tokens, 8 kv heads, 23 / 24 / 26 against 30 / 30 / 32; 64 of 4000
+// 69 / 74 / 77 against 96 / 97 / 100; one of 16000 25 / 25 / 27 against 27 / 26 / 26.
 #include <cmath>
 #include <type_traits>
 
@@ -40,8 +47,8 @@ typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kGroups = 512;  // workgroups: two per CU
-constexpr int kGroupsWide = 256;  // of many rows: one per CU
+constexpr int kGroups = 512;      // workgroups: two per CU, so two waves a SIMD, as many as the registers allow
+constexpr int kGroupsWide = 256;  // of many rows: one per CU, which its LDS fills
 // Up to how many rows a row's parts are folded by 8, 4 and 2 groups of lanes. us with 8 / 4 / 2 / 1: 32 rows of 21 parts
 // 4.1 / 4.7 / 5.4 / 6.7, 256 of 36 5.0 / 5.2 / 6.9 / 12, 1024 of 17 7.3 / 6.7 / 7.0 / 9.4, 2048 of 10 10.0 / 7.5 / 7.8 / 10.0
 // (of 5: 8.3 / 6.0 / 5.4 / 5.5), 4608 of 11 13.4 / 8.3 / 7.8 / 8.6, 7488 of 6 23 / 16.6 / 11.6 / 9.3.
@@ -57,13 +64,12 @@ struct DecodeArgs {
     int64_t bt_cols;
     int64_t num_blocks;
     int batch, q_len, heads, kv_heads;
-    int group;   // query heads per kv head
-    int rows;    // q_len * group: of an item
-    int tiles;   // row tiles of an item
-    int tile_rows;
-    int waves;   // shares of the list (waves', or with many rows workgroups'), per row tile
+    int group;  // query heads per kv head
+    int rows;   // q_len * group: of an item
+    int tiles;  // row tiles of an item
+    int waves;  // shares of the list (waves', or with many rows workgroups'), per row tile
     int causal;
-    int merge;   // every part goes to the workspace
+    int merge;  // every part goes to the workspace
     float scale_log2;
     uint16_t *out;
     float *lse;
@@ -729,8 +735,12 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(std::conditiona
 // each other's waits. A workgroup takes a row tile of 64 rows, whose query is in LDS (O alone takes half of a wave's
 // registers); its waves take an item's units in turn, each through a double buffer of its own in LDS, so that
 // nothing holds them together: with a ring that all read, and a barrier for every 4 units, 117 x 64 heads on 16001 tokens
-// took 108 to 118 us. Their parts are joined through LDS, so that few go to memory. A wave works in halves of 32 tokens.
+// took 108 to 118 us. Their parts are joined through LDS, so that few go to memory. A wave works in halves of 32 tokens,
+// 64 products and 287 vector instructions each (codes 64 and their permutations 32, exponentials 32, their arguments,
+// sums and conversions 84): these bound it, and the start and the joint where a workgroup has few units.
 // The shares of the list are workgroups', neighbours on one XCD, so that the row tiles of a share meet in its L2.
+// Kernel, then fold: 117 x 64 heads on 16001 tokens (fp16) 98 + 9 us a call, the matrix cores 27% busy, the vector
+// units 45%; 64 x 32 on 8192 34 + 8.
 constexpr int kWideThreads = 512, kWideWaves = kWideThreads / 64;
 constexpr int kWideQ = kWideWaves * 2 * kUnitBytes;  // [NB][4] operands of 1 KB, behind the waves' buffers
 constexpr int kWideStarts = kWideQ + 4 * 4 * 1024;
@@ -1370,12 +1380,11 @@ void fill(DecodeArgs *a, FoldSide *f, const Pool &pool, const Side &p, int64_t b
     a->batch = (int)batch;
     a->rows = (int)p.rows;
     a->tiles = (int)p.tiles;
-    a->tile_rows = (int)p.tile_rows;
     a->waves = (int)p.waves;
     a->part_o = reinterpret_cast<float *>(ws + p.off_o);
     a->part_ml = reinterpret_cast<float2 *>(ws + p.off_ml);
     a->sums = reinterpret_cast<int32_t *>(ws + p.off_sums);
-    *f = FoldSide{a->part_o, a->part_ml, a->sums, a->batch, a->waves, a->tiles, a->tile_rows, (int)p.slot_rows};
+    *f = FoldSide{a->part_o, a->part_ml, a->sums, a->batch, a->waves, a->tiles, (int)p.tile_rows, (int)p.slot_rows};
 }
 
 int run(const void *q, const Pool &pool, const Pool *prefix, int64_t batch, int64_t q_len, int64_t heads,
