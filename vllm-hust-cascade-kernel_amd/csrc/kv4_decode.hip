@@ -299,7 +299,7 @@ template <int DT, int NB>
 struct Rows {
     u32x4 q[NB][Form<DT, NB>::kTerms][4];  // dims 32 g + 8 c .. + 7
     f32x4 o[NB][8];  // O^T: dims 32 g + 8 r + block of the row
-    float m[NB];     // the sum's reference point (log2; the same for all g) is m - kBias
+    float m[NB];     // the sum's reference point (log2; the same for all g), kBias below a score
     float l[NB];     // this lane's share of the sum
     uint32_t bad;    // bit i: row i sees a value that is not a number in this lane's dims
 };
@@ -386,7 +386,7 @@ __device__ __forceinline__ void add_values(Rows<DT, NB> &s, const u32x4 (&v)[4],
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         const int i = I0 + k;
-        const float sub = s.m[i] == -INFINITY ? 0.f : s.m[i] - Form<DT, NB>::kBias;
+        const float sub = s.m[i] == -INFINITY ? 0.f : s.m[i];
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -452,14 +452,15 @@ __device__ __forceinline__ void add_values(Rows<DT, NB> &s, const u32x4 (&v)[4],
     }
 }
 
-// Moves the reference points of rows whose scores pass them by 2^kSlack (most: the lane's largest) to the
-// largest; no score passes them by as much again.
+// Moves the reference points of rows whose scores pass them by 2^(kSlack + kBias) (most: the lane's largest) to 2^kBias
+// below the largest; no score of these passes them by as much again.
 template <int NB>
 __device__ __forceinline__ void move_points(f32x4 (&o)[NB][8], float (&m)[NB], float (&l)[NB], const float (&most)[NB]) {
+    constexpr float kBias = Form<CK_DTYPE_BF16, NB>::kBias;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
         const float all = over_groups(most[i], [](float x, float y) { return fmaxf(x, y); });
-        const float to = all > m[i] + kSlack ? all : m[i];
+        const float to = all > m[i] + (kSlack + kBias) ? all - kBias : m[i];
         const float by = to == m[i] ? 1.f : exp2_fast(m[i] - to);
         l[i] *= by;
 #pragma unroll
@@ -507,6 +508,7 @@ __device__ __forceinline__ void hide_values(uint32_t &bad, uint32_t &x, uint32_t
 template <int DT, int NB, class U>
 __device__ __forceinline__ void compute(Rows<DT, NB> &s, const U &u, float scale_log2, int lane, bool tail,
                                         const int (&sees)[NB], int left) {
+    constexpr float kBias = Form<DT, NB>::kBias;
     constexpr bool kHalf = Form<DT, NB>::kHalf, kHalfKeys = kHalf && DT == CK_DTYPE_F16;
     u32x4 k[4];
 #pragma unroll
@@ -544,9 +546,9 @@ __device__ __forceinline__ void compute(Rows<DT, NB> &s, const U &u, float scale
 #pragma unroll
         for (int e = 3; e < 15; e += 2) most = max3(most, sc[i][e >> 2][e & 3], sc[i][(e + 1) >> 2][(e + 1) & 3]);
         most = fmaxf(most, sc[i][3][3]) * scale_log2;
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > s.m[i] + kSlack) != 0, 0)) {
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > s.m[i] + (kSlack + kBias)) != 0, 0)) {
             const float all = over_groups(most, [](float x, float y) { return fmaxf(x, y); });
-            const float m = all > s.m[i] + kSlack ? all : s.m[i];
+            const float m = all > s.m[i] + (kSlack + kBias) ? all - kBias : s.m[i];
             const float f = m == s.m[i] ? 1.f : exp2_fast(s.m[i] - m);
             s.l[i] *= f;
 #pragma unroll
@@ -618,7 +620,7 @@ __device__ __forceinline__ void decode_share(const KernArgs args, const L &list,
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             const int r = 16 * i + n16;
-            const float l = over_groups(s.l[i], [](float x, float y) { return x + y; }), m = s.m[i] - Form<DT, NB>::kBias;
+            const float l = over_groups(s.l[i], [](float x, float y) { return x + y; }), m = s.m[i];
             if (r >= a->rows) continue;
             if (whole) {
                 using E = Elem<DT>;
@@ -736,11 +738,12 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(std::conditiona
 // registers); its waves take an item's units in turn, each through a double buffer of its own in LDS, so that
 // nothing holds them together: with a ring that all read, and a barrier for every 4 units, 117 x 64 heads on 16001 tokens
 // took 108 to 118 us. Their parts are joined through LDS, so that few go to memory. A wave works in halves of 32 tokens,
-// 64 products and 287 vector instructions each (codes 64 and their permutations 32, exponentials 32, their arguments,
-// sums and conversions 84): these bound it, and the start and the joint where a workgroup has few units.
+// 64 products and 271 vector instructions each (codes 64 and their permutations 32, exponentials 32, their arguments,
+// sums and conversions 84); these bound it, at 950 TFLOP/s over a long prefix, and the start and the joint where a
+// workgroup has few units. Where a half's last tokens are hidden, only scores and scales are changed in the loop; a half
+// that holds nothing is passed over (two such halves of 16001 tokens cost 6 us of 109 outside it).
 // The shares of the list are workgroups', neighbours on one XCD, so that the row tiles of a share meet in its L2.
-// Kernel, then fold: 117 x 64 heads on 16001 tokens (fp16) 98 + 9 us a call, the matrix cores 27% busy, the vector
-// units 45%; 64 x 32 on 8192 34 + 8.
+// Kernel and fold, us a call: 117 x 64 heads on 16001 tokens and suffixes (fp16) 102, 64 x 32 on 8192 39.
 constexpr int kWideThreads = 512, kWideWaves = kWideThreads / 64;
 constexpr int kWideQ = kWideWaves * 2 * kUnitBytes;  // [NB][4] operands of 1 KB, behind the waves' buffers
 constexpr int kWideStarts = kWideQ + 4 * 4 * 1024;
@@ -754,18 +757,30 @@ struct Half {
     uint32_t ks, v[4][2], vs[2];
 };
 typedef __attribute__((__vector_size__(2 * sizeof(unsigned)))) unsigned u32x2;
-__device__ __forceinline__ void read_half(Half &x, const CK_LDS char *slot, int h, int lane) {
-    const CK_LDS char *at = slot + 16 * lane;
+__device__ __forceinline__ void read_keys(Half &x, const CK_LDS char *slot, int h, int lane) {
     const CK_LDS char *k_at = slot + keys_in_lds(lane) + 2048 * h;
     x.k[0] = *reinterpret_cast<const CK_LDS u32x4 *>(k_at);
     x.k[1] = *reinterpret_cast<const CK_LDS u32x4 *>(k_at + 256);
     x.ks = *reinterpret_cast<const CK_LDS uint16_t *>(slot + kKsAt + 4 * lane + 2 * h);
     const u32x2 s = *reinterpret_cast<const CK_LDS u32x2 *>(slot + kVsAt + ((lane & 15) >> 2) * 64 + 16 * (lane >> 4) + 8 * h);
     x.vs[0] = s[0], x.vs[1] = s[1];
+}
+__device__ __forceinline__ void read_values(Half &x, const CK_LDS char *slot, int h, int lane) {
+    const CK_LDS char *at = slot + 16 * lane;
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
         const u32x2 y = *reinterpret_cast<const CK_LDS u32x2 *>(at + kVAt + 1024 * d + 8 * h);
         x.v[d][0] = y[0], x.v[d][1] = y[1];
+    }
+}
+
+// The order of a part of a loop: N times a product and V vector instructions, which run beside it.
+template <int N, int V>
+__device__ __forceinline__ void mix() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
     }
 }
 
@@ -775,8 +790,18 @@ __device__ __forceinline__ void half_scores(f32x4 (&sc)[NB][2], const Half &x, c
 #pragma unroll
     for (int i = 0; i < NB; ++i) sc[i][0] = sc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     const float f[2] = {scale_of<0>(x.ks), scale_of<1>(x.ks)};
+    // the query's operands of the next dims come while these are multiplied; as two terms there are no registers for it
+    constexpr int kAhead = DT != CK_DTYPE_F16 || HALF ? 1 : 0;
+    u32x4 y[1 + kAhead][NB];
+    auto read_q = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) y[c & kAhead][i] = *reinterpret_cast<const CK_LDS u32x4 *>(q + (4 * i + c) * 1024);
+    };
+    if (kAhead) read_q(0);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
+        if (c + kAhead < 4) read_q(c + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
         u32x4 a[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -786,22 +811,22 @@ __device__ __forceinline__ void half_scores(f32x4 (&sc)[NB][2], const Half &x, c
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const u32x4 y = *reinterpret_cast<const CK_LDS u32x4 *>(q + (4 * i + c) * 1024);
+            const u32x4 &z = y[c & kAhead][i];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 if constexpr (HALF) {
-                    sc[i][t] = mfma_f16(a[t], y, sc[i][t]);
+                    sc[i][t] = mfma_f16(a[t], z, sc[i][t]);
                 } else if constexpr (DT == CK_DTYPE_F16) {
                     u32x4 hi, lo;
-                    two_terms(y, hi, lo);
+                    two_terms(z, hi, lo);
                     sc[i][t] = mfma_bf16(a[t], hi, sc[i][t]);
                     sc[i][t] = mfma_bf16(a[t], lo, sc[i][t]);
                 } else {
-                    sc[i][t] = mfma_bf16(a[t], y, sc[i][t]);
+                    sc[i][t] = mfma_bf16(a[t], z, sc[i][t]);
                 }
             }
         }
-        if (NB > 2 || !HALF) __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 // The largest score of a row block's lane.
@@ -809,7 +834,7 @@ __device__ __forceinline__ float largest(const f32x4 (&s)[2]) {
     float x = max3(s[0][0], s[0][1], s[0][2]);
     x = max3(x, s[0][3], s[1][0]);
     x = max3(x, s[1][1], s[1][2]);
-    return fmaxf(x, s[1][3]);
+    return max3(x, s[1][3], s[1][3]);  // fmaxf would first make its operands canonical
 }
 
 // P of row blocks I0 .. I0 + N - 1 over a half, its sums, and O^T += V^T P^T.
@@ -821,7 +846,7 @@ __device__ __forceinline__ void half_values(f32x4 (&o)[NB][8], float (&l)[NB], c
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         const int i = I0 + k;
-        const float sub = m[i] == -INFINITY ? 0.f : m[i] - Form<CK_DTYPE_BF16, NB>::kBias;
+        const float sub = !HALF && m[i] == -INFINITY ? 0.f : m[i];  // HALF: no such row
         float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -847,9 +872,10 @@ __device__ __forceinline__ void half_values(f32x4 (&o)[NB][8], float (&l)[NB], c
         f[4 * w + 2] = scale_of<2>(x.vs[w]);
         f[4 * w + 3] = scale_of<3>(x.vs[w]);
     }
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-        u32x4 even, odd;
+    constexpr int kAhead = HALF ? 1 : 0;  // the next dims' operands are made beside the products
+    u32x4 even[1 + kAhead], odd[1 + kAhead];
+    auto operands = [&](int d) __attribute__((always_inline)) {
+        u32x4 &a = even[d & kAhead], &b = odd[d & kAhead];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             const uint32_t c = x.v[d][w];
@@ -861,45 +887,84 @@ __device__ __forceinline__ void half_values(f32x4 (&o)[NB][8], float (&l)[NB], c
                 t[0] = pair_bf16<0>(c, f[4 * w]), t[1] = pair_bf16<1>(c, f[4 * w + 1]);
                 t[2] = pair_bf16<2>(c, f[4 * w + 2]), t[3] = pair_bf16<3>(c, f[4 * w + 3]);
             }
-            even[2 * w] = __builtin_amdgcn_perm(t[1], t[0], 0x05040100);
-            odd[2 * w] = __builtin_amdgcn_perm(t[1], t[0], 0x07060302);
-            even[2 * w + 1] = __builtin_amdgcn_perm(t[3], t[2], 0x05040100);
-            odd[2 * w + 1] = __builtin_amdgcn_perm(t[3], t[2], 0x07060302);
+            a[2 * w] = __builtin_amdgcn_perm(t[1], t[0], 0x05040100);
+            b[2 * w] = __builtin_amdgcn_perm(t[1], t[0], 0x07060302);
+            a[2 * w + 1] = __builtin_amdgcn_perm(t[3], t[2], 0x05040100);
+            b[2 * w + 1] = __builtin_amdgcn_perm(t[3], t[2], 0x07060302);
         }
+    };
+    if (kAhead) {
+        operands(0);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        if (kAhead == 0) operands(d);
+        else if (d < 3) operands(d + 1);
 #pragma unroll
         for (int e = 0; e < kParts; ++e)
 #pragma unroll
             for (int k = 0; k < N; ++k) {
                 f32x4 &lo = o[I0 + k][2 * d], &hi = o[I0 + k][2 * d + 1];
-                lo = HALF ? mfma_f16(even, p[k][e], lo) : mfma_bf16(even, p[k][e], lo);
-                hi = HALF ? mfma_f16(odd, p[k][e], hi) : mfma_bf16(odd, p[k][e], hi);
+                lo = HALF ? mfma_f16(even[d & kAhead], p[k][e], lo) : mfma_bf16(even[d & kAhead], p[k][e], lo);
+                hi = HALF ? mfma_f16(odd[d & kAhead], p[k][e], hi) : mfma_bf16(odd[d & kAhead], p[k][e], hi);
             }
+        if constexpr (kAhead) mix<2 * N, 2>();
         __builtin_amdgcn_sched_barrier(0);
     }
 }
 
-// Any half: of any scales, with tokens that some row does not see (row0, group: of the wave's rows, where several
-// tokens of a request are causal among themselves, first_sees < left), or with scores past a reference point.
+// How many of a half's tokens a lane's row of block i sees.
+__device__ __forceinline__ int sees_of(int i, int n16, int left, int first_sees, int row0, int group) {
+    return first_sees < left ? min(first_sees + (row0 + 16 * i + n16) / group, left) : left;
+}
+// Scores of tokens that a row does not see: -inf.
+template <int NB>
+__device__ __forceinline__ void hide_scores(f32x4 (&sc)[NB][2], int lane, int left, int first_sees, int row0, int group) {
+    const int y = lane_again(lane);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int n = sees_of(i, y & 15, left, first_sees, row0, group) - 8 * (y >> 4);  // token of sc[i][t][r]: 8 g + 4 t + r
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e >= n) sc[i][e >> 2][e & 3] = -INFINITY;
+    }
+}
+// Ordinary scales in the place of those behind `left`, which may be any.
+template <int DT>
+__device__ __forceinline__ void end_half(Half &x, int left, int lane) {
+    const int y = lane_again(lane), n16 = y & 15, t = 8 * (n16 >> 2) + (n16 & 3);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) x.vs[w] = first_bytes(x.vs[w], left - 8 * (y >> 4) - 4 * w, kMidScales);
+    if constexpr (DT == CK_DTYPE_F16) {
+        if (t >= left) x.ks = (x.ks & 0xff00) | (kMidScales & 0xff);
+        if (t + 4 >= left) x.ks = (x.ks & 0xff) | (kMidScales & 0xff00);
+    }
+}
+
+// Any half: of any scales, with scores past a reference point, with rows that have seen nothing yet. row0, group: of the
+// wave's rows, where several tokens of a request are causal among themselves (first_sees < left). An fp16 query's keys are
+// made as in the usual half where their scales allow it: of random scores 117 x 64 heads on 16001 tokens then take 103 us
+// instead of 115, as each wave moves its points a few times.
 template <int DT, int NB>
 __device__ __forceinline__ void any_half(f32x4 (&o)[NB][8], float (&m)[NB], float (&l)[NB], uint32_t &bad, const CK_LDS char *q,
                                          const CK_LDS char *slot, int h, float scale_log2, int lane, int left, int first_sees,
                                          int row0, int group) {
     Half x;
-    read_half(x, slot, h, lane);
+    read_keys(x, slot, h, lane);
+    read_values(x, slot, h, lane);
     f32x4 sc[NB][2];
-    half_scores<false, DT, NB>(sc, x, q);
+    if (DT == CK_DTYPE_F16 && __builtin_amdgcn_ballot_w64(past_half(x.ks | (kMidScales & 0xffff0000)) != 0) == 0)
+        half_scores<true, DT, NB>(sc, x, q);
+    else
+        half_scores<false, DT, NB>(sc, x, q);
     if (first_sees < 32) {
-        const int y = lane_again(lane), g = y >> 4;
+        hide_scores<NB>(sc, lane, left, first_sees, row0, group);
+        const int y = lane_again(lane);
         int sees[NB];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            sees[i] = first_sees < left ? min(first_sees + (row0 + 16 * i + (y & 15)) / group, left) : left;
-            const int n = sees[i] - 8 * g;  // token of sc[i][t][r]: 8 g + 4 t + r
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (e >= n) sc[i][e >> 2][e & 3] = -INFINITY;
-        }
-        hide_values<NB>(bad, x.vs[0], x.vs[1], sees, left, g);
+        for (int i = 0; i < NB; ++i) sees[i] = sees_of(i, y & 15, left, first_sees, row0, group);
+        hide_values<NB>(bad, x.vs[0], x.vs[1], sees, left, y >> 4);
     }
     float most[NB];
 #pragma unroll
@@ -918,6 +983,7 @@ template <int DT, bool PAIR>
 __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditional_t<PAIR, PairArgs, DecodeArgs>) {
     using E = Elem<DT>;
     constexpr int NB = 4, kTileRows = 16 * NB, kParts = kWideWaves / 2;
+    constexpr float kBias = Form<DT, NB>::kBias;
     const KernArgs args = (KernArgs)__builtin_amdgcn_kernarg_segment_ptr();
     KernArgs a = args_again(args);
     extern __shared__ __attribute__((aligned(16))) char wide_raw[];
@@ -947,6 +1013,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
         const bool before = i0 > 0, after = i1 < each, causal = a->causal;
         const int q_len = a->q_len, group = a->group;
         const float scale_log2 = a->scale_log2;
+        int fewer = causal ? q_len - 1 : 0;  // keys that the request's first row does not see
+        asm volatile("" : "+s"(fewer));      // nor loaded again for every half
         cur += i1 - i0;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
@@ -989,8 +1057,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
                 move_unit(of_lane(d_at, 0), slot_of(0), lane_again(lane));
             }
             int k = 0, half = 0;
-            // The first loop takes what it can, halves seen whole by all rows, of fp16's scales and with no score past a
-            // reference point; nothing else changes O in it, or the compiler would hold O twice and copy it.
+            // The first loop takes halves of fp16's scales with no score past a reference point; nothing else changes O in
+            // it, or the compiler would hold O twice and copy it.
             for (;;) {
                 int left, first_sees;
                 const CK_LDS char *slot;
@@ -1007,33 +1075,41 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
                     }
                     slot = slot_of(k);
                     left = len - (c0 + kWideWaves * k) * kUnit - 32 * half;
-                    first_sees = causal ? left - q_len + 1 : left;
-                    if (__builtin_expect(first_sees < 32, 0)) break;
+                    first_sees = left - fewer;
+                    const bool tail = first_sees < 32;
                     Half x;
-                    read_half(x, slot, half, lane);
+                    read_keys(x, slot, half, lane);
+                    if (__builtin_expect(tail, 0)) end_half<DT>(x, left, lane);
                     uint32_t past = past_half(x.vs[0]) | past_half(x.vs[1]);
                     if constexpr (DT == CK_DTYPE_F16) past |= past_half(x.ks | (kMidScales & 0xffff0000));
                     f32x4 sc[NB][2];
                     half_scores<DT == CK_DTYPE_F16, DT, NB>(sc, x, q);
+                    read_values(x, slot, half, lane);
+                    __builtin_amdgcn_sched_barrier(0);
                     if (__builtin_expect(__builtin_amdgcn_ballot_w64(past != 0) != 0, 0)) break;
+                    if (__builtin_expect(tail, 0)) hide_scores<NB>(sc, lane, left, first_sees, row0, group);
                     bool moves = false;
 #pragma unroll
-                    for (int i = 0; i < NB; ++i) moves |= largest(sc[i]) * scale_log2 > m[i] + kSlack;
+                    for (int i = 0; i < NB; ++i) moves |= !(fmaf(largest(sc[i]), scale_log2, -m[i]) <= kSlack + kBias);  // NaN too
                     if (__builtin_expect(__builtin_amdgcn_ballot_w64(moves) != 0, 0)) {
                         if (!fresh) break;
+                        bool none = false;
 #pragma unroll
-                        for (int i = 0; i < NB; ++i)  // nothing to scale yet
-                            m[i] = over_groups(largest(sc[i]), [](float x, float y) { return fmaxf(x, y); }) * scale_log2;
+                        for (int i = 0; i < NB; ++i) {  // nothing to scale yet
+                            m[i] = over_groups(largest(sc[i]), [](float x, float y) { return fmaxf(x, y); }) * scale_log2 - kBias;
+                            none |= !(m[i] > -INFINITY);
+                        }
+                        if (__builtin_expect(__builtin_amdgcn_ballot_w64(none) != 0, 0)) break;
                     }
                     fresh = false;
                     half_values<true, 0, NB, NB>(o, l, m, x, sc, scale_log2);
-                    half ^= 1;
+                    half = left > 32 ? half ^ 1 : 0;  // the second holds nothing
                     if (half == 0 && ++k == n) break;
                 }
                 if (k == n) break;
                 fresh = false;
                 any_half<DT, NB>(o, m, l, bad, q, slot, half, scale_log2, lane, left, first_sees, row0, group);
-                half ^= 1;
+                half = left > 32 ? half ^ 1 : 0;
                 if (half == 0 && ++k == n) break;
             }
         }
@@ -1098,7 +1174,6 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
                 }
             }
             sum = over_groups(sum, [](float x, float y) { return x + y; });
-            const float ref = top - Form<DT, NB>::kBias;
             const bool whole = !before && !after && !a->merge;
             const int at = 16 * i + n16, r = kTileRows * tile + at;
             if (r < a->rows) {
@@ -1111,7 +1186,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
                     for (int d = 0; d < 4; ++d)
                         *reinterpret_cast<uint2 *>(a->out + row * kD + 32 * g + 8 * d + k0) =
                             make_uint2(E::pack2(y[0][d] * inv, y[1][d] * inv), E::pack2(y[2][d] * inv, y[3][d] * inv));
-                    if (g == 0 && k0 == 0) a->lse[row] = sum == 0.f ? -INFINITY : (ref + __log2f(sum)) * kLn2;
+                    if (g == 0 && k0 == 0) a->lse[row] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * kLn2;
                 } else {
                     const int slot_rows = min(kTileRows, a->rows);
                     const int64_t slot = part_slot(before, after, share, a->waves, item) * a->tiles + tile;
@@ -1119,7 +1194,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
 #pragma unroll
                     for (int d = 0; d < 4; ++d)
                         *reinterpret_cast<f32x4 *>(to + (2 * d + (wave & 1)) * slot_rows * 16) = f32x4{y[0][d], y[1][d], y[2][d], y[3][d]};
-                    if (g == 0 && k0 == 0) a->part_ml[slot * slot_rows + at] = make_float2(ref, sum);
+                    if (g == 0 && k0 == 0) a->part_ml[slot * slot_rows + at] = make_float2(top, sum);
                 }
             }
         }
