@@ -789,7 +789,6 @@ template <bool HALF, int DT, int NB>
 __device__ __forceinline__ void half_scores(f32x4 (&sc)[NB][2], const Half &x, const CK_LDS char *q) {
 #pragma unroll
     for (int i = 0; i < NB; ++i) sc[i][0] = sc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const float f[2] = {scale_of<0>(x.ks), scale_of<1>(x.ks)};
     // the query's operands of the next dims come while these are multiplied; as two terms there are no registers for it
     constexpr int kAhead = DT != CK_DTYPE_F16 || HALF ? 1 : 0;
     u32x4 y[1 + kAhead][NB];
@@ -798,6 +797,7 @@ __device__ __forceinline__ void half_scores(f32x4 (&sc)[NB][2], const Half &x, c
         for (int i = 0; i < NB; ++i) y[c & kAhead][i] = *reinterpret_cast<const CK_LDS u32x4 *>(q + (4 * i + c) * 1024);
     };
     if (kAhead) read_q(0);
+    const float f[2] = {scale_of<0>(x.ks), scale_of<1>(x.ks)};
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         if (c + kAhead < 4) read_q(c + kAhead);
@@ -862,7 +862,7 @@ __device__ __forceinline__ void half_values(f32x4 (&o)[NB][8], float (&l)[NB], c
             }
         }
         l[i] += sum[0] + sum[1];
-        if (NB > 2) __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_sched_barrier(0);
     }
     float f[8];
 #pragma unroll
