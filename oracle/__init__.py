@@ -20,6 +20,8 @@ Modules and the reference code each follows (paths relative to the reference roo
 * ``gemm``      -- gate_up GEMM with the f3 epilogue modes
                    (``ascend-kernel/csrc/ops/f3_floor/op_kernel/kernel_f3_floor.cpp:150-308``,
                    ``.../f3_floor/design.md:94-111``).
+* ``latent``, ``kv4`` -- latent attention and the 4-bit K/V cache in 64 bits (torch), which have no
+                   counterpart in the reference, with bounds of the kernels' documented roundings.
 * ``inputs``    -- seeded input generators (``fa_fp32_ref.py:30-61``,
                    ``lse_merge_cases.py:32-42``) extended with permuted block tables.
 

@@ -26,6 +26,13 @@ reference's custom ops under ``torch.ops.npu`` (the loader of
   shares a prefix, and ``torch.ops.npu.latent_prefill(query, key, key_rope, value, actual_q_seqlens,
   actual_kv_seqlens, scale, causal=True) -> (out [T,H,128], lse fp32 [T*H])`` takes prompts with the
   keys and values of each head laid out.
+* a K/V cache in 4 bits (uint8 pool [blocks, KVH, abi.KV4_PAGE_BYTES], pages of 128 tokens, bf16 or fp16
+  outside): ``torch.ops.npu.kv4_cache_write(key, value, slots, cache)`` quantises tokens into it,
+  ``torch.ops.npu.kv4_cache_read(cache, slots, dtype=None) -> (key, value)`` gives them back,
+  ``torch.ops.npu.kv4_decode(query, cache, block_table, actual_kv_seqlens, scale, q_seqlen_value=1)
+  -> (out [T,H,128], lse fp32 [T*H])`` attends over it and ``torch.ops.npu.kv4_cascade_decode(query,
+  prefix_cache, prefix_block_table, prefix_kv_seqlens, suffix_cache, suffix_block_table, suffix_kv_seqlens,
+  scale) -> (out, lse)`` does for a batch that shares a prefix.
 
 ``cascade_amd.gate`` holds the cascade-vs-full decision harness.
 

@@ -741,9 +741,9 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(std::conditiona
 // 64 products and 271 vector instructions each (codes 64 and their permutations 32, exponentials 32, their arguments,
 // sums and conversions 84); these bound it, at 950 TFLOP/s over a long prefix, and the start and the joint where a
 // workgroup has few units. Where a half's last tokens are hidden, only scores and scales are changed in the loop; a half
-// that holds nothing is passed over (two such halves of 16001 tokens cost 6 us of 109 outside it).
+// that holds nothing is passed over (the one and the other cost 16001 tokens 3 us of 106 outside it).
 // The shares of the list are workgroups', neighbours on one XCD, so that the row tiles of a share meet in its L2.
-// Kernel and fold, us a call: 117 x 64 heads on 16001 tokens and suffixes (fp16) 102, 64 x 32 on 8192 39.
+// us a call with the fold: 117 x 64 heads on 16001 tokens and suffixes (fp16) 99, 64 x 32 on 8192 38.
 constexpr int kWideThreads = 512, kWideWaves = kWideThreads / 64;
 constexpr int kWideQ = kWideWaves * 2 * kUnitBytes;  // [NB][4] operands of 1 KB, behind the waves' buffers
 constexpr int kWideStarts = kWideQ + 4 * 4 * 1024;
