@@ -241,7 +241,7 @@ def test_many_requests(q_len, heads, kv_heads, batch):
     _check_decode(q[rows], pool, table[some], [lens[b] for b in some], SCALE, q_len, part)
 
 
-@pytest.mark.parametrize("heads,kv_heads,batch", [(40, 2, 700), (20, 1, 3), (64, 1, 40), (33, 3, 2), (16, 1, 600)])
+@pytest.mark.parametrize("heads,kv_heads,batch", [(40, 2, 700), (20, 1, 3), (64, 1, 40), (33, 3, 2), (16, 1, 600), (48, 6, 48), (40, 20, 90)])
 def test_cascade_of_other_groups(heads, kv_heads, batch):
     """Suffixes of more than 16 rows have a launch of their own; and many suffixes."""
     g = _gen(10)

@@ -288,12 +288,15 @@ def header(tmp_path_factory):
     src = d / "kv4_map.cpp"
     src.write_text("""#include "kv4_map.h"
 using namespace ck::kv4;
-extern "C" int shares(int w, int waves, int *lo) {
-    const Cut c = list_cut(w, waves);
-    for (int k = 0; k <= c.chunks; ++k) lo[k] = cut_lo(c, k);
-    return c.chunks;
+extern "C" int shares(int w, int waves, int least, int each, int pieces, int *lo) {
+    const Shares s = list_shares(w, waves, least, each, pieces);
+    for (int k = 0; k <= s.count; ++k) lo[k] = share_lo(s, k);
+    return s.count;
 }
-extern "C" int owner(int w, int waves, int x) { return cut_chunk(list_cut(w, waves), x); }
+extern "C" void range(int w, int waves, int least, int each, int pieces, int h, int u, int n, int *out) {
+    const ShareRange r = shares_of(list_shares(w, waves, least, each, pieces), h, u, n);
+    out[0] = r.first, out[1] = r.count;
+}
 extern "C" long long slot(int before, int after, int wave, int waves, int item) { return part_slot(before, after, wave, waves, item); }
 """)
     lib = d / "kv4_map.so"
@@ -304,22 +307,31 @@ extern "C" long long slot(int before, int after, int wave, int waves, int item) 
 
 
 @pytest.mark.parametrize("merge", [False, True])
-@pytest.mark.parametrize("waves", [1, 3, 85, 256, 2048])
-@pytest.mark.parametrize("units", [[1], [0, 0, 7], [5, 0, 1, 300, 2], [1] * 400, [9000], [64, 64, 64]])
-def test_parts_of_the_list(header, units, waves, merge):
-    """The waves' shares, walked as the kernels walk them: every place once, a slot for one part only and within the
-    workspace, and the parts that the fold looks for are those that were left."""
+@pytest.mark.parametrize("least", [1, 4])
+@pytest.mark.parametrize("waves", [1, 3, 17, 85, 256, 2048])
+@pytest.mark.parametrize("units", [[1], [3], [251], [0, 0, 7], [5, 0, 1, 300, 2], [1] * 400, [9000], [64, 64, 64], [0]])
+def test_parts_of_the_list(header, units, waves, least, merge):
+    """The shares, walked as the kernels walk them: every place once, a slot for one part only and within the
+    workspace, and the parts that the fold looks for are those that were left. Of one request's list an item's
+    shares may be its own."""
     kv_heads = 3
     w = sum(units) * kv_heads
+    pieces = waves // kv_heads if least > 1 and len(units) == 1 else 0
+    args = (w, waves, least, units[0], pieces)
     lo = (ctypes.c_int * (waves + 1))()
-    n = header.shares(w, waves, lo)
+    n = header.shares(*args, lo)
     lo = list(lo)[:n + 1]
-    assert n == min(w, waves) and (w == 0 or (lo[0] == 0 and lo[-1] == w and min(np.diff(lo)) > 0))
+    assert 0 <= n <= waves and (n == 0) == (w == 0)
+    assert w == 0 or (lo[0] == 0 and lo[-1] == w and min(np.diff(lo)) > 0)
+    if pieces and w:  # cut at the items, unless that makes shares much longer
+        assert all(x in lo for x in range(0, w, units[0])) or max(np.diff(lo)) + 8 < -(-units[0] // pieces)
     left, at, item = {}, 0, 0
     for each in units:
         for h in range(kv_heads):
             if each:
-                c0, c1 = header.owner(w, waves, at), header.owner(w, waves, at + each - 1)
+                out = (ctypes.c_int * 2)()
+                header.range(*args, h if len(units) == 1 else 0, at, each, out)
+                c0, c1 = out[0], out[0] + out[1] - 1
                 assert lo[c0] <= at < lo[c0 + 1] and lo[c1] <= at + each - 1 < lo[c1 + 1]
                 for k in range(c0, c1 + 1):  # what wave k has of the item
                     before, after = int(lo[k] > at), int(lo[k + 1] < at + each)

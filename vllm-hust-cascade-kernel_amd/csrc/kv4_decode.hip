@@ -67,7 +67,8 @@ struct DecodeArgs {
     int group;  // query heads per kv head
     int rows;   // q_len * group: of an item
     int tiles;  // row tiles of an item
-    int waves;  // shares of the list (waves', or with many rows workgroups'), per row tile
+    int waves;  // at most so many shares of the list (waves', or with many rows workgroups'), per row tile
+    int pieces;  // many rows of one request: at most so many shares of a kv head, or 0
     int causal;
     int merge;  // every part goes to the workspace
     float scale_log2;
@@ -77,6 +78,7 @@ struct DecodeArgs {
     float *part_o;
     float2 *part_ml;  // [slot][tile][tile's rows]: reference point (log2), sum of p
     int32_t *sums;    // [batch + 1]: units before each request (of one kv head)
+    Shares *shares;   // how the list is cut, behind them; both for the fold
 };
 
 // The arguments, read where they are used: held in scalar registers throughout they would spill.
@@ -571,9 +573,10 @@ __device__ __forceinline__ void decode_share(const KernArgs args, const L &list,
     constexpr int kRows = 16 * NB;
     constexpr bool kQAhead = NB == 1;  // the next item's queries are loaded ahead
     const int total = list.total;
-    const Cut cut = list_cut(total * a->kv_heads, a->waves);
-    if (w >= cut.chunks) return;
-    const int lo = scalar(cut_lo(cut, w)), hi = scalar(cut_lo(cut, w + 1));
+    const Shares cut = list_shares(total * a->kv_heads, a->waves, 1, 0, 0);
+    if (w >= cut.count) return;
+    if (w == 0 && lane == 0) *a->shares = cut;
+    const int lo = scalar(share_lo(cut, w)), hi = scalar(share_lo(cut, w + 1));
     const int slot_rows = min(kRows, a->rows);
 
     Rows<DT, NB> s;
@@ -745,6 +748,9 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(std::conditiona
 // The shares of the list are workgroups', neighbours on one XCD, so that the row tiles of a share meet in its L2.
 // us a call with the fold: 117 x 64 heads on 16001 tokens and suffixes (fp16) 99, 64 x 32 on 8192 38.
 constexpr int kWideThreads = 512, kWideWaves = kWideThreads / 64;
+// Units that a share has at least: fewer shares leave fewer parts. us with 1 / 2 / 4 / 8: 16 x 32 heads on 2048 tokens 25.7 /
+// 23.3 / 22.5 / 24.2, 40 x 40 (4 kv heads) on 2048 28.7 / 28.7 / 25.1 / 25.9, 64 x 32 on 1000 26.4 / 26.4 / 25.8 / 27.2.
+constexpr int kWideLeast = 4;
 constexpr int kWideQ = kWideWaves * 2 * kUnitBytes;  // [NB][4] operands of 1 KB, behind the waves' buffers
 constexpr int kWideStarts = kWideQ + 4 * 4 * 1024;
 constexpr int kWideLds = kWideStarts + (2 * kWideThreads + kWideWaves) * 4;
@@ -995,9 +1001,10 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
     if constexpr (PAIR) own_total = List<kWideThreads, false>(args + 1, starts, len0, scan, tid).total;
     const int block = scalar((int)xcd_remap(blockIdx.x, gridDim.x));
     const int share = scalar(block / a->tiles), tile = block - share * a->tiles;
-    const Cut cut = list_cut(list.total * a->kv_heads, a->waves);
-    int cur = share < cut.chunks ? scalar(cut_lo(cut, share)) : 0;
-    const int hi = share < cut.chunks ? scalar(cut_lo(cut, share + 1)) : 0;
+    const Shares cut = list_shares(list.total * a->kv_heads, a->waves, kWideLeast, list.total, a->pieces);
+    if (block == 0 && tid == 0) *a->shares = cut;
+    int cur = share < cut.count ? scalar(share_lo(cut, share)) : 0;
+    const int hi = share < cut.count ? scalar(share_lo(cut, share + 1)) : 0;
     const int row0 = kTileRows * tile;
     CK_LDS char *buffer = smem + wave * 2 * kUnitBytes;
 
@@ -1211,7 +1218,8 @@ struct FoldSide {
     const float *part_o;
     const float2 *part_ml;
     const int32_t *sums;
-    int batch, waves, tiles, tile_rows, slot_rows;
+    const Shares *shares;
+    int waves, tiles, tile_rows, slot_rows;
 };
 struct FoldArgs {
     FoldSide own, prefix;
@@ -1232,7 +1240,8 @@ struct Parts {
 };
 __device__ __forceinline__ Parts parts_of(const FoldSide &f, int kv_heads, int b, int h, int r) {
     Parts p;
-    const int before = f.sums[b], each = f.sums[b + 1] - before, total = f.sums[f.batch];
+    const int before = f.sums[b], each = f.sums[b + 1] - before;
+    const Shares cut = *f.shares;
     const int tile = r / f.tile_rows, at = r - tile * f.tile_rows;
     p.item = b * kv_heads + h;
     p.waves = f.waves;
@@ -1242,10 +1251,9 @@ __device__ __forceinline__ Parts parts_of(const FoldSide &f, int kv_heads, int b
     p.ml = f.part_ml + ((int64_t)tile * f.slot_rows + at);
     p.c0 = p.count = 0;
     if (each > 0) {
-        const Cut cut = list_cut(total * kv_heads, f.waves);
-        const int u = before * kv_heads + h * each;
-        p.c0 = cut_chunk(cut, u);
-        p.count = cut_chunk(cut, u + each - 1) - p.c0 + 1;
+        const ShareRange r = shares_of(cut, h, before * kv_heads + h * each, each);
+        p.c0 = r.first;
+        p.count = r.count;
     }
     return p;
 }
@@ -1359,7 +1367,7 @@ int plan_side(int64_t batch, int64_t rows, int64_t kv_heads, int64_t kv_cap, boo
     p->slot_rows = rows < p->tile_rows ? rows : p->tile_rows;
     p->slots = (2 * p->waves + (merge ? batch * kv_heads : 0)) * p->tiles;
     p->off_sums = at;
-    p->off_ml = p->off_sums + pad256((batch + 1) * 4);
+    p->off_ml = p->off_sums + pad256((batch + 1) * 4 + (int64_t)sizeof(Shares));
     p->off_o = p->off_ml + pad256(p->slots * p->slot_rows * 8);
     p->end = p->off_o + p->slots * p->slot_rows * kD * 4;
     return CK_OK;
@@ -1446,7 +1454,7 @@ int check_pool(const Pool &p) {
     return aligned_to(p.cache, 16) && aligned_to(p.bt, 4) && aligned_to(p.lens, 8) ? CK_OK : CK_E_INVALID_ARG;
 }
 
-void fill(DecodeArgs *a, FoldSide *f, const Pool &pool, const Side &p, int64_t batch, char *ws) {
+void fill(DecodeArgs *a, FoldSide *f, const Pool &pool, const Side &p, int64_t batch, int64_t kv_heads, char *ws) {
     a->cache = static_cast<const uint8_t *>(pool.cache);
     a->bt = pool.bt;
     a->lens = pool.lens;
@@ -1459,7 +1467,9 @@ void fill(DecodeArgs *a, FoldSide *f, const Pool &pool, const Side &p, int64_t b
     a->part_o = reinterpret_cast<float *>(ws + p.off_o);
     a->part_ml = reinterpret_cast<float2 *>(ws + p.off_ml);
     a->sums = reinterpret_cast<int32_t *>(ws + p.off_sums);
-    *f = FoldSide{a->part_o, a->part_ml, a->sums, a->batch, a->waves, a->tiles, (int)p.tile_rows, (int)p.slot_rows};
+    a->shares = reinterpret_cast<Shares *>(a->sums + batch + 1);
+    a->pieces = p.wide && batch == 1 ? (int)(p.waves / kv_heads) : 0;
+    *f = FoldSide{a->part_o, a->part_ml, a->sums, a->shares, a->waves, a->tiles, (int)p.tile_rows, (int)p.slot_rows};
 }
 
 int run(const void *q, const Pool &pool, const Pool *prefix, int64_t batch, int64_t q_len, int64_t heads,
@@ -1494,10 +1504,10 @@ int run(const void *q, const Pool &pool, const Pool *prefix, int64_t batch, int6
     b = a;
     a.q_len = (int)q_len;
     a.causal = q_len > 1;
-    fill(&a, &f.own, pool, p.own, batch, ws);
+    fill(&a, &f.own, pool, p.own, batch, kv_heads, ws);
     if (prefix) {  // one request, the batch's tokens in it, none hidden from another
         b.q_len = (int)batch;
-        fill(&b, &f.prefix, *prefix, p.prefix, 1, ws);
+        fill(&b, &f.prefix, *prefix, p.prefix, 1, kv_heads, ws);
     }
     f.q_len = (int)q_len;
     f.heads = a.heads;
