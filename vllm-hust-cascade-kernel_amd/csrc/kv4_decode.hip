@@ -13,8 +13,8 @@
 //   tokens 8 g .. + 7; two conversions give (token, dim pair) words, two byte permutations turn them to (dim, token
 //   pair). P is in its operand's place as it leaves the scores. The pool's order is that of these operands, so that a
 //   lane loads 16 bytes at a time and nothing is exchanged.
-// * The softmax's reference point m of a row moves only when a score passes it by 2^kSlack (any point gives the
-//   same result), so that O is hardly ever rescaled.
+// * The softmax's reference point m of a row moves only when a score passes the one it was set by by 2^kSlack (any
+//   point gives the same result), so that O is hardly ever rescaled.
 // * The units (64 tokens, 8704 bytes that lie together) of all requests and kv heads form one list, cut evenly
 //   over a grid that fills the chip once, so ragged lengths balance. An item (request and kv head) inside one share is
 //   written as it is; parts of a cut one go to the workspace, not normalised, and kv4_combine_kernel folds them.
@@ -1350,6 +1350,8 @@ struct Side {
 int plan_side(int64_t batch, int64_t rows, int64_t kv_heads, int64_t kv_cap, bool merge, int64_t at, int64_t waves, Side *p) {
     p->rows = rows;
     p->wide = rows > 32;
+    // 16 rows in the form for 16 / for 32, us a call: one request of 1300 tokens (8 kv heads) 10.1 / 10.7, 24 of 1000 20.0 /
+    // 21.9, 64 of 4000 58.7 / 67.3; the form for 32 against that for 64 is at the top
     p->blocks = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     p->tile_rows = 16 * p->blocks;
     p->tiles = ceil_div(rows, p->tile_rows);
