@@ -482,7 +482,8 @@ __device__ __forceinline__ uint32_t first_bytes(uint32_t w, int n, uint32_t rest
 // The values' scales of a half unit that not every row sees whole (sees and left counted from its first token; x, y those
 // of tokens 8 g .. + 7). Those of tokens from `left` on go, and values that are not numbers would reach rows that
 // do not see them (0 times them is none): their scales become ordinary ones, and rows that do see one are marked.
-// A lane (g, n) has the dims of group g of its rows' O.
+// A lane (g, n) has the dims of group g of its rows' O. A row may see more tokens than the unit has (kUnit stands
+// for no such token).
 template <int NB>
 __device__ __forceinline__ void hide_values(uint32_t &bad, uint32_t &x, uint32_t &y, const int (&sees)[NB], int left, int g) {
     int first_bad = kUnit;
@@ -502,7 +503,7 @@ __device__ __forceinline__ void hide_values(uint32_t &bad, uint32_t &x, uint32_t
     first_bad = (int)over_groups((float)first_bad, [](float x, float y) { return fminf(x, y); });
     first_bad = __shfl(first_bad, 4 * g);
 #pragma unroll
-    for (int i = 0; i < NB; ++i) bad |= first_bad < sees[i] ? 1u << i : 0;
+    for (int i = 0; i < NB; ++i) bad |= first_bad < min(sees[i], kUnit) ? 1u << i : 0;
 }
 
 // One unit. Where tail: tokens from sees[i] on are hidden from row block i's row, those from `left` on
