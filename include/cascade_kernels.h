@@ -445,7 +445,9 @@ int ck_kv4_cache_read(const void *cache, const int64_t *slots, int64_t num_block
  *   lse      fp32 [batch * q_len * num_heads]
  *   workspace  of ck_kv4_decode_plan's bytes for kv_cap = bt_cols * 128, 16-byte aligned
  * Sums and softmax statistics are fp32. P enters the second product within 2^-17 of it up to 16 rows
- * (q_len * num_heads / kv_heads; of a prefix batch * num_heads / kv_heads), within 2^-11 of it above. scale > 0,
+ * (q_len * num_heads / kv_heads; of a prefix batch * num_heads / kv_heads), within 2^-11 of it above. Values may be
+ * as large as ck_kv4_cache_write leaves them (1.5 * 2^127): their mean is finite. Among 32 dims in which some
+ * token's scale is 2^65 and more, values below 2^-78 may count as 0. scale > 0,
  * at most 2.3e38. bt_cols * 128 is at most 2^30, batch and q_len at most 2^24, num_heads at most 2^16;
  * batch * q_len * num_heads stays below 2^24, batch * kv_heads * ceil(bt_cols * 128 / 64) below 2^31.
  * Calls past a limit are refused (CK_E_INVALID_ARG) before anything is launched.

@@ -17,7 +17,7 @@
 //   point gives the same result), so that O is hardly ever rescaled.
 // * The units (64 tokens, 8704 bytes that lie together) of all requests and kv heads form one list, cut evenly
 //   over a grid that fills the chip once, so ragged lengths balance. An item (request and kv head) inside one share is
-//   written as it is; parts of a cut one go to the workspace, not normalised, and kv4_combine_kernel folds them.
+//   written as it is; parts of a cut one go to the workspace, and kv4_combine_kernel folds them.
 // * Up to 32 rows a wave computes alone (kv4_decode_kernel): up to 16 with units in registers, the next one's loads
 //   under way while one is computed; up to 32 with a ring of two units in LDS. More rows take kv4_wide_kernel.
 // * Shared prefix: the batch is one request's rows over the prefix. Where the suffixes have up to 16 rows each, one
@@ -44,6 +44,9 @@ namespace {
 using namespace kv4;
 
 typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
+
+// 1 / x within a step, for weights that are to sum up to 1; of a sum of nothing 0.
+__device__ __forceinline__ float one_over(float x) { return x == 0.f ? 0.f : __builtin_amdgcn_rcpf(x); }
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
@@ -74,7 +77,7 @@ struct DecodeArgs {
     float scale_log2;
     uint16_t *out;
     float *lse;
-    // Parts, not normalised: [slot][tile][8][tile's rows][4 g][4], dims 32 g + 4 j + e
+    // Parts, each the mean over its tokens: [slot][tile][8][tile's rows][4 g][4], dims 32 g + 4 j + e
     float *part_o;
     float2 *part_ml;  // [slot][tile][tile's rows]: reference point (log2), sum of p
     int32_t *sums;    // [batch + 1]: units before each request (of one kv head)
@@ -304,6 +307,7 @@ struct Rows {
     float m[NB];     // the sum's reference point (log2; the same for all g), kBias below a score
     float l[NB];     // this lane's share of the sum
     uint32_t bad;    // bit i: row i sees a value that is not a number in this lane's dims
+    uint32_t far;    // bit d: O's dims 32 d .. + 31 are lowered (the same in all lanes)
 };
 template <int DT, int NB>
 __device__ __forceinline__ void clear(Rows<DT, NB> &s) {
@@ -315,6 +319,7 @@ __device__ __forceinline__ void clear(Rows<DT, NB> &s) {
         s.l[i] = 0.f;
     }
     s.bad = 0;
+    s.far = 0;
 }
 // Gives O what hide_values() has put off.
 template <int NB>
@@ -454,21 +459,51 @@ __device__ __forceinline__ void add_values(Rows<DT, NB> &s, const u32x4 (&v)[4],
     }
 }
 
+// Values up to the largest that are written, 6 * 2^125 = 1.5 * 2^127: their mean is finite, a sum of them need not be. Below a
+// scale of 2^65 (byte kFar) the sum p v of 2^30 tokens, p at most 2^(kSlack + 7) = 2^15, stays below 6 * 2^64 * 2^45 < 2^112.
+// A wave that meets a larger scale in an item holds O of that group of 32 dims times 2^-48 from then on, and lowers
+// the group's scales: 1.5 * 2^(127 - 48 + 45) = 1.5 * 2^124 at most. What goes under, of values below 2^-78, is under 2^-143 of the
+// value that did it. Parts are joined as means, with weights that sum up to 1, by which no sum passes the values.
+constexpr int kFar = 192, kLowered = 48;
+constexpr float kLower = 0x1p-48f, kRaise = 0x1p48f;
+// Nonzero where a scale byte of w is kFar and more.
+__device__ __forceinline__ uint32_t far_bytes(uint32_t w) { return w & (w << 1) & 0x80808080; }
+// The groups of dims in which some lane's tokens have such a scale, the lanes n / 4 each; any: some of this lane's.
+__device__ __forceinline__ uint32_t far_groups(bool any) {
+    const uint64_t b = __builtin_amdgcn_ballot_w64(any);
+    uint32_t x = (uint32_t)(b >> 32) | (uint32_t)b;
+    x |= x >> 16;  // lanes n
+    return ((x & 0xf) != 0 ? 1 : 0) | ((x & 0xf0) != 0 ? 2 : 0) | ((x & 0xf00) != 0 ? 4 : 0) | ((x & 0xf000) != 0 ? 8 : 0);
+}
+// The scales of four tokens in a lowered group (255 stays what it is); a lane (g, n) has those of group n / 4.
+__device__ __forceinline__ uint32_t lowered(uint32_t w) {
+    uint32_t to = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const uint32_t e = (w >> (8 * b)) & 0xff;
+        to |= (e == kBad ? kBad : max(e, (uint32_t)kLowered) - kLowered) << (8 * b);
+    }
+    return to;
+}
+__device__ __forceinline__ bool has_lowered(uint32_t far, int lane) { return (far >> ((lane & 15) >> 2)) & 1; }
+// What a lane's O of group g is to be multiplied by.
+__device__ __forceinline__ float by_group(uint32_t groups, int lane, float by) { return (groups >> (lane >> 4)) & 1 ? by : 1.f; }
+
 // Moves the reference points of rows whose scores pass them by 2^(kSlack + kBias) (most: the lane's largest) to 2^kBias
-// below the largest; no score of these passes them by as much again.
+// below the largest; no score of these passes them by as much again. lower: what else O is multiplied by.
 template <int NB>
-__device__ __forceinline__ void move_points(f32x4 (&o)[NB][8], float (&m)[NB], float (&l)[NB], const float (&most)[NB]) {
+__device__ __forceinline__ void move_points(f32x4 (&o)[NB][8], float (&m)[NB], float (&l)[NB], const float (&most)[NB], float lower) {
     constexpr float kBias = Form<CK_DTYPE_BF16, NB>::kBias;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
         const float all = over_groups(most[i], [](float x, float y) { return fmaxf(x, y); });
         const float to = all > m[i] + (kSlack + kBias) ? all - kBias : m[i];
-        const float by = to == m[i] ? 1.f : exp2_fast(m[i] - to);
+        const float by = to == m[i] ? 1.f : exp2_fast(m[i] - to), o_by = by * lower;
         l[i] *= by;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[i][k][r] *= by;
+            for (int r = 0; r < 4; ++r) o[i][k][r] *= o_by;
         m[i] = to;
     }
 }
@@ -543,17 +578,25 @@ __device__ __forceinline__ void compute(Rows<DT, NB> &s, const U &u, float scale
         hide_values<NB>(s.bad, x[2], x[3], sees2, left - 32, g);
         vs = u32x4{x[0], x[1], x[2], x[3]};
     }
+    const bool half = kHalf && s.far == 0 &&
+                      __builtin_expect(!__builtin_amdgcn_ballot_w64((past_half(vs[0]) | past_half(vs[1]) | past_half(vs[2]) | past_half(vs[3])) != 0), 1);
+    uint32_t more = 0;  // groups of dims to be lowered
+    if (!half) {
+        const bool any = (far_bytes(vs[0]) | far_bytes(vs[1]) | far_bytes(vs[2]) | far_bytes(vs[3])) != 0;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(any) != 0, 0)) more = far_groups(any) & ~s.far;
+    }
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
         float most = max3(sc[i][0][0], sc[i][0][1], sc[i][0][2]);
 #pragma unroll
         for (int e = 3; e < 15; e += 2) most = max3(most, sc[i][e >> 2][e & 3], sc[i][(e + 1) >> 2][(e + 1) & 3]);
         most = fmaxf(most, sc[i][3][3]) * scale_log2;
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > s.m[i] + (kSlack + kBias)) != 0, 0)) {
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > s.m[i] + (kSlack + kBias)) != 0 || more != 0, 0)) {
             const float all = over_groups(most, [](float x, float y) { return fmaxf(x, y); });
             const float m = all > s.m[i] + (kSlack + kBias) ? all - kBias : s.m[i];
-            const float f = m == s.m[i] ? 1.f : exp2_fast(s.m[i] - m);
+            float f = m == s.m[i] ? 1.f : exp2_fast(s.m[i] - m);
             s.l[i] *= f;
+            f *= by_group(more, lane_again(lane), kLower);
 #pragma unroll
             for (int k = 0; k < 8; ++k)
 #pragma unroll
@@ -561,10 +604,17 @@ __device__ __forceinline__ void compute(Rows<DT, NB> &s, const U &u, float scale
             s.m[i] = m;
         }
     }
-    if (kHalf && __builtin_expect(!__builtin_amdgcn_ballot_w64((past_half(vs[0]) | past_half(vs[1]) | past_half(vs[2]) | past_half(vs[3])) != 0), 1))
+    s.far |= more;
+    if (__builtin_expect(half, 1)) {
         add_values<true, 0, NB>(s, v, vs, sc, scale_log2);
-    else
-        add_values<false, 0, NB>(s, v, again(vs), sc, scale_log2);
+    } else {
+        u32x4 x = again(vs);
+        if (__builtin_expect(s.far != 0, 0) && has_lowered(s.far, lane_again(lane))) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) x[w] = lowered(x[w]);
+        }
+        add_values<false, 0, NB>(s, v, x, sc, scale_log2);
+    }
 }
 
 // What a wave makes of its share w of the list; more than one row block: through its ring of two units in LDS.
@@ -625,16 +675,20 @@ __device__ __forceinline__ void decode_share(const KernArgs args, const L &list,
         for (int i = 0; i < NB; ++i) {
             const int r = 16 * i + n16;
             const float l = over_groups(s.l[i], [](float x, float y) { return x + y; }), m = s.m[i];
+            const float inv = (l == 0.f ? 0.f : 1.0f / l) * by_group(s.far, x, kRaise);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s.o[i][k][e] *= inv;
             if (r >= a->rows) continue;
             if (whole) {
                 using E = Elem<DT>;
                 const int64_t row = ((int64_t)b * a->q_len + tok[i]) * a->heads + h * a->group + (r - tok[i] * a->group);
-                const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
                     u32x4 x;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = E::pack2(s.o[i][2 * e][d] * inv, s.o[i][2 * e + 1][d] * inv);
+                    for (int e = 0; e < 4; ++e) x[e] = E::pack2(s.o[i][2 * e][d], s.o[i][2 * e + 1][d]);
                     *reinterpret_cast<u32x4 *>(a->out + row * kD + 32 * g4 + 8 * d) = x;
                 }
                 if (g4 == 0) a->lse[row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
@@ -954,8 +1008,8 @@ __device__ __forceinline__ void end_half(Half &x, int left, int lane) {
 // made as in the usual half where their scales allow it: of random scores 117 x 64 heads on 16001 tokens then take 103 us
 // instead of 115, as each wave moves its points a few times.
 template <int DT, int NB>
-__device__ __forceinline__ void any_half(f32x4 (&o)[NB][8], float (&m)[NB], float (&l)[NB], uint32_t &bad, const CK_LDS char *q,
-                                         const CK_LDS char *slot, int h, float scale_log2, int lane, int left, int first_sees,
+__device__ __forceinline__ void any_half(f32x4 (&o)[NB][8], float (&m)[NB], float (&l)[NB], uint32_t &bad, uint32_t &far,
+                                         const CK_LDS char *q, const CK_LDS char *slot, int h, float scale_log2, int lane, int left, int first_sees,
                                          int row0, int group) {
     Half x;
     read_keys(x, slot, h, lane);
@@ -976,7 +1030,10 @@ __device__ __forceinline__ void any_half(f32x4 (&o)[NB][8], float (&m)[NB], floa
     float most[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) most[i] = largest(sc[i]) * scale_log2;
-    move_points<NB>(o, m, l, most);
+    const uint32_t more = far_groups((far_bytes(x.vs[0]) | far_bytes(x.vs[1])) != 0) & ~far;
+    far |= more;
+    move_points<NB>(o, m, l, most, by_group(more, lane_again(lane), kLower));
+    if (has_lowered(far, lane_again(lane))) x.vs[0] = lowered(x.vs[0]), x.vs[1] = lowered(x.vs[1]);
     static_for<NB>([&](auto i) __attribute__((always_inline)) {
         // a row block at a time, and nothing kept from one for the next: there are no registers for more
         asm volatile("" : "+v"(x.vs[0]), "+v"(x.vs[1]));
@@ -1011,7 +1068,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
 
     f32x4 o[NB][8];
     float m[NB], l[NB];
-    uint32_t bad;
+    uint32_t bad, far;
     while (cur < hi) {
         a = args_again(args);
         const Found f = list.find_of_wave(a, cur, lane);
@@ -1031,7 +1088,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
             m[i] = -INFINITY;
             l[i] = 0.f;
         }
-        bad = 0;
+        bad = far = 0;
         bool fresh = true;  // nothing has been added to O
         // The first unit, and the query's operands, some of each wave. Units of this wave: c0 + 8 k, lane k has the
         // address.
@@ -1088,7 +1145,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
                     Half x;
                     read_keys(x, slot, half, lane);
                     if (__builtin_expect(tail, 0)) end_half<DT>(x, left, lane);
-                    uint32_t past = past_half(x.vs[0]) | past_half(x.vs[1]);
+                    uint32_t past = past_half(x.vs[0]) | past_half(x.vs[1]) | far;
                     if constexpr (DT == CK_DTYPE_F16) past |= past_half(x.ks | (kMidScales & 0xffff0000));
                     f32x4 sc[NB][2];
                     half_scores<DT == CK_DTYPE_F16, DT, NB>(sc, x, q);
@@ -1116,15 +1173,17 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
                 }
                 if (k == n) break;
                 fresh = false;
-                any_half<DT, NB>(o, m, l, bad, q, slot, half, scale_log2, lane, left, first_sees, row0, group);
+                any_half<DT, NB>(o, m, l, bad, far, q, slot, half, scale_log2, lane, left, first_sees, row0, group);
                 half = left > 32 ? half ^ 1 : 0;
                 if (half == 0 && ++k == n) break;
             }
         }
 
         add_bad<NB>(o, bad);
+        if (lane == 0) scan[wave] = (int)far;
 
-        // ---- the waves' parts, joined: waves 4 to 7's into those of 0 to 3; then a wave takes half the dims of a row block
+        // ---- the waves' parts, joined: waves 4 to 7's into those of 0 to 3, means from then on; then a wave takes half the
+        // dims of a row block
         __syncthreads();
         CK_LDS char *part = smem + (wave & (kParts - 1)) * kWidePart + 16 * lane_again(lane);
         auto ml_at = [](int i) { return 4 * 8 * 1024 + 1024 * (i >> 1) + 8 * (i & 1); };
@@ -1139,14 +1198,19 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
         if (wave >= kParts) leave();
         __syncthreads();
         if (wave < kParts) {
+            const float up0 = by_group(far, lane_again(lane), kRaise);
+            const float up1 = by_group((uint32_t)scalar(scan[wave + kParts]), lane_again(lane), kRaise);
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 const f32x2 ml = *reinterpret_cast<const CK_LDS f32x2 *>(part + ml_at(i));
                 const float top = fmaxf(m[i], ml[0]);
-                const float f0 = m[i] == -INFINITY ? 0.f : exp2_fast(m[i] - top);
-                const float f1 = ml[0] == -INFINITY ? 0.f : exp2_fast(ml[0] - top);
-                l[i] = l[i] * f0 + ml[1] * f1;
+                float f0 = m[i] == -INFINITY ? 0.f : exp2_fast(m[i] - top);
+                float f1 = ml[0] == -INFINITY ? 0.f : exp2_fast(ml[0] - top);
+                l[i] = over_groups(l[i] * f0 + ml[1] * f1, [](float x, float y) { return x + y; });
                 m[i] = top;
+                const float inv = one_over(l[i]);
+                f0 *= inv * up0;
+                f1 *= inv * up1;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const f32x4 y = *reinterpret_cast<const CK_LDS f32x4 *>(part + (8 * i + k) * 1024);
@@ -1169,11 +1233,16 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
                 ml[w] = *reinterpret_cast<const CK_LDS f32x2 *>(p + w * kWidePart + ml_at(i));
                 top = fmaxf(top, ml[w][0]);
             }
+#pragma unroll
+            for (int w = 0; w < kParts; ++w) {
+                ml[w][1] *= ml[w][0] == -INFINITY ? 0.f : exp2_fast(ml[w][0] - top);
+                sum += ml[w][1];
+            }
+            const float inv = one_over(sum);
             f32x4 y[4];
 #pragma unroll
             for (int w = 0; w < kParts; ++w) {
-                const float f = ml[w][0] == -INFINITY ? 0.f : exp2_fast(ml[w][0] - top);
-                sum = fmaf(ml[w][1], f, sum);
+                const float f = ml[w][1] * inv;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const f32x4 z = *reinterpret_cast<const CK_LDS f32x4 *>(p + w * kWidePart + (8 * i + k0 + k) * 1024);
@@ -1181,7 +1250,6 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
                     for (int r = 0; r < 4; ++r) y[k][r] = w ? fmaf(z[r], f, y[k][r]) : z[r] * f;
                 }
             }
-            sum = over_groups(sum, [](float x, float y) { return x + y; });
             const bool whole = !before && !after && !a->merge;
             const int at = 16 * i + n16, r = kTileRows * tile + at;
             if (r < a->rows) {
@@ -1189,11 +1257,10 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
                 if (whole) {
                     const int t = r / a->group;
                     const int64_t row = ((int64_t)b * q_len + t) * a->heads + h * a->group + (r - t * a->group);
-                    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
 #pragma unroll
                     for (int d = 0; d < 4; ++d)
                         *reinterpret_cast<uint2 *>(a->out + row * kD + 32 * g + 8 * d + k0) =
-                            make_uint2(E::pack2(y[0][d] * inv, y[1][d] * inv), E::pack2(y[2][d] * inv, y[3][d] * inv));
+                            make_uint2(E::pack2(y[0][d], y[1][d]), E::pack2(y[2][d], y[3][d]));
                     if (g == 0 && k0 == 0) a->lse[row] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * kLn2;
                 } else {
                     const int slot_rows = min(kTileRows, a->rows);
@@ -1259,7 +1326,8 @@ __device__ __forceinline__ Parts parts_of(const FoldSide &f, int kv_heads, int b
     return p;
 }
 
-// 32 lanes hold a row's dims, lane (j, g) dims 32 g + 4 j .. + 3; PG such groups share its parts.
+// 32 lanes hold a row's dims, lane (j, g) dims 32 g + 4 j .. + 3; PG such groups share its parts. O is the mean over the
+// parts so far, their weights made to sum up to 1 for each batch.
 template <int DT, int PG>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(FoldArgs a) {
     constexpr int kBlockRows = 8 / PG;
@@ -1286,17 +1354,22 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(FoldArgs a) {
 #pragma unroll
                 for (int i = 0; i < kBatch; ++i)
                     if (i0 + i * PG < p.count) top = fmaxf(top, ml[i].x);
-                const float old = m == -INFINITY ? 0.f : exp2_fast(m - top);
-                l *= old;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] *= old;
+                const float old = (m == -INFINITY ? 0.f : exp2_fast(m - top)) * l;
+                l = old;
 #pragma unroll
                 for (int i = 0; i < kBatch; ++i) {
                     if (i0 + i * PG >= p.count) continue;
-                    const float f = ml[i].x == -INFINITY ? 0.f : exp2_fast(ml[i].x - top);
-                    l = fmaf(ml[i].y, f, l);
+                    ml[i].y *= ml[i].x == -INFINITY ? 0.f : exp2_fast(ml[i].x - top);
+                    l += ml[i].y;
+                }
+                const float inv = one_over(l);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = fmaf(po[i][e], f, o[e]);
+                for (int e = 0; e < 4; ++e) o[e] *= old * inv;
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    if (i0 + i * PG >= p.count) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = fmaf(po[i][e], ml[i].y * inv, o[e]);
                 }
                 m = top;
             }
@@ -1317,22 +1390,26 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(FoldArgs a) {
 #pragma unroll
         for (int i = 1; i < PG; ++i) top = fmaxf(top, part_ml[group + i].x);
         l = 0.f;
-        o = f32x4{0.f, 0.f, 0.f, 0.f};
+        float f[PG];
 #pragma unroll
         for (int i = 0; i < PG; ++i) {
             const float2 ml = part_ml[group + i];
-            const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - top);
-            l = fmaf(ml.y, f, l);
+            f[i] = (ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - top)) * ml.y;
+            l += f[i];
+        }
+        const float inv = one_over(l);
+        o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < PG; ++i) {
             const f32x4 x = part[group + i][lane];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f[i] * inv, o[e]);
         }
         m = top;
     }
     if (done) return;
     using E = Elem<DT>;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    const uint2 x = make_uint2(E::pack2(o[0] * inv, o[1] * inv), E::pack2(o[2] * inv, o[3] * inv));
+    const uint2 x = make_uint2(E::pack2(o[0], o[1]), E::pack2(o[2], o[3]));
     *reinterpret_cast<uint2 *>(a.out + (int64_t)row * kD + 32 * g4 + 4 * j) = x;
     if (lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
