@@ -803,9 +803,6 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(std::conditiona
 // The shares of the list are workgroups', neighbours on one XCD, so that the row tiles of a share meet in its L2.
 // us a call with the fold: 117 x 64 heads on 16001 tokens and suffixes (fp16) 99, 64 x 32 on 8192 38.
 constexpr int kWideThreads = 512, kWideWaves = kWideThreads / 64;
-// Units that a share has at least: fewer shares leave fewer parts. us with 1 / 2 / 4 / 8: 16 x 32 heads on 2048 tokens 25.7 /
-// 23.3 / 22.5 / 24.2, 40 x 40 (4 kv heads) on 2048 28.7 / 28.7 / 25.1 / 25.9, 64 x 32 on 1000 26.4 / 26.4 / 25.8 / 27.2.
-constexpr int kWideLeast = 4;
 constexpr int kWideQ = kWideWaves * 2 * kUnitBytes;  // [NB][4] operands of 1 KB, behind the waves' buffers
 constexpr int kWideStarts = kWideQ + 4 * 4 * 1024;
 constexpr int kWideLds = kWideStarts + (2 * kWideThreads + kWideWaves) * 4;
@@ -1059,7 +1056,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv4_wide_kernel(std::conditio
     if constexpr (PAIR) own_total = List<kWideThreads, false>(args + 1, starts, len0, scan, tid).total;
     const int block = scalar((int)xcd_remap(blockIdx.x, gridDim.x));
     const int share = scalar(block / a->tiles), tile = block - share * a->tiles;
-    const Shares cut = list_shares(list.total * a->kv_heads, a->waves, kWideLeast, list.total, a->pieces);
+    const Shares cut = list_shares(list.total * a->kv_heads, a->waves, list_least(a->batch), list.total, a->pieces);
     if (block == 0 && tid == 0) *a->shares = cut;
     int cur = share < cut.count ? scalar(share_lo(cut, share)) : 0;
     const int hi = share < cut.count ? scalar(share_lo(cut, share + 1)) : 0;

@@ -25,6 +25,13 @@ struct Shares {
     int each;   // an item's places, or 0
     int count;  // of all
 };
+// Places that a share of a call with more than 32 rows a kv head holds (`least`). Of one request fewer shares leave fewer parts:
+// us with 1 / 2 / 4 / 8, 16 x 32 heads on 2048 tokens 25.7 / 23.3 / 22.5 / 24.2, 40 x 40 (4 kv heads) on 2048 28.7 / 28.7 / 25.1 /
+// 25.9, 64 x 32 on 1000 26.4 / 26.4 / 25.8 / 27.2. Of several, a share of more places is several items one after another,
+// each with its start and joint: us with 1 / 2 / 4, 5 tokens of 64 heads (8 kv heads), 16 requests of 64 tokens 17.0 / 25.8 / 42.9,
+// 64 of 64 26.7 / 26.8 / 44.3, 4 of 125 to 500 17.2 / 23.8 / 24.4, 64 of 4000 99.0 / 99.0 / 98.7; 4 of 500 17.6 / 17.4 / 17.0.
+CK_HD int list_least(int batch) { return batch == 1 ? 4 : 1; }
+
 CK_HD int longest(const Cut &c) { return c.q + (c.rem > 0 ? 1 : 0); }
 CK_HD Shares list_shares(int w, int waves, int least, int each, int pieces) {
     const int most = w > 0 ? (w - 1) / least + 1 : 0;
