@@ -19,6 +19,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 if HERE not in sys.path:
     sys.path.insert(0, HERE)
+import asm_lanes  # noqa: E402
 import asm_waits  # noqa: E402
 
 REPO = os.path.dirname(HERE)
@@ -109,6 +110,7 @@ def check_assembly(src):
     if src in OWN_ACC_REGISTERS:
         check_acc_registers(asm)
     asm_waits.check(asm)
+    asm_lanes.check(asm)
 
 
 def build_kernels(jobs):
