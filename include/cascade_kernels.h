@@ -445,7 +445,8 @@ int ck_kv4_cache_read(const void *cache, const int64_t *slots, int64_t num_block
  *   lse      fp32 [batch * q_len * num_heads]
  *   workspace  of ck_kv4_decode_plan's bytes for kv_cap = bt_cols * 128, 16-byte aligned
  * Sums and softmax statistics are fp32. P enters the second product within 2^-17 of it up to 16 rows
- * (q_len * num_heads / kv_heads; of a prefix batch * num_heads / kv_heads), within 2^-11 of it above. Values may be
+ * (q_len * num_heads / kv_heads; of a prefix batch * num_heads / kv_heads). Above, it enters within 2^-11 of it and 2^-32 of
+ * the row's largest weight (an fp16 number, whose smallest steps these are; the sum of P has all of it). Values may be
  * as large as ck_kv4_cache_write leaves them (1.5 * 2^127): their mean is finite. Among 32 dims in which some
  * token's scale is 2^65 and more, values below 2^-78 may count as 0. scale > 0,
  * at most 2.3e38. bt_cols * 128 is at most 2^30, batch and q_len at most 2^24, num_heads at most 2^16;

@@ -289,8 +289,9 @@ __device__ __forceinline__ void load_unit(Unit &u, uint64_t at, int lane) {
 // bf16 terms, within 2^-17 of fp32, an fp16 query the first as two bf16 terms, which hold all of it. More row blocks
 // are bound by arithmetic: where a unit's scales lie in [2^-23, 2^8] fp16 holds every value, and P is one fp16
 // number, 2^7 p (fp16's normal range ends at 2^-14; with the largest score at most 2^kSlack past the reference
-// point 2^7 p stays below 65504), half a step off, 2^-11; so does an fp16 query's key. Units of other scales are
-// computed as above. 24 x 3 x 64 heads over 5000 tokens (fp16): 36.7 -> 27.9 us, the units in LDS instead of
+// point 2^7 p stays below 65504), half a step off: 2^-11 of p, and 2^-32 of the row's largest weight (2^7 p is 2^7 there at the
+// least, fp16's smallest steps are 2^-24) however small p is. An fp16 query's keys are fp16 numbers too, exactly. Units of
+// other scales are computed as above. 24 x 3 x 64 heads over 5000 tokens (fp16): 36.7 -> 27.9 us, the units in LDS instead of
 // registers among it.
 template <int DT, int NB>
 struct Form {

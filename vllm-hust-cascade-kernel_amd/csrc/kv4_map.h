@@ -14,7 +14,8 @@ using lat::cut_lo;
 
 // The list holds, request after request and within it kv head after kv head, the units (64 tokens)
 // of each: n units of request b's head h from n * h + kv_heads * (units of the requests before) on.
-// Its w places are cut evenly into at most `waves` shares of some `least` places and more.
+// Its w places are cut evenly into at most `waves` shares, and at most ceil(w / least): of about `least` places and more (of 5
+// places and a least of 4: 3 and 2).
 // pieces > 0: the list is items of `each` places, which may be cut into so many shares each. A share that goes from one
 // item into the next costs about kSpan places (a second start and joint of its parts); where shares that end with the
 // items are not longer than that, they are taken. us without / with: 48 x 48 heads (6 kv heads) on 8000 tokens 43.7 / 36.1,
@@ -25,7 +26,7 @@ struct Shares {
     int each;   // an item's places, or 0
     int count;  // of all
 };
-// Places that a share of a call with more than 32 rows a kv head holds (`least`). Of one request fewer shares leave fewer parts:
+// About how many places a share of a call with more than 32 rows a kv head holds at least. Of one request fewer shares leave fewer parts:
 // us with 1 / 2 / 4 / 8, 16 x 32 heads on 2048 tokens 25.7 / 23.3 / 22.5 / 24.2, 40 x 40 (4 kv heads) on 2048 28.7 / 28.7 / 25.1 /
 // 25.9, 64 x 32 on 1000 26.4 / 26.4 / 25.8 / 27.2. Of several, a share of more places is several items one after another,
 // each with its start and joint: us with 1 / 2 / 4, 5 tokens of 64 heads (8 kv heads), 16 requests of 64 tokens 17.0 / 25.8 / 42.9,
