@@ -258,8 +258,10 @@ __global__ __launch_bounds__(kThreads) void kv4_read8_kernel(ReadArgs a) {
 }
 
 // Rows (tokens times kv heads) from which 16 lanes take eight tokens. us a call, one / eight, of a prompt's slots: 16384 rows
-// write 4.2 / 5.0, read 4.4 / 4.7; 32768 6.1 / 6.2, 6.4 / 5.9; 49152 8.3 / 7.1, 8.5 / 7.1; 131072 20.5 / 15.7,
-// 17.8 / 15.1; 524288 77 / 69, 96 / 77. Slots in no order cost eight more: 49152 12.8 / 14.4, 10.1 / 10.3.
+// write 4.2 / 5.0, read 4.4 / 4.7; 32768 6.1 / 6.2, 6.4 / 5.9; 49152 8.4 / 7.5, 8.5 / 7.0; 131072 20.8 / 16.0,
+// 17.7 / 14.3; 524288 79 / 69, 96 / 77. Slots in no order, which the host cannot tell from a prompt's, cost eight more, of
+// 8 kv heads: 49152 12.7 / 14.4, 10.1 / 10.4; 65536 15.9 / 19.0, 12.9 / 16.1; 131072 30 / 32, 24 / 30; 262144 63 / 65, 46 / 60;
+// 524288 154 / 169, 103 / 120. Calls of so many tokens are prompts; a step's tokens, in no order, are fewer.
 constexpr int64_t kManyRows = 49152;
 constexpr int64_t kMostHeads = 1 << 10, kMostStride = 1 << 28;
 

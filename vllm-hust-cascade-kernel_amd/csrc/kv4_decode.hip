@@ -22,15 +22,16 @@
 //   under way while one is computed; up to 32 with a ring of two units in LDS. More rows take kv4_wide_kernel.
 // * Shared prefix: the batch is one request's rows over the prefix. Where the suffixes have up to 16 rows each, one
 //   launch takes both lists, a wave its share of the prefix and then of the suffixes; one fold for all parts.
-//   us a call, one launch / two: 8 x 32 heads on 2000 + 200 tokens 16.0 / 18.4, 64 x 32 on 8000 + 200 40 / 47,
-//   on 500 + 2000 46 / 51, 256 x 32 on 8000 + 300 78 / 85.
+//   us a call, one launch / two: 8 x 32 heads on 2000 + 200 tokens 16.5 / 18.7, 64 x 32 on 8000 + 200 35.7 / 41.5,
+//   on 500 + 2000 44.6 / 47.9, 256 x 32 on 8000 + 300 73 / 79.
 //
-// Measured (kernel + fold in us; query / kv heads): 64 requests of 2048 to 8192 tokens, 32 / 8, 73 + 5, 4.8 TB/s; 16 of 16384
-// to 65536, 64 / 8, 160 + 7, 5.3 TB/s; 5 of 5000 to 20011, 20 / 20 in fp16, 31 + 5; one of 1300, 32 / 8, 6 + 4, chains of
+// Measured (kernel + fold in us; query / kv heads): 64 requests of 2048 to 8192 tokens, 32 / 8, 72 + 6, 4.9 TB/s; 16 of 16384
+// to 65536, 64 / 8, 160 + 7, 5.3 TB/s; 5 of 5000 to 20011, 20 / 20 in fp16, 32 + 5; one of 1300, 32 / 8, 6 + 4, chains of
 // round trips (lengths, table, unit, fold) and two launches. 24 requests of 1250 to 5000, 3 tokens, 64 / 8 in fp16 (24
-// rows): 28 + 8, 12 of them vector instructions, 25 MB of parts written and read. 17 / 24 / 32 rows in the form for
-// 32 against the one for 64, us a call: 24 requests of 1000 tokens, 8 kv heads, 23 / 24 / 26 against 30 / 30 / 32; 64 of 4000
-// 69 / 74 / 77 against 96 / 97 / 100; one of 16000 25 / 25 / 27 against 27 / 26 / 26.
+// rows): 29 + 8, 12 of them vector instructions, 25 MB of parts written and read. 17 / 24 / 32 rows in the form for
+// 32 against the one for 64, us a call: 24 requests of 1000 tokens, 8 kv heads, 23 / 25 / 26 against 30 / 30 / 32; 64 of 4000
+// 70 / 74 / 78 against 90 / 94 / 97; 4 of 500 11 / 11 / 12 against 16 / 17 / 17. One of 16000 would be sooner in the form for 64, whose
+// shares end with the kv heads: 25 / 26 / 28 against 20 / 20 / 21.
 #include <cmath>
 #include <type_traits>
 
@@ -53,8 +54,8 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kGroups = 512;      // workgroups: two per CU, so two waves a SIMD, as many as the registers allow
 constexpr int kGroupsWide = 256;  // of many rows: one per CU, which its LDS fills
 // Up to how many rows a row's parts are folded by 8, 4 and 2 groups of lanes. us with 8 / 4 / 2 / 1: 32 rows of 21 parts
-// 4.1 / 4.7 / 5.4 / 6.7, 256 of 36 5.0 / 5.2 / 6.9 / 12, 1024 of 17 7.3 / 6.7 / 7.0 / 9.4, 2048 of 10 10.0 / 7.5 / 7.8 / 10.0
-// (of 5: 8.3 / 6.0 / 5.4 / 5.5), 4608 of 11 13.4 / 8.3 / 7.8 / 8.6, 7488 of 6 23 / 16.6 / 11.6 / 9.3.
+// 4.2 / 4.8 / 5.4 / 6.4, 256 of 36 4.6 / 5.3 / 6.6 / 9.6, 1024 of 17 7.6 / 6.8 / 7.3 / 9.5, 2048 of 10 10.0 / 7.1 / 7.4 / 9.2
+// (of 5: 8.9 / 6.7 / 5.5 / 5.4), 4608 of 11 14.3 / 8.9 / 8.2 / 8.3, 7488 of 6 19.8 / 14.6 / 11.7 / 9.0.
 constexpr int kFoldRows[3] = {512, 2048, 6144};
 constexpr float kSlack = 8.f;
 constexpr uint32_t kRsrcFlags = 0x00020000;
@@ -797,12 +798,12 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_decode_kernel(std::conditiona
 // registers); its waves take an item's units in turn, each through a double buffer of its own in LDS, so that
 // nothing holds them together: with a ring that all read, and a barrier for every 4 units, 117 x 64 heads on 16001 tokens
 // took 108 to 118 us. Their parts are joined through LDS, so that few go to memory. A wave works in halves of 32 tokens,
-// 64 products and 271 vector instructions each (codes 64 and their permutations 32, exponentials 32, their arguments,
+// 64 products and 273 vector instructions each (codes 64 and their permutations 32, exponentials 32, their arguments,
 // sums and conversions 84); these bound it, at 950 TFLOP/s over a long prefix, and the start and the joint where a
 // workgroup has few units. Where a half's last tokens are hidden, only scores and scales are changed in the loop; a half
 // that holds nothing is passed over (the one and the other cost 16001 tokens 3 us of 106 outside it).
 // The shares of the list are workgroups', neighbours on one XCD, so that the row tiles of a share meet in its L2.
-// us a call with the fold: 117 x 64 heads on 16001 tokens and suffixes (fp16) 99, 64 x 32 on 8192 38.
+// us a call with the fold: 117 x 64 heads on 16001 tokens and suffixes (fp16) 100, 64 x 32 on 8192 39.
 constexpr int kWideThreads = 512, kWideWaves = kWideThreads / 64;
 constexpr int kWideQ = kWideWaves * 2 * kUnitBytes;  // [NB][4] operands of 1 KB, behind the waves' buffers
 constexpr int kWideStarts = kWideQ + 4 * 4 * 1024;
@@ -1426,8 +1427,8 @@ struct Side {
 int plan_side(int64_t batch, int64_t rows, int64_t kv_heads, int64_t kv_cap, bool merge, int64_t at, int64_t waves, Side *p) {
     p->rows = rows;
     p->wide = rows > 32;
-    // 16 rows in the form for 16 / for 32, us a call: one request of 1300 tokens (8 kv heads) 10.1 / 10.7, 24 of 1000 20.0 /
-    // 21.9, 64 of 4000 58.7 / 67.3; the form for 32 against that for 64 is at the top
+    // 16 rows in the form for 16 / for 32, us a call: one request of 1300 tokens (8 kv heads) 10.3 / 11.0, 24 of 1000 20.0 /
+    // 21.9, 64 of 4000 59.4 / 68.7; the form for 32 against that for 64 is at the top
     p->blocks = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     p->tile_rows = 16 * p->blocks;
     p->tiles = ceil_div(rows, p->tile_rows);

@@ -18,8 +18,8 @@ using lat::cut_lo;
 // places and a least of 4: 3 and 2).
 // pieces > 0: the list is items of `each` places, which may be cut into so many shares each. A share that goes from one
 // item into the next costs about kSpan places (a second start and joint of its parts); where shares that end with the
-// items are not longer than that, they are taken. us without / with: 48 x 48 heads (6 kv heads) on 8000 tokens 43.7 / 36.1,
-// 16 x 32 (8) on 6000 31.1 / 25.1, 117 x 64 on 1000 39 / 31.7, on 16001 100.9 / 99.0.
+// items are not longer than that, they are taken. us without / with: 48 x 48 heads (6 kv heads) on 8000 tokens 42.4 / 36.3,
+// 16 x 32 (8) on 6000 31.6 / 25.9, 117 x 64 on 1000 39.0 / 32.6, on 16001 105.3 / 103.1.
 constexpr int kSpan = 8;
 struct Shares {
     Cut cut;    // of the list, or of an item
@@ -27,8 +27,8 @@ struct Shares {
     int count;  // of all
 };
 // About how many places a share of a call with more than 32 rows a kv head holds at least. Of one request fewer shares leave fewer parts:
-// us with 1 / 2 / 4 / 8, 16 x 32 heads on 2048 tokens 25.7 / 23.3 / 22.5 / 24.2, 40 x 40 (4 kv heads) on 2048 28.7 / 28.7 / 25.1 /
-// 25.9, 64 x 32 on 1000 26.4 / 26.4 / 25.8 / 27.2. Of several, a share of more places is several items one after another,
+// us with 1 / 2 / 4 / 8, 16 x 32 heads on 2048 tokens 26.1 / 24.2 / 23.3 / 25.9, on 512 22.3 / 21.8 / 21.5 / 23.0, 20 x 16 (4 kv
+// heads) on 4000 24.1 / 24.2 / 23.1 / 24.7, 64 x 32 on 1000 26.9 / 27.0 / 27.1 / 27.7. Of several, a share of more places is several items one after another,
 // each with its start and joint: us with 1 / 2 / 4, 5 tokens of 64 heads (8 kv heads), 16 requests of 64 tokens 17.0 / 25.8 / 42.9,
 // 64 of 64 26.7 / 26.8 / 44.3, 4 of 125 to 500 17.2 / 23.8 / 24.4, 64 of 4000 99.0 / 99.0 / 98.7; 4 of 500 17.6 / 17.4 / 17.0.
 CK_HD int list_least(int batch) { return batch == 1 ? 4 : 1; }
