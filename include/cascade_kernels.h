@@ -448,7 +448,7 @@ int ck_kv4_cache_read(const void *cache, const int64_t *slots, int64_t num_block
  * (q_len * num_heads / kv_heads; of a prefix batch * num_heads / kv_heads). Above, it enters within 2^-11 of it and 2^-32 of
  * the row's largest weight (an fp16 number, whose smallest steps these are; the sum of P has all of it). Values may be
  * as large as ck_kv4_cache_write leaves them (1.5 * 2^127): their mean is finite. Among 32 dims in which some
- * token's scale is 2^65 and more, values below 2^-78 may count as 0. scale > 0,
+ * token's scale is 2^65 and more, scales below 2^-79 count as that (values below 2^-77 are off by less than 2^-76). scale > 0,
  * at most 2.3e38. bt_cols * 128 is at most 2^30, batch and q_len at most 2^24, num_heads at most 2^16;
  * batch * q_len * num_heads stays below 2^24, batch * kv_heads * ceil(bt_cols * 128 / 64) below 2^31.
  * Calls past a limit are refused (CK_E_INVALID_ARG) before anything is launched.

@@ -13,18 +13,19 @@ from tests.test_gpu_kv4_edges import FORMS, _check_cascade, _scales
 pytestmark = pytest.mark.gpu
 
 
-def _check_groups(q, k, v, sees, scale, rows, got):
+def _check_groups(q, k, v, sees, scale, rows, got, more=0.0):
     """Rows of a kv head against the definition, 32 dims at a time: what large values may lose (2^-32 of the largest of
-    them) does not widen the bound of the other dims."""
+    them) does not widen the bound of the other dims. more: added to the bound of out."""
     out, lse = got
     if k.shape[0] == 0:
         assert (out == 0).all() and (lse == -math.inf).all()
         return
     for d in range(0, 128, 32):
-        close(out[:, d:d + 32], lse, o4.attend(q, k, v[:, d:d + 32], sees, scale, q.dtype, rows))
+        o, l, b_o, b_l = o4.attend(q, k, v[:, d:d + 32], sees, scale, q.dtype, rows)
+        close(out[:, d:d + 32], lse, (o, l, b_o + more, b_l))
 
 
-def _check_decode_groups(q, pool, table, lens, scale, q_len, got):
+def _check_decode_groups(q, pool, table, lens, scale, q_len, got, more=0.0):
     kv_heads, n = pool.shape[1], q.shape[1] // pool.shape[1]
     q, out, lse = q.view(-1, q_len, kv_heads, n, 128), got[0].view(-1, q_len, kv_heads, n, 128), got[1].view(-1, q_len, kv_heads, n)
     for b, length in enumerate(lens):
@@ -32,7 +33,7 @@ def _check_decode_groups(q, pool, table, lens, scale, q_len, got):
         sees = (length - q_len + 1 + torch.arange(q_len, device=DEV)).repeat_interleave(n)
         for h in range(kv_heads):
             _check_groups(q[b, :, h].reshape(-1, 128), k[:, h], v[:, h], sees, scale, q_len * n,
-                          (out[b, :, h].reshape(-1, 128), lse[b, :, h].reshape(-1)))
+                          (out[b, :, h].reshape(-1, 128), lse[b, :, h].reshape(-1)), more)
 
 
 def _check_cascade_groups(q, ppool, ptable, prefix, pool, table, suffixes, scale, got):
@@ -110,6 +111,24 @@ def test_values_up_to_the_largest(how, q_len, heads, kv_heads):
             for prefix in (4, 3):
                 got = OPS.kv4_cascade_decode(q, a, table[prefix:prefix + 1], _i64([lens[prefix]]), b, table, _i64(lens), SCALE)
                 _check_cascade_groups(q, a, table[prefix:prefix + 1], lens[prefix], b, table, lens, SCALE, got)
+
+
+@pytest.mark.parametrize("q_len,heads,kv_heads", FORMS)
+@pytest.mark.parametrize("first", [0, 40])
+def test_tiny_values_in_the_dims_of_large_ones(first, q_len, heads, kv_heads):
+    """Beside a scale of 2^65 and more those below 2^-79 (byte 48) count as that: a value of at most 6 * 2^-80 is taken as at most
+    6 * 2^-79, so that it, and a mean of such, is off by less than 2^-76. Where a large value's code is 0 a dim holds nothing else."""
+    g = _gen(25)
+    lens = [40, 200, 1000]
+    table, blocks = _tables(g, lens)
+    pool = o4.random_pool(g, blocks, kv_heads, DEV)
+    for u in (0, 8704):
+        at = pool[..., u + 8448:u + 8704].unflatten(-1, (4, 64))
+        some = torch.rand(at.shape, generator=g, device=DEV) < 0.01
+        low = torch.randint(max(8, first), first + 16, at.shape, generator=g, device=DEV, dtype=torch.uint8)
+        at.copy_(torch.where(some, 252, low))
+    q = _normal(g, len(lens) * q_len, heads, 128)
+    _check_decode_groups(q, pool, table, lens, SCALE, q_len, OPS.kv4_decode(q, pool, table, _i64(lens), SCALE, q_len), 2.0 ** -76)
 
 
 @pytest.mark.parametrize("q_len,heads,kv_heads", FORMS)

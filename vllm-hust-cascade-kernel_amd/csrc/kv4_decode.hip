@@ -464,8 +464,9 @@ __device__ __forceinline__ void add_values(Rows<DT, NB> &s, const u32x4 (&v)[4],
 // Values up to the largest that are written, 6 * 2^125 = 1.5 * 2^127: their mean is finite, a sum of them need not be. Below a
 // scale of 2^65 (byte kFar) the sum p v of 2^30 tokens, p at most 2^(kSlack + 7) = 2^15, stays below 6 * 2^64 * 2^45 < 2^112.
 // A wave that meets a larger scale in an item holds O of that group of 32 dims times 2^-48 from then on, and lowers
-// the group's scales: 1.5 * 2^(127 - 48 + 45) = 1.5 * 2^124 at most. What goes under, of values below 2^-78, is under 2^-143 of the
-// value that did it. Parts are joined as means, with weights that sum up to 1, by which no sum passes the values.
+// the group's scales: 1.5 * 2^(127 - 48 + 45) = 1.5 * 2^124 at most. Scale bytes below 48 become 0, which is 2^-127: values of
+// less than 6 * 2^-80 are off by less than 6 * 2^-79, 2^-76. Parts are joined as means, with weights that sum up to 1, by which no
+// sum passes the values.
 constexpr int kFar = 192, kLowered = 48;
 constexpr float kLower = 0x1p-48f, kRaise = 0x1p48f;
 // Nonzero where a scale byte of w is kFar and more.
